@@ -419,6 +419,69 @@ int64_t vmcpde_sytrd_medium_workspace_bytes(int32_t n);
 int vmcpde_sytrd_medium(const double* T, int64_t ldt, int32_t n, double* D, double* E, double* tau, double* V, int64_t ldv, void* workspace,
                         int64_t workspace_bytes, void* stream);
 
+/* ---- layers: the dense layer, layer norm, the global norm -------------------------------------------------------------------- */
+/* What a fit of a wide conditioner is made of, beside the flow kernels (whose networks live in LDS): net.py:53-61 is a chain of dense
+ * layers, var_state.py:45-53 hands out the gradient of a likelihood fit.  Element types of these entry points; every other one is fp64.
+ * Sums, statistics and epilogues are held in fp32 for fp32 and 16-bit elements, in fp64 for fp64.  Row pitches count elements; a row's
+ * elements lie behind each other.  Nothing needs to be aligned beyond its elements. */
+enum { VMCPDE_F64 = 0, VMCPDE_F32 = 1, VMCPDE_F16 = 2, VMCPDE_BF16 = 3 };
+enum { VMCPDE_ACT_NONE = 0, VMCPDE_ACT_TANH = 1, VMCPDE_ACT_GELU = 2 /* z Phi(z), the exact form */, VMCPDE_ACT_SILU = 3 };
+
+/* y = scale * act(x W + b) + r for x [rows][n_in], W [n_in][n_out] (net.py:55-56: the kernel's layout in the flat parameter vector), or
+ * stored [n_out][n_in] with kernel_t != 0.  b, r, slope may be NULL.  slope [rows][n_out] receives act'(x W + b) for the backward pass:
+ * fp16 for both 16-bit types, else the element type.
+ * Backward, with dz = scale * slope * dy (slope NULL: 1):  dx = dz W^T [rows][n_in], dkernel = x^T dz [n_in][n_out] (this order whatever
+ * kernel_t), dbias = sum of dz over the rows; each may be NULL = not wanted, x may be NULL without dkernel, kernel without dx.  The residual's gradient is dy.  dz is rounded
+ * to the element type, in which the matrix pipe takes it; sums are fp32 / fp64.  No atomics: the same call gives the same bits. */
+typedef struct {
+  int32_t dtype, activation, kernel_t, reserved;
+  int64_t rows, n_in, n_out;
+  const void* x;        int64_t ldx;
+  const void* kernel;   int64_t ldk;
+  const void* bias;
+  const void* residual; int64_t ldr;
+  double scale;
+  void* y;              int64_t ldy;
+  void* slope;          /* written by vmcpde_dense, read by vmcpde_dense_backward; row pitch n_out */
+  const void* dy;       int64_t ldd;
+  void* dx; void* dkernel; void* dbias;
+} vmcpde_dense_args;
+int64_t vmcpde_dense_workspace_bytes(const vmcpde_dense_args* args, int32_t backward);   /* -1: the arguments are refused */
+int vmcpde_dense(const vmcpde_dense_args* args, void* workspace, int64_t workspace_bytes, void* stream);
+int vmcpde_dense_backward(const vmcpde_dense_args* args, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Layer norm of the rows of x [rows][cols]: y = (x - mean) * rstd * weight + bias, rstd = 1 / sqrt(variance + eps) (variance over cols, not
+ * cols - 1).  weight, bias may be NULL; they have the element type, or fp32 beside 16-bit elements.  mean, rstd [rows] (fp32, fp64 for fp64)
+ * are written by the forward pass where given and read by the backward pass:  dx, dweight, dbias, each may be NULL = not wanted. */
+typedef struct {
+  int32_t dtype, weight_dtype;
+  int64_t rows, cols;
+  const void* x;  int64_t ldx;
+  const void* weight; const void* bias;
+  double eps;
+  void* y;        int64_t ldy;
+  void* mean; void* rstd;
+  const void* dy; int64_t ldd;
+  void* dx;       /* row pitch cols */
+  void* dweight; void* dbias;
+} vmcpde_norm_args;
+int vmcpde_layer_norm(const vmcpde_norm_args* args, void* stream);
+int64_t vmcpde_layer_norm_backward_workspace_bytes(const vmcpde_norm_args* args);
+int vmcpde_layer_norm_backward(const vmcpde_norm_args* args, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* norm[0] ([dev], fp64) = sqrt of the sum of the squares of all tensors' elements; with clip != 0 also
+ * out_t = in_t * (norm > max_norm ? max_norm / norm : 1) for every tensor (a NaN norm scales by 1, an infinite one by 0).  in == out clips
+ * in place; any other overlap of an `out` with a tensor is refused.  The table is host memory and is read before the call returns. */
+typedef struct {
+  const void* in;
+  void* out;       /* ignored with clip == 0 */
+  int64_t n;
+  int32_t dtype, reserved;
+} vmcpde_tensor;
+int64_t vmcpde_global_norm_workspace_bytes(const vmcpde_tensor* tensors, int32_t count);
+int vmcpde_global_norm(const vmcpde_tensor* tensors, int32_t count, int32_t clip, double max_norm, double* norm, void* workspace,
+                       int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -46,6 +46,20 @@ class EqConsts(C.Structure):
                 ("lam", C.c_double), ("T", C.c_double), ("gamma", C.c_double)]
 
 
+class DenseArgs(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("activation", C.c_int32), ("kernel_t", C.c_int32), ("reserved", C.c_int32),
+                ("rows", C.c_int64), ("n_in", C.c_int64), ("n_out", C.c_int64), ("x", C.c_void_p), ("ldx", C.c_int64),
+                ("kernel", C.c_void_p), ("ldk", C.c_int64), ("bias", C.c_void_p), ("residual", C.c_void_p), ("ldr", C.c_int64),
+                ("scale", C.c_double), ("y", C.c_void_p), ("ldy", C.c_int64), ("slope", C.c_void_p), ("dy", C.c_void_p), ("ldd", C.c_int64),
+                ("dx", C.c_void_p), ("dkernel", C.c_void_p), ("dbias", C.c_void_p)]
+
+
+class NormArgs(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("weight_dtype", C.c_int32), ("rows", C.c_int64), ("cols", C.c_int64), ("x", C.c_void_p), ("ldx", C.c_int64),
+                ("weight", C.c_void_p), ("bias", C.c_void_p), ("eps", C.c_double), ("y", C.c_void_p), ("ldy", C.c_int64), ("mean", C.c_void_p),
+                ("rstd", C.c_void_p), ("dy", C.c_void_p), ("ldd", C.c_int64), ("dx", C.c_void_p), ("dweight", C.c_void_p), ("dbias", C.c_void_p)]
+
+
 _vp, _i32, _i64, _u64, _f64, _int = C.c_void_p, C.c_int32, C.c_int64, C.c_uint64, C.c_double, C.c_int
 
 _PROTOS = {
@@ -126,6 +140,14 @@ _PROTOS = {
     "vmcpde_apply_reflectors": (_int, [_vp, _i64, _vp, _i32, _vp, _i64, _i32, _vp]),
     "vmcpde_sytrd_medium_max_n": (_i32, []),
     "vmcpde_sytrd_medium_workspace_bytes": (_i64, [_i32]),
+    "vmcpde_dense_workspace_bytes": (_i64, [C.POINTER(DenseArgs), _i32]),
+    "vmcpde_dense": (_int, [C.POINTER(DenseArgs), _vp, _i64, _vp]),
+    "vmcpde_dense_backward": (_int, [C.POINTER(DenseArgs), _vp, _i64, _vp]),
+    "vmcpde_layer_norm": (_int, [C.POINTER(NormArgs), _vp]),
+    "vmcpde_layer_norm_backward_workspace_bytes": (_i64, [C.POINTER(NormArgs)]),
+    "vmcpde_layer_norm_backward": (_int, [C.POINTER(NormArgs), _vp, _i64, _vp]),
+    "vmcpde_global_norm_workspace_bytes": (_i64, [_vp, _i32]),
+    "vmcpde_global_norm": (_int, [_vp, _i32, _i32, _f64, _vp, _vp, _i64, _vp]),
     "vmcpde_sytrd_medium": (_int, [_vp, _i64, _i32, _vp, _vp, _vp, _vp, _i64, _vp, _i64, _vp]),
 }
 

@@ -15,8 +15,9 @@ PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 LIBDIR = PKG / "_lib"
 LIB = LIBDIR / "libvmcpde.so"
-SOURCES = ["model.hip", "flow.hip", "sampler.hip", "gram.hip", "gram_i8.hip", "moments.hip", "solve.hip", "eig.hip", "jacobi.hip", "tridiag.hip", "comm.hip"]
-HEADERS = [CSRC / "common.hpp", CSRC / "mfma_tile.hpp", CSRC / "gram_order.hpp", CSRC / "wave_ops.hpp", CSRC / "flow_kernels.inc", PKG.parent / "include" / "vmcpde.h"]
+SOURCES = ["model.hip", "flow.hip", "sampler.hip", "gram.hip", "gram_i8.hip", "moments.hip", "solve.hip", "eig.hip", "jacobi.hip", "tridiag.hip", "comm.hip",
+           "dense.hip", "layer_norm.hip", "global_norm.hip"]
+HEADERS = [CSRC / "common.hpp", CSRC / "mfma_tile.hpp", CSRC / "gram_order.hpp", CSRC / "wave_ops.hpp", CSRC / "layers.hpp", CSRC / "flow_kernels.inc", PKG.parent / "include" / "vmcpde.h"]
 ARCH = "gfx950"
 # per-file flags.  solve.hip: keep MFMA accumulators in VGPRs -- the diagonal-block sweep edits them with VALU instructions between
 # MFMAs, and with the default AGPR form every step pays 40 v_accvgpr moves (measured: the whole factorisation 0.1 ms slower)
@@ -46,7 +47,9 @@ def build(force: bool = False, verbose: bool = False, variant: str = "", extra_f
     lib = LIBDIR / f"libvmcpde_{variant}.so" if variant else LIB
     objs = []
     flags = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}", "-fno-gpu-rdc",
-             "-Wall", "-Wno-unused-function", "-ffp-contract=on", *extra_flags]
+             "-Wall", "-Wno-unused-function", "-ffp-contract=on",
+             "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",       # some packed fp32 forms have given wrong results on this chip
+             *extra_flags]
     for src in SOURCES:
         s = CSRC / src
         o = objdir / (src.replace(".hip", ".o"))

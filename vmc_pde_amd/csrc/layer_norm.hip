@@ -1,0 +1,436 @@
+// Layer norm over the last axis, forward and backward.
+//   mean = <x>, rstd = 1 / sqrt(<(x - mean)^2> + eps), h = (x - mean) rstd, y = h w + b
+//   g = dy w:  dx = rstd (g - <g> - h <g h>),  dw = sum_rows dy h,  db = sum_rows dy
+//
+// Bound by memory.  A row is read once and stays in registers (fp32, fp64 rows in fp64): the mean is taken first and the variance from the
+// deviations, so a row far from zero loses nothing.  16, 64, 256 or 1024 lanes share a row, so that a lane holds at most four 16-byte
+// vectors; longer rows go through the kernels that read them again.  Loads and stores are 16 bytes a lane at any alignment (global memory
+// takes them unaligned; only a row's last, partial vector goes element by element), so odd widths cost one path, not another kernel.
+// The weights' gradients: every workgroup takes every gridDim-th group of rows and adds its columns in registers; the workgroups' sums are
+// added in index order by a second launch -- no atomics, the same bits every time.
+#include "layers.hpp"
+
+using namespace vmcpde;
+
+namespace {
+
+template <typename A> __device__ __forceinline__ A reciprocal_root(A v);
+template <> __device__ __forceinline__ float reciprocal_root(float v) { return 1.0f / sqrtf(v); }
+template <> __device__ __forceinline__ double reciprocal_root(double v) { return 1.0 / sqrt(v); }
+
+// Sums of K values over the LANES lanes that share a row; every lane returns them.  `sh`: K x waves values, one slot a call in a row's turn.
+template <int LANES, int K, typename A>
+__device__ __forceinline__ void row_sum(A (&v)[K], A* sh) {
+  if constexpr (LANES <= 64) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] = group_sum<LANES>(v[k]);
+  } else {
+    constexpr int WAVES = LANES / 64;
+    const int wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      v[k] = group_sum<64>(v[k]);
+      if ((threadIdx.x & 63) == 0) sh[k * WAVES + wave] = v[k];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      v[k] = sh[k * WAVES];
+#pragma unroll
+      for (int w = 1; w < WAVES; ++w) v[k] += sh[k * WAVES + w];
+    }
+  }
+}
+
+template <typename T, typename W, int LANES, int ITER, int THREADS>
+__global__ __launch_bounds__(THREADS) void norm_forward_kernel(const T* __restrict__ x, int64_t ldx, const W* __restrict__ weight, const W* __restrict__ bias,
+                                                               typename Wide<T>::type eps, int64_t rows, int64_t cols, T* __restrict__ y, int64_t ldy,
+                                                               typename Wide<T>::type* __restrict__ mean_out, typename Wide<T>::type* __restrict__ rstd_out) {
+  typedef typename Wide<T>::type A;
+  constexpr int V = vec_of<T>(), GROUPS = THREADS / LANES;
+  __shared__ A sh[2][THREADS / 64];
+  const int lane = threadIdx.x % LANES;
+  const int64_t row = (int64_t)blockIdx.x * GROUPS + threadIdx.x / LANES;
+  const bool live = row < rows;              // (a whole group of lanes; the sums below need every lane of a wave)
+  const T* xr = x + (live ? row : 0) * ldx;
+  A v[ITER][V];
+  A s[1] = {0};
+#pragma unroll
+  for (int i = 0; i < ITER; ++i) {
+    load_vec<T, V>(xr, ((int64_t)i * LANES + lane) * V, cols, v[i]);
+#pragma unroll
+    for (int k = 0; k < V; ++k) s[0] += v[i][k];
+  }
+  row_sum<LANES>(s, sh[0]);
+  const A mean = s[0] / (A)cols;
+  A q[1] = {0};
+#pragma unroll
+  for (int i = 0; i < ITER; ++i)
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      v[i][k] -= mean;
+      if (((int64_t)i * LANES + lane) * V + k < cols) q[0] += v[i][k] * v[i][k];
+    }
+  row_sum<LANES>(q, sh[1]);
+  const A rstd = reciprocal_root<A>(q[0] / (A)cols + eps);
+  if (!live) return;
+  if (lane == 0 && mean_out) {
+    mean_out[row] = mean;
+    rstd_out[row] = rstd;
+  }
+  T* yr = y + row * ldy;
+#pragma unroll
+  for (int i = 0; i < ITER; ++i) {
+    const int64_t col = ((int64_t)i * LANES + lane) * V;
+    if (col < cols) {
+      A w[V], b[V];
+      if (weight) load_vec<W, V>(weight, col, cols, w);
+      if (bias) load_vec<W, V>(bias, col, cols, b);
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        A h = v[i][k] * rstd;
+        if (weight) h *= w[k];
+        if (bias) h += b[k];
+        v[i][k] = h;
+      }
+      store_vec<T, V>(yr, col, cols, v[i]);
+    }
+  }
+}
+
+// rows that no 1024 lanes hold: read three times (the second and third time from the caches)
+template <typename T, typename W>
+__global__ __launch_bounds__(1024) void norm_forward_wide_kernel(const T* __restrict__ x, int64_t ldx, const W* __restrict__ weight, const W* __restrict__ bias,
+                                                                 typename Wide<T>::type eps, int64_t cols, T* __restrict__ y, int64_t ldy,
+                                                                 typename Wide<T>::type* __restrict__ mean_out, typename Wide<T>::type* __restrict__ rstd_out) {
+  typedef typename Wide<T>::type A;
+  constexpr int V = vec_of<T>();
+  __shared__ A sh[2][16];
+  const int64_t row = blockIdx.x;
+  const T* xr = x + row * ldx;
+  A s[1] = {0}, q[1] = {0}, v[V];
+  for (int64_t c = threadIdx.x * V; c < cols; c += 1024 * V) {
+    load_vec<T, V>(xr, c, cols, v);
+#pragma unroll
+    for (int k = 0; k < V; ++k) s[0] += v[k];
+  }
+  row_sum<1024>(s, sh[0]);
+  const A mean = s[0] / (A)cols;
+  for (int64_t c = threadIdx.x * V; c < cols; c += 1024 * V) {
+    load_vec<T, V>(xr, c, cols, v);
+#pragma unroll
+    for (int k = 0; k < V; ++k)
+      if (c + k < cols) q[0] += (v[k] - mean) * (v[k] - mean);
+  }
+  row_sum<1024>(q, sh[1]);
+  const A rstd = reciprocal_root<A>(q[0] / (A)cols + eps);
+  if (threadIdx.x == 0 && mean_out) {
+    mean_out[row] = mean;
+    rstd_out[row] = rstd;
+  }
+  for (int64_t c = threadIdx.x * V; c < cols; c += 1024 * V) {
+    A w[V], b[V];
+    load_vec<T, V>(xr, c, cols, v);
+    if (weight) load_vec<W, V>(weight, c, cols, w);
+    if (bias) load_vec<W, V>(bias, c, cols, b);
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      v[k] = (v[k] - mean) * rstd;
+      if (weight) v[k] *= w[k];
+      if (bias) v[k] += b[k];
+    }
+    store_vec<T, V>(y + row * ldy, c, cols, v);
+  }
+}
+
+// dx (may be null) and, with `partial`, this workgroup's column sums: partial[group][2][cols] = { sum dy h, sum dy }
+template <typename T, typename W, int LANES, int ITER, int THREADS>
+__global__ __launch_bounds__(THREADS) void norm_backward_kernel(const T* __restrict__ dy, int64_t ldd, const T* __restrict__ x, int64_t ldx,
+                                                                const typename Wide<T>::type* __restrict__ mean_in,
+                                                                const typename Wide<T>::type* __restrict__ rstd_in, const W* __restrict__ weight,
+                                                                int64_t rows, int64_t cols, T* __restrict__ dx, typename Wide<T>::type* __restrict__ partial) {
+  typedef typename Wide<T>::type A;
+  constexpr int V = vec_of<T>(), GROUPS = THREADS / LANES, WAVES = THREADS / 64;
+  constexpr int SHARED = LANES <= 64 ? WAVES * LANES * ITER * V : 4 * WAVES;   // column sums of every wave, or the slots of the row sums
+  __shared__ A sh[SHARED];
+  const int lane = threadIdx.x % LANES;
+  const A inv = (A)1 / (A)cols;
+  A dw[ITER][V], db[ITER][V];
+#pragma unroll
+  for (int i = 0; i < ITER; ++i)
+#pragma unroll
+    for (int k = 0; k < V; ++k) dw[i][k] = db[i][k] = 0;
+  int turn = 0;
+  for (int64_t first = (int64_t)blockIdx.x * GROUPS; first < rows; first += (int64_t)gridDim.x * GROUPS, turn ^= 1) {
+    const int64_t row = first + threadIdx.x / LANES;
+    const bool live = row < rows;
+    const int64_t r = live ? row : 0;
+    const int64_t width = live ? cols : 0;      // lanes of no row read nothing and add zeros
+    const A mean = mean_in[r], rstd = rstd_in[r];
+    A h[ITER][V], g[ITER][V];
+    A s[2] = {0, 0};
+#pragma unroll
+    for (int i = 0; i < ITER; ++i) {
+      const int64_t col = ((int64_t)i * LANES + lane) * V;
+      A w[V];
+      load_vec<T, V>(dy + r * ldd, col, width, g[i]);
+      load_vec<T, V>(x + r * ldx, col, width, h[i]);
+      if (weight) load_vec<W, V>(weight, col, cols, w);
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        h[i][k] = col + k < width ? (h[i][k] - mean) * rstd : (A)0;
+        dw[i][k] += g[i][k] * h[i][k];
+        db[i][k] += g[i][k];
+        if (weight) g[i][k] *= w[k];
+        s[0] += g[i][k];
+        s[1] += g[i][k] * h[i][k];
+      }
+    }
+    if (dx) {
+      row_sum<LANES>(s, sh + (LANES > 64 ? turn * 2 * WAVES : 0));   // (two slots in turn: a wave may be a row ahead of the slowest)
+      const A c1 = s[0] * inv, c2 = s[1] * inv;
+#pragma unroll
+      for (int i = 0; i < ITER; ++i) {
+        const int64_t col = ((int64_t)i * LANES + lane) * V;
+        if (col < width) {
+#pragma unroll
+          for (int k = 0; k < V; ++k) g[i][k] = rstd * (g[i][k] - c1 - h[i][k] * c2);
+          store_vec<T, V>(dx + r * cols, col, cols, g[i]);
+        }
+      }
+    }
+  }
+  if (!partial) return;
+  A* out = partial + (int64_t)blockIdx.x * 2 * cols;
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    if constexpr (LANES > 64) {
+#pragma unroll
+      for (int i = 0; i < ITER; ++i) store_vec<A, V>(out + which * cols, ((int64_t)i * LANES + lane) * V, cols, which ? db[i] : dw[i]);
+    } else {
+      const int wave = threadIdx.x >> 6;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < ITER; ++i)
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+          A v = which ? db[i][k] : dw[i][k];
+          if constexpr (LANES == 16) {
+            v += __shfl_xor(v, 16);
+            v += __shfl_xor(v, 32);
+          }
+          if ((threadIdx.x & 63) < LANES) sh[(wave * ITER + i) * LANES * V + lane * V + k] = v;
+        }
+      __syncthreads();
+      for (int c = threadIdx.x; c < ITER * LANES * V; c += THREADS) {
+        A v = 0;
+        for (int w = 0; w < WAVES; ++w) v += sh[w * ITER * LANES * V + c];
+        if (c < cols) out[which * cols + c] = v;
+      }
+    }
+  }
+}
+
+template <typename T, typename W>
+__global__ __launch_bounds__(1024) void norm_backward_wide_kernel(const T* __restrict__ dy, int64_t ldd, const T* __restrict__ x, int64_t ldx,
+                                                                  const typename Wide<T>::type* __restrict__ mean_in,
+                                                                  const typename Wide<T>::type* __restrict__ rstd_in, const W* __restrict__ weight,
+                                                                  int64_t cols, T* __restrict__ dx) {
+  typedef typename Wide<T>::type A;
+  constexpr int V = vec_of<T>();
+  __shared__ A sh[2 * 16];
+  const int64_t row = blockIdx.x;
+  const A mean = mean_in[row], rstd = rstd_in[row], inv = (A)1 / (A)cols;
+  A s[2] = {0, 0}, g[V], h[V], w[V];
+  for (int64_t c = threadIdx.x * V; c < cols; c += 1024 * V) {
+    load_vec<T, V>(dy + row * ldd, c, cols, g);
+    load_vec<T, V>(x + row * ldx, c, cols, h);
+    if (weight) load_vec<W, V>(weight, c, cols, w);
+#pragma unroll
+    for (int k = 0; k < V; ++k)
+      if (c + k < cols) {
+        const A a = weight ? g[k] * w[k] : g[k];
+        s[0] += a;
+        s[1] += a * ((h[k] - mean) * rstd);
+      }
+  }
+  row_sum<1024>(s, sh);
+  const A c1 = s[0] * inv, c2 = s[1] * inv;
+  for (int64_t c = threadIdx.x * V; c < cols; c += 1024 * V) {
+    load_vec<T, V>(dy + row * ldd, c, cols, g);
+    load_vec<T, V>(x + row * ldx, c, cols, h);
+    if (weight) load_vec<W, V>(weight, c, cols, w);
+#pragma unroll
+    for (int k = 0; k < V; ++k) g[k] = rstd * ((weight ? g[k] * w[k] : g[k]) - c1 - (h[k] - mean) * rstd * c2);
+    store_vec<T, V>(dx + row * cols, c, cols, g);
+  }
+}
+
+// column sums of rows blockIdx.y, blockIdx.y + gridDim.y, ...: four lanes of rows x 64 columns, the lanes added in their order
+template <typename T>
+__global__ __launch_bounds__(256) void norm_columns_kernel(const T* __restrict__ dy, int64_t ldd, const T* __restrict__ x, int64_t ldx,
+                                                           const typename Wide<T>::type* __restrict__ mean_in,
+                                                           const typename Wide<T>::type* __restrict__ rstd_in, int64_t rows, int64_t cols,
+                                                           typename Wide<T>::type* __restrict__ partial) {
+  typedef typename Wide<T>::type A;
+  __shared__ A sh[2][4][64];
+  const int64_t col = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63);
+  const int part = threadIdx.x >> 6;
+  A dw = 0, db = 0;
+  if (col < cols)
+    for (int64_t r = (int64_t)blockIdx.y * 4 + part; r < rows; r += (int64_t)gridDim.y * 4) {
+      const A d = (A)dy[r * ldd + col];
+      dw += d * (((A)x[r * ldx + col] - mean_in[r]) * rstd_in[r]);
+      db += d;
+    }
+  sh[0][part][threadIdx.x & 63] = dw;
+  sh[1][part][threadIdx.x & 63] = db;
+  __syncthreads();
+  if (part < 2 && col < cols) {
+    A v = 0;
+    for (int w = 0; w < 4; ++w) v += sh[part][w][threadIdx.x & 63];
+    partial[((int64_t)blockIdx.y * 2 + part) * cols + col] = v;
+  }
+}
+
+// lanes that share a row, vectors a lane holds of it, workgroup size; lanes = 0: the kernels for wide rows
+struct Shape { int lanes, iter, threads; };
+
+// most: vectors a lane may hold below 1024 lanes.  4 forward (one array of the row in registers), 2 backward (four arrays of it)
+Shape shape_of(int64_t cols, int vec, int most) {
+  for (int lanes : {16, 64, 256, 1024}) {
+    const int limit = lanes == 1024 ? 4 : most;
+    const int64_t vectors = ceil_div(cols, (int64_t)lanes * vec);
+    if (vectors <= limit) return {lanes, vectors <= 1 ? 1 : vectors <= 2 ? 2 : 4, lanes <= 256 ? 256 : 1024};
+  }
+  return {0, 0, 1024};
+}
+
+// workgroups of the backward pass: enough to fill the card, few enough that their column sums stay small beside the rows
+int64_t backward_groups(const Shape& s, int64_t rows) {
+  const int64_t per = s.lanes ? s.threads / s.lanes : 4;
+  const int64_t most = s.threads == 1024 ? 256 : 1024;
+  const int64_t n = ceil_div(rows, per);
+  return n < 1 ? 1 : n < most ? n : most;
+}
+
+template <typename T, typename W>
+struct Norm {
+  typedef typename Wide<T>::type A;
+  static constexpr int V = vec_of<T>();
+
+  template <int LANES, int ITER, int THREADS>
+  static void forward_as(const vmcpde_norm_args& a, hipStream_t s) {
+    norm_forward_kernel<T, W, LANES, ITER, THREADS><<<(unsigned)ceil_div(a.rows, THREADS / LANES), THREADS, 0, s>>>(
+        static_cast<const T*>(a.x), a.ldx, static_cast<const W*>(a.weight), static_cast<const W*>(a.bias), (A)a.eps, a.rows, a.cols, static_cast<T*>(a.y), a.ldy,
+        static_cast<A*>(a.mean), static_cast<A*>(a.rstd));
+  }
+  template <int LANES, int THREADS>
+  static void forward_iter(int iter, const vmcpde_norm_args& a, hipStream_t s) {
+    if (iter == 1) forward_as<LANES, 1, THREADS>(a, s);
+    else if (iter == 2) forward_as<LANES, 2, THREADS>(a, s);
+    else forward_as<LANES, 4, THREADS>(a, s);
+  }
+  static void forward(const vmcpde_norm_args& a, hipStream_t s) {
+    const Shape p = shape_of(a.cols, V, 4);
+    if (p.lanes == 16) forward_iter<16, 256>(p.iter, a, s);
+    else if (p.lanes == 64) forward_iter<64, 256>(p.iter, a, s);
+    else if (p.lanes == 256) forward_iter<256, 256>(p.iter, a, s);
+    else if (p.lanes == 1024) forward_iter<1024, 1024>(p.iter, a, s);
+    else
+      norm_forward_wide_kernel<T, W><<<(unsigned)a.rows, 1024, 0, s>>>(static_cast<const T*>(a.x), a.ldx, static_cast<const W*>(a.weight), static_cast<const W*>(a.bias),
+                                                                       (A)a.eps, a.cols, static_cast<T*>(a.y), a.ldy, static_cast<A*>(a.mean), static_cast<A*>(a.rstd));
+  }
+
+  template <int LANES, int ITER, int THREADS>
+  static void backward_as(const vmcpde_norm_args& a, int64_t groups, A* partial, hipStream_t s) {
+    norm_backward_kernel<T, W, LANES, ITER, THREADS><<<(unsigned)groups, THREADS, 0, s>>>(
+        static_cast<const T*>(a.dy), a.ldd, static_cast<const T*>(a.x), a.ldx, static_cast<const A*>(a.mean), static_cast<const A*>(a.rstd),
+        static_cast<const W*>(a.weight), a.rows, a.cols, static_cast<T*>(a.dx), partial);
+  }
+  template <int LANES, int THREADS>
+  static void backward_iter(int iter, const vmcpde_norm_args& a, int64_t groups, A* partial, hipStream_t s) {
+    if (iter == 1) backward_as<LANES, 1, THREADS>(a, groups, partial, s);
+    else backward_as<LANES, 2, THREADS>(a, groups, partial, s);
+  }
+  static void backward(const vmcpde_norm_args& a, void* workspace, hipStream_t s) {
+    const Shape p = shape_of(a.cols, V, 2);
+    const int64_t groups = backward_groups(p, a.rows);
+    A* partial = a.dweight || a.dbias ? static_cast<A*>(workspace) : nullptr;
+    if (p.lanes == 16) backward_iter<16, 256>(p.iter, a, groups, partial, s);
+    else if (p.lanes == 64) backward_iter<64, 256>(p.iter, a, groups, partial, s);
+    else if (p.lanes == 256) backward_iter<256, 256>(p.iter, a, groups, partial, s);
+    else if (p.lanes == 1024 && p.iter <= 2) backward_iter<1024, 1024>(p.iter, a, groups, partial, s);
+    else if (p.lanes == 1024) backward_as<1024, 4, 1024>(a, groups, partial, s);
+    else {
+      if (a.dx && a.rows)
+        norm_backward_wide_kernel<T, W><<<(unsigned)a.rows, 1024, 0, s>>>(static_cast<const T*>(a.dy), a.ldd, static_cast<const T*>(a.x), a.ldx,
+                                                                          static_cast<const A*>(a.mean), static_cast<const A*>(a.rstd),
+                                                                          static_cast<const W*>(a.weight), a.cols, static_cast<T*>(a.dx));
+      if (partial)
+        norm_columns_kernel<T><<<dim3((unsigned)ceil_div(a.cols, 64), (unsigned)groups), 256, 0, s>>>(
+            static_cast<const T*>(a.dy), a.ldd, static_cast<const T*>(a.x), a.ldx, static_cast<const A*>(a.mean), static_cast<const A*>(a.rstd), a.rows, a.cols,
+            partial);
+    }
+    if (partial)
+      add_columns_kernel<A, W><<<dim3((unsigned)ceil_div(a.cols, 64), 2), 1024, 0, s>>>(partial, (int)groups, 2 * a.cols, a.cols, static_cast<W*>(a.dweight),
+                                                                                          static_cast<W*>(a.dbias));
+  }
+};
+
+// calls F<T, W> of the element type and the weights' type
+template <typename F>
+int by_types(const vmcpde_norm_args& a, F f) {
+  switch (a.dtype) {
+    case VMCPDE_F64: f(Norm<double, double>()); break;
+    case VMCPDE_F32: f(Norm<float, float>()); break;
+    case VMCPDE_F16: a.weight_dtype == VMCPDE_F32 ? f(Norm<f16_t, float>()) : f(Norm<f16_t, f16_t>()); break;
+    default: a.weight_dtype == VMCPDE_F32 ? f(Norm<bf16_t, float>()) : f(Norm<bf16_t, bf16_t>());
+  }
+  VMC_CHECK_HIP(hipGetLastError());
+  return 0;
+}
+
+int check(const vmcpde_norm_args* a) {
+  VMC_REQUIRE(a, "layer norm: null arguments");
+  VMC_REQUIRE(dtype_ok(a->dtype), "layer norm: type %d", a->dtype);
+  VMC_REQUIRE(a->weight_dtype == a->dtype || (a->weight_dtype == VMCPDE_F32 && dtype_size(a->dtype) == 2),
+              "layer norm: weights of type %d for elements of type %d (the same, or fp32 for 16-bit elements)", a->weight_dtype, a->dtype);
+  VMC_REQUIRE(a->rows >= 0 && a->rows < (int64_t)1 << 31, "layer norm: %lld rows", (long long)a->rows);
+  VMC_REQUIRE(a->cols >= 1 && a->cols < (int64_t)1 << 31, "layer norm: %lld columns", (long long)a->cols);
+  VMC_REQUIRE(a->rows == 0 || (a->x && a->ldx >= a->cols), "layer norm: x is null or its row pitch %lld is below its %lld columns", (long long)a->ldx, (long long)a->cols);
+  return 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+int vmcpde_layer_norm(const vmcpde_norm_args* a, void* stream) {
+  if (const int rc = check(a)) return rc;
+  VMC_REQUIRE(a->eps >= 0, "vmcpde_layer_norm: eps = %g", a->eps);
+  VMC_REQUIRE(!a->mean == !a->rstd, "vmcpde_layer_norm: mean and rstd go together");
+  if (a->rows == 0) return 0;
+  VMC_REQUIRE(a->y && a->ldy >= a->cols, "vmcpde_layer_norm: y is null or its row pitch is below its columns");
+  return by_types(*a, [&](auto norm) { norm.forward(*a, static_cast<hipStream_t>(stream)); });
+}
+
+int64_t vmcpde_layer_norm_backward_workspace_bytes(const vmcpde_norm_args* a) {
+  if (check(a)) return -1;
+  const Shape p = shape_of(a->cols, 16 / dtype_size(a->dtype), 2);
+  return backward_groups(p, a->rows) * 2 * a->cols * (a->dtype == VMCPDE_F64 ? 8 : 4);
+}
+
+int vmcpde_layer_norm_backward(const vmcpde_norm_args* a, void* workspace, int64_t workspace_bytes, void* stream) {
+  if (const int rc = check(a)) return rc;
+  VMC_REQUIRE(a->rows == 0 || (a->dy && a->ldd >= a->cols && a->mean && a->rstd), "vmcpde_layer_norm_backward: null dy, mean or rstd, or a row pitch below the columns");
+  if (a->dweight || a->dbias) {
+    const int64_t need = vmcpde_layer_norm_backward_workspace_bytes(a);
+    VMC_REQUIRE(workspace && workspace_bytes >= need, "vmcpde_layer_norm_backward: workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)need);
+  } else if (a->rows == 0 || !a->dx) {
+    return 0;
+  }
+  return by_types(*a, [&](auto norm) { norm.backward(*a, workspace, static_cast<hipStream_t>(stream)); });
+}
+
+}  // extern "C"

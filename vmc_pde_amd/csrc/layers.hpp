@@ -1,0 +1,101 @@
+// Shared by the layer operators (dense.hip, layer_norm.hip, global_norm.hip): element types, reductions, small vectors.
+#pragma once
+#include "common.hpp"
+#include "wave_ops.hpp"
+
+namespace vmcpde {
+
+typedef __bf16 bf16_t;
+typedef _Float16 f16_t;
+
+// Arithmetic type of an element type: sums, statistics and epilogues of 16-bit elements are held in fp32, of fp64 in fp64.
+template <typename T> struct Wide { typedef float type; };
+template <> struct Wide<double> { typedef double type; };
+// act'(z) kept between the passes: fp16 for both 16-bit types.  Every slope lies in [-0.13, 1.13], where fp16 resolves 2^-11 relative
+// (6e-8 absolute near zero); bf16's 2^-8 would add an error as large as the output's own rounding to every gradient.
+template <typename T> struct Slope { typedef T type; };
+template <> struct Slope<bf16_t> { typedef f16_t type; };
+
+template <typename T, int N>
+struct alignas(sizeof(T) * N) Pack { T v[N]; };
+
+inline int dtype_size(int dtype) { return dtype == VMCPDE_F64 ? 8 : dtype == VMCPDE_F32 ? 4 : 2; }
+inline bool dtype_ok(int dtype) { return dtype >= VMCPDE_F64 && dtype <= VMCPDE_BF16; }
+inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+inline int64_t round_up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
+inline int64_t ceil_div(int64_t v, int64_t m) { return (v + m - 1) / m; }
+
+// Sum over groups of GROUP consecutive lanes (16 or 64), every lane of the group returns it.  DPP steps, no LDS.
+template <int CTRL>
+__device__ __forceinline__ float dpp_move(float v) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, false));
+}
+template <int GROUP, typename A>
+__device__ __forceinline__ A group_sum(A v) {
+  static_assert(GROUP == 16 || GROUP == 64, "a DPP row or a wave");
+  v += dpp_move<0xb1>(v);    // quad_perm [1,0,3,2]
+  v += dpp_move<0x4e>(v);    // quad_perm [2,3,0,1]
+  v += dpp_move<0x124>(v);   // row_ror:4
+  v += dpp_move<0x128>(v);   // row_ror:8
+  if constexpr (GROUP == 64) {
+    v += __shfl_xor(v, 16);
+    v += __shfl_xor(v, 32);
+  }
+  return v;
+}
+
+// elements of a 16-byte vector
+template <typename T> constexpr int vec_of() { return 16 / (int)sizeof(T); }
+
+// elements col .. col + V of a row, zero behind its end; 16 bytes a lane at any alignment (global memory takes unaligned vectors)
+template <typename T, int V, typename A>
+__device__ __forceinline__ void load_vec(const T* __restrict__ row, int64_t col, int64_t cols, A (&out)[V]) {
+  struct __attribute__((packed, aligned(sizeof(T)))) Raw { T v[V]; };
+  if (col + V <= cols) {
+    const Raw r = *reinterpret_cast<const Raw*>(row + col);
+#pragma unroll
+    for (int k = 0; k < V; ++k) out[k] = (A)r.v[k];
+  } else {
+#pragma unroll
+    for (int k = 0; k < V; ++k) out[k] = col + k < cols ? (A)row[col + k] : (A)0;
+  }
+}
+template <typename T, int V, typename A>
+__device__ __forceinline__ void store_vec(T* __restrict__ row, int64_t col, int64_t cols, const A (&in)[V]) {
+  struct __attribute__((packed, aligned(sizeof(T)))) Raw { T v[V]; };
+  if (col + V <= cols) {
+    Raw r;
+#pragma unroll
+    for (int k = 0; k < V; ++k) r.v[k] = (T)in[k];
+    *reinterpret_cast<Raw*>(row + col) = r;
+  } else {
+#pragma unroll
+    for (int k = 0; k < V; ++k)
+      if (col + k < cols) row[col + k] = (T)in[k];
+  }
+}
+
+// out_w[col] = sum_g partial[g * pitch + w * cols + col] for w = blockIdx.y (a null out is skipped): the last step of a sum over rows.
+// 64 columns x 16 parts of the groups a workgroup; the parts are added in their order.
+template <typename A, typename W>
+static __global__ __launch_bounds__(1024) void add_columns_kernel(const A* __restrict__ partial, int groups, int64_t pitch, int64_t cols, W* __restrict__ out0,
+                                                           W* __restrict__ out1) {
+  __shared__ A sh[16][64];
+  const int which = blockIdx.y, part = threadIdx.x >> 6, c = threadIdx.x & 63;
+  W* out = which ? out1 : out0;
+  if (!out) return;
+  const int64_t col = (int64_t)blockIdx.x * 64 + c;
+  A v = 0;
+  if (col < cols) {
+#pragma unroll 8
+    for (int g = part; g < groups; g += 16) v += partial[(int64_t)g * pitch + which * cols + col];
+  }
+  sh[part][c] = v;
+  __syncthreads();
+  if (part == 0 && col < cols) {
+    for (int p = 1; p < 16; ++p) v += sh[p][c];
+    out[col] = (W)v;
+  }
+}
+
+}  // namespace vmcpde

@@ -17,6 +17,7 @@ import torch
 
 from . import _native as nat
 from . import global_defs
+from . import layers
 from . import net
 from . import util
 
@@ -141,7 +142,10 @@ class VarState:
         return None
 
     # ---- var_state.py:36-64 -----------------------------------------------------------------------------------
-    def __call__(self, coords, mode="eval", avg=False):
+    def __call__(self, coords, mode="eval", avg=False, max_norm=None):
+        """`max_norm` (with mode="costfun", avg=True): the averaged gradient clipped to that 2-norm (`layers.clip_by_global_norm`)."""
+        if max_norm is not None and not (mode == "costfun" and avg):
+            raise ValueError('max_norm clips the averaged gradient: it needs mode="costfun" and avg=True')
         if mode == "eval":
             x = torch.as_tensor(coords, dtype=global_defs.tReal, device=self.device)
             lead = x.shape[:-1]
@@ -155,7 +159,10 @@ class VarState:
             r = self.evaluate(coords, want_g=False)
             value, grad = -r["logp"][None, ...], -r["J"]
             if avg:
-                return value.mean(), grad.mean(dim=(0, 1))
+                mean = grad.mean(dim=(0, 1))
+                if max_norm is not None:
+                    layers.clip_by_global_norm(mean, max_norm)
+                return value.mean(), mean
             return value, grad
         raise ValueError(f"unknown mode {mode}")
 
