@@ -1,7 +1,7 @@
 """Plain 64-bit forms of the layer operators on the CPU, and how far a right implementation may be from them.
 
 u = half a step of a type (finfo.eps / 2).  Every bound is a sum over the roundings that the operators' documentation allows: sums and epilogues in
-fp32 (fp64 for fp64), dz rounded to the element type, act' kept in fp16 beside 16-bit elements, one rounding of each output."""
+fp32 (fp64 for fp64), dz rounded to the element type, act' kept in fp16 for bf16, in fp32 for fp16, one rounding of each output."""
 import math
 
 import torch
@@ -43,8 +43,9 @@ def product_error(p, q, depth, u):
 
 def dense(x, kernel, bias, residual, act, scale, dy, dtype):
     """{name: (value, bound)} of y, slope, dx, dkernel, dbias."""
-    u, uw, us = half_step(dtype), half_step(wide_of(dtype)), half_step(torch.float16 if dtype in (torch.float16, torch.bfloat16) else dtype)
-    tiny, tiny_s = smallest(dtype), smallest(torch.float16 if dtype in (torch.float16, torch.bfloat16) else dtype)
+    kept = {torch.bfloat16: torch.float16, torch.float16: torch.float32}.get(dtype, dtype)
+    u, uw, us = half_step(dtype), half_step(wide_of(dtype)), half_step(kept)
+    tiny, tiny_s = smallest(dtype), smallest(kept)
     x, kernel, bias, residual, dy = map(f64, (x, kernel, bias, residual, dy))
     k, n, rows = kernel.shape[0], kernel.shape[1], x.shape[0]
     z = x @ kernel + (bias if bias is not None else 0)

@@ -62,6 +62,30 @@ __device__ __forceinline__ void finish(const Epilogue<T>& e, int64_t row, int64_
   if (e.slope) e.slope[row * e.n + col] = (typename Slope<T>::type)slope;
 }
 
+// columns col .. col + 4 of a row (those inside it)
+template <typename T, typename A>
+__device__ __forceinline__ void finish4(const Epilogue<T>& e, int64_t row, int64_t col, const A (&z)[4]) {
+  A a[4], slope[4], more[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) a[k] = z[k];
+  if (e.bias) {
+    load_vec<T, 4>(e.bias, col, e.n, more);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) a[k] += more[k];
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) activate<A>(e.act, a[k], a[k], slope[k]);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) a[k] *= e.scale;
+  if (e.residual) {
+    load_vec<T, 4>(e.residual + row * e.ldr, col, e.n, more);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) a[k] += more[k];
+  }
+  store_vec<T, 4>(e.y + row * e.ldy, col, e.n, a);
+  if (e.slope) store_vec<typename Slope<T>::type, 4>(e.slope + row * e.n, col, e.n, slope);
+}
+
 // ---- products ----------------------------------------------------------------------------------------------------------------------
 
 // C [m][n] = sum_k P(row, k) Q(k, col).  An operand lies along k (element (r, k) at r * ld + k), or with `across` along its rows / columns
@@ -72,6 +96,7 @@ struct Product {
   int64_t ldp, ldq;
   int32_t m, n, k;
   int32_t p_across, q_across;
+  int32_t kp, kq;          // 16-bit products: k that P and Q hold (k may be rounded up to whole chunks; what lies behind is zero)
 };
 
 template <typename A> struct Acc;
@@ -174,15 +199,199 @@ __global__ __launch_bounds__(256) void product_wide_kernel(Product g, int tiles_
     }
 }
 
-// the slices' sums added in their order, and the epilogue
+// ---- 16-bit products on the matrix pipe --------------------------------------------------------------------------------------------------
+
+typedef short short8 __attribute__((ext_vector_type(8)));
+typedef short short4v __attribute__((ext_vector_type(4)));
+typedef float float4v __attribute__((ext_vector_type(4)));
+typedef bf16_t bf16x8 __attribute__((ext_vector_type(8)));
+typedef f16_t f16x8 __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(3))) char lds_char;
+typedef __attribute__((address_space(3))) short4v lds_short4;
+typedef __attribute__((address_space(3))) short8 lds_short8;
+
+constexpr int HK = 64;                    // k a step
+constexpr int OUTSIDE = 0x7ffffff0;       // byte offset behind every record: such a lane reads zeros
+
+__device__ __forceinline__ float4v mfma16(bf16_t, short8 a, short8 b, float4v c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ float4v mfma16(f16_t, short8 a, short8 b, float4v c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+// One operand's tile, R rows x HK of k, 16-byte chunks straight from memory into LDS.  Along k: [row][8 chunks], chunk c of row r at
+// place c ^ (r & 7).  Across: [k][R / 8 chunks], chunk c of line k at place c ^ s(k); there the transposing LDS read hands a lane four k of
+// its row.  The places are permuted on the memory side (a lane fetches the chunk that belongs where it writes), so that the fragment
+// reads of a wave fall on different banks.
+template <int R, bool ACROSS, int THREADS>
+struct HalfTile {
+  static constexpr int LOADS = R * HK / 8 / THREADS;
+  static constexpr int BYTES = R * HK * 2;
+  static constexpr int PER_LINE = R / 8;                       // chunks of a line of k
+  const char* base;
+  int64_t left, step;                                          // bytes from base to the operand's end; bytes a step of k moves on
+  int offset[LOADS], chunk_k[LOADS];
+  int frag, line;                                              // this lane's place in a fragment read
+
+  static __device__ __forceinline__ int swizzle(int k) {       // lines k whose reads meet: k & 3 and bit 3 of k
+    if constexpr (PER_LINE >= 16) return 2 * ((k & 3) | ((k >> 1) & 4));
+    else if constexpr (PER_LINE == 8) return 2 * (((k >> 1) & 1) | ((k >> 2) & 2));
+    else return 2 * ((k >> 3) & 1);
+  }
+
+  // rows = the operand's rows (columns of C for Q), k_total its k; row0: this tile's first; row_w: the wave's first row in the tile
+  __device__ __forceinline__ void init(const void* p, int64_t ld, int rows, int k_total, int row0, int k0, int row_w) {
+    const int t = threadIdx.x, lane = t & 63, i = lane & 15, g = lane >> 4;
+    const int64_t first = ACROSS ? (int64_t)k0 * ld + row0 : (int64_t)row0 * ld + k0;
+    const int64_t end = ACROSS ? (int64_t)(k_total - 1) * ld + rows : (int64_t)(rows - 1) * ld + k_total;
+    base = static_cast<const char*>(p) + first * 2;
+    left = ((end - first) * 2 + 3) & ~(int64_t)3;              // the record ends with a whole dword (an odd width's last one: half of it is used)
+    step = (ACROSS ? HK * ld : HK) * 2;
+#pragma unroll
+    for (int j = 0; j < LOADS; ++j) {
+      const int u = j * THREADS + t;
+      if constexpr (ACROSS) {
+        const int k = u / PER_LINE, c = (u % PER_LINE) ^ swizzle(k);
+        offset[j] = k * (int)ld * 2 + c * 16;
+        chunk_k[j] = 0;
+      } else {
+        const int r = u / 8, c = (u % 8) ^ (r & 7);
+        offset[j] = r * (int)ld * 2 + c * 16;
+        chunk_k[j] = c * 8;
+      }
+    }
+    if constexpr (ACROSS) {
+      line = g * 8 + (i >> 2);
+      const int c = row_w / 8 + ((i & 3) >> 1);
+      frag = line * (R * 2) + ((c ^ swizzle(line)) << 4) + (i & 1) * 8;
+    } else {
+      line = 0;
+      frag = (row_w + i) * 128 + ((g ^ (i & 7)) << 4);
+    }
+  }
+
+  // fetch the tile at k (k_left of it inside the operand) and move on
+  __device__ __forceinline__ void fetch(lds_char* to, int k_left) {
+    const int64_t l = left < 0 ? 0 : left;
+    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, l < OUTSIDE ? (int)l : OUTSIDE, 0x00020000);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+#pragma unroll
+    for (int j = 0; j < LOADS; ++j) {
+      const int at = ACROSS || chunk_k[j] < k_left ? offset[j] : OUTSIDE;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, to + (j * THREADS + wave * 64) * 16, 16, at, 0, 0, 0);
+    }
+    base += step;
+    left -= step;
+  }
+
+  // rows row_w + 16 t .. + 16, k = 32 s + 8 (lane / 16) .. + 8 of the tile
+  __device__ __forceinline__ short8 fragment(const lds_char* tile, int t, int s) const {
+    if constexpr (ACROSS) {
+      const lds_char* a = tile + ((frag ^ (t << 5)) + s * 32 * R * 2);
+      const short4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)a), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(a + 4 * R * 2));
+      return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    } else {
+      return *(const lds_short8*)(tile + ((frag ^ (s << 6)) + t * 2048));
+    }
+  }
+};
+
+// BM x BN of C by WM x WN waves; k in [k_begin, k_end) (k_begin a multiple of HK).  Two buffers: a step's fetches fly while the step before
+// is multiplied.  The column operand goes in as the matrix instruction's first, so a lane's four results lie along a row of C:
+// out(row, col, v): C[row][col .. col + 4].
+template <typename H, int BM, int BN, int WM, int WN, bool PX, bool QX, typename F>
+__device__ __forceinline__ void half_product(const Product& g, int row0, int col0, int k_begin, int k_end, F out) {
+  constexpr int THREADS = 64 * WM * WN, TM = BM / WM / 16, TN = BN / WN / 16;
+  typedef HalfTile<BM, PX, THREADS> P;
+  typedef HalfTile<BN, QX, THREADS> Q;
+  __shared__ __attribute__((aligned(16))) char tiles[2 * (P::BYTES + Q::BYTES)];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int wr = (wave / WN) * TM * 16, wc = (wave % WN) * TN * 16;
+  P p;
+  Q q;
+  p.init(g.p, g.ldp, g.m, min(k_end, g.kp), row0, k_begin, wr);
+  q.init(g.q, g.ldq, g.n, min(k_end, g.kq), col0, k_begin, wc);
+  float4v acc[TM][TN];
+#pragma unroll
+  for (int a = 0; a < TM; ++a)
+#pragma unroll
+    for (int b = 0; b < TN; ++b) acc[a][b] = {0, 0, 0, 0};
+  auto multiply = [&](const lds_char* tp, const lds_char* tq) {
+#pragma unroll
+    for (int s = 0; s < HK / 32; ++s) {
+      short8 fp[TM], fq[TN];
+#pragma unroll
+      for (int b = 0; b < TN; ++b) fq[b] = q.fragment(tq, b, s);
+#pragma unroll
+      for (int a = 0; a < TM; ++a) fp[a] = p.fragment(tp, a, s);
+#pragma unroll
+      for (int a = 0; a < TM; ++a)
+#pragma unroll
+        for (int b = 0; b < TN; ++b) acc[a][b] = mfma16(H(), fq[b], fp[a], acc[a][b]);
+    }
+  };
+  lds_char* const lds = (lds_char*)tiles;
+  int at = 0;
+  if (k_begin < k_end) {
+    p.fetch(lds, k_end - k_begin);
+    q.fetch(lds + P::BYTES, k_end - k_begin);
+  }
+  auto step = [&](lds_char* __restrict__ now_p, lds_char* __restrict__ now_q, lds_char* __restrict__ next_p, lds_char* __restrict__ next_q, int k_left) {
+    if (k_left > 0) {
+      p.fetch(next_p, k_left);
+      q.fetch(next_q, k_left);
+    }
+    multiply(now_p, now_q);
+  };
+  for (int k = k_begin; k < k_end; k += HK) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();                      // this step's tiles are there, and the other buffer's readers are done
+    const int other = at ^ (P::BYTES + Q::BYTES);
+    step(lds + at, lds + at + P::BYTES, lds + other, lds + other + P::BYTES, k_end - k - HK);
+    at = other;
+  }
+  const int i = lane & 15, quad = (lane >> 4) * 4;
+#pragma unroll
+  for (int a = 0; a < TM; ++a)
+#pragma unroll
+    for (int b = 0; b < TN; ++b) {
+      const float v[4] = {acc[a][b][0], acc[a][b][1], acc[a][b][2], acc[a][b][3]};
+      out(row0 + wr + a * 16 + i, col0 + wc + b * 16 + quad, v);
+    }
+}
+
+// C in BM x BN tiles, slice blockIdx.y of the k range (`part` != null: its sums).  Workgroups go round the eight XCDs by their number: each
+// XCD takes one contiguous eighth of the tiles, in bands of eight tile rows, so that the operands a band shares stay in its L2.
+template <typename H, int BM, int BN, int WM, int WN, bool PX, bool QX>
+__global__ __launch_bounds__(64 * WM * WN) void product_half_kernel(Product g, int tiles_m, int tiles_n, int k_slice, float* __restrict__ part, Epilogue<H> e) {
+  const int tiles = tiles_m * tiles_n, id = blockIdx.x, xcd = id & 7, each = tiles >> 3, more = tiles & 7;
+  const int tile = xcd * each + (xcd < more ? xcd : more) + (id >> 3);
+  const int band = tile / (8 * tiles_n), in_band = tile - band * 8 * tiles_n, height = min(8, tiles_m - band * 8);
+  const int row0 = (band * 8 + in_band % height) * BM, col0 = (in_band / height) * BN;
+  const int k_begin = blockIdx.y * k_slice, k_end = min(k_begin + k_slice, g.k);
+  half_product<H, BM, BN, WM, WN, PX, QX>(g, row0, col0, k_begin, k_end, [&](int row, int col, const float (&v)[4]) {
+    if (row >= g.m || col >= g.n) return;
+    if (part) store_vec<float, 4>(part + ((int64_t)blockIdx.y * g.m + row) * g.n, col, g.n, v);
+    else finish4<H>(e, row, col, v);
+  });
+}
+
+// the slices' sums added in their order, and the epilogue: four columns a lane
 template <typename T>
 __global__ __launch_bounds__(256) void product_join_kernel(const typename Wide<T>::type* __restrict__ part, int slices, int64_t m, int64_t n, Epilogue<T> e) {
   typedef typename Wide<T>::type A;
-  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (at >= m * n) return;
-  A z = 0;
-  for (int s = 0; s < slices; ++s) z += part[(int64_t)s * m * n + at];
-  finish<T, A>(e, at / n, at % n, z);
+  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x, quads = (n + 3) / 4, row = at / quads, col = (at - row * quads) * 4;
+  if (row >= m) return;
+  A z[4] = {0, 0, 0, 0};
+#pragma unroll 4
+  for (int s = 0; s < slices; ++s) {
+    A v[4];
+    load_vec<A, 4>(part + ((int64_t)s * m + row) * n, col, n, v);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) z[k] += v[k];
+  }
+  finish4<T>(e, row, col, z);
 }
 
 // ---- the gradient before the activation ----------------------------------------------------------------------------------------------
@@ -228,19 +437,26 @@ __global__ __launch_bounds__(256) void dense_dz_kernel(const T* __restrict__ dy,
 
 // ---- plans ---------------------------------------------------------------------------------------------------------------------------
 
+template <typename T> constexpr bool is_half() { return sizeof(T) == 2; }
+
 struct Tiles { int bm, bn, slices, k_slice; };
 
+// Tile and k slices of a product.  128 x 128 fills the matrix pipe; sides of at most 32 rows or columns take 32, so that little is multiplied for
+// nothing.  16-bit operands take 256 x 256, which reads each operand half as often, where such tiles still fill the card.  Where the tiles leave CUs
+// idle the k range is cut, and the slices' sums are joined by a second launch.
 template <typename T>
 Tiles tiles_of(int64_t m, int64_t n, int64_t k) {
+  constexpr int64_t step = is_half<T>() ? HK : WIDE_K;
   Tiles t;
   t.bm = m <= 32 ? 32 : 128;
   t.bn = n <= 32 ? 32 : 128;
+  if (is_half<T>() && ceil_div(m, 256) * ceil_div(n, 256) >= 192) t.bm = t.bn = 256;
   const int64_t tiles = ceil_div(m, t.bm) * ceil_div(n, t.bn);
   int64_t slices = 1;
-  if (tiles > 0 && tiles < 256) slices = std::min<int64_t>(std::min<int64_t>(ceil_div(512, tiles), ceil_div(k, 4 * WIDE_K)), 512);
+  if (tiles > 0 && tiles < 256) slices = std::min<int64_t>(std::min<int64_t>(ceil_div(512, tiles), ceil_div(k, 4 * step)), 512);
   if (slices < 1) slices = 1;
-  t.k_slice = (int)round_up(ceil_div(k, slices), WIDE_K);
-  if (t.k_slice < WIDE_K) t.k_slice = WIDE_K;
+  t.k_slice = (int)round_up(ceil_div(k, slices), step);
+  if (t.k_slice < step) t.k_slice = (int)step;
   t.slices = (int)std::max<int64_t>(1, ceil_div(k, t.k_slice));
   return t;
 }
@@ -251,18 +467,35 @@ int64_t product_bytes(int64_t m, int64_t n, int64_t k) {
   return t.slices > 1 ? round_up((int64_t)t.slices * m * n * (int64_t)sizeof(typename Wide<T>::type), 256) : 0;
 }
 
+template <typename T, int BM, int BN, int WM, int WN>
+void product_half(const Product& g, const Tiles& t, float* part, const Epilogue<T>& e, hipStream_t s) {
+  const int tiles_m = (int)ceil_div(g.m, BM), tiles_n = (int)ceil_div(g.n, BN);
+  const dim3 grid((unsigned)(tiles_m * tiles_n), (unsigned)t.slices);
+  if (!g.p_across && g.q_across) product_half_kernel<T, BM, BN, WM, WN, false, true><<<grid, 64 * WM * WN, 0, s>>>(g, tiles_m, tiles_n, t.k_slice, part, e);
+  else if (!g.p_across) product_half_kernel<T, BM, BN, WM, WN, false, false><<<grid, 64 * WM * WN, 0, s>>>(g, tiles_m, tiles_n, t.k_slice, part, e);
+  else product_half_kernel<T, BM, BN, WM, WN, true, true><<<grid, 64 * WM * WN, 0, s>>>(g, tiles_m, tiles_n, t.k_slice, part, e);
+}
+
 template <typename T>
 void product(const Product& g, const Epilogue<T>& e, void* workspace, hipStream_t s) {
   typedef typename Wide<T>::type A;
   const Tiles t = tiles_of<T>(g.m, g.n, g.k);
   A* part = t.slices > 1 ? static_cast<A*>(workspace) : nullptr;
-  const int tiles_n = (int)ceil_div(g.n, t.bn);
-  const dim3 grid((unsigned)(ceil_div(g.m, t.bm) * tiles_n), (unsigned)t.slices);
-  if (t.bm == 128 && t.bn == 128) product_wide_kernel<T, 128, 128, 2><<<grid, 256, 0, s>>>(g, tiles_n, t.k_slice, part, e);
-  else if (t.bm == 128) product_wide_kernel<T, 128, 32, 4><<<grid, 256, 0, s>>>(g, tiles_n, t.k_slice, part, e);
-  else if (t.bn == 128) product_wide_kernel<T, 32, 128, 1><<<grid, 256, 0, s>>>(g, tiles_n, t.k_slice, part, e);
-  else product_wide_kernel<T, 32, 32, 2><<<grid, 256, 0, s>>>(g, tiles_n, t.k_slice, part, e);
-  if (part) product_join_kernel<T><<<(unsigned)ceil_div((int64_t)g.m * g.n, 256), 256, 0, s>>>(part, t.slices, g.m, g.n, e);
+  if constexpr (is_half<T>()) {
+    if (t.bm == 256) product_half<T, 256, 256, 2, 4>(g, t, part, e, s);
+    else if (t.bm == 128 && t.bn == 128) product_half<T, 128, 128, 2, 2>(g, t, part, e, s);
+    else if (t.bm == 128) product_half<T, 128, 32, 4, 1>(g, t, part, e, s);
+    else if (t.bn == 128) product_half<T, 32, 128, 1, 4>(g, t, part, e, s);
+    else product_half<T, 32, 32, 2, 2>(g, t, part, e, s);
+  } else {
+    const int tiles_n = (int)ceil_div(g.n, t.bn);
+    const dim3 grid((unsigned)(ceil_div(g.m, t.bm) * tiles_n), (unsigned)t.slices);
+    if (t.bm == 128 && t.bn == 128) product_wide_kernel<T, 128, 128, 2><<<grid, 256, 0, s>>>(g, tiles_n, t.k_slice, part, e);
+    else if (t.bm == 128) product_wide_kernel<T, 128, 32, 4><<<grid, 256, 0, s>>>(g, tiles_n, t.k_slice, part, e);
+    else if (t.bn == 128) product_wide_kernel<T, 32, 128, 1><<<grid, 256, 0, s>>>(g, tiles_n, t.k_slice, part, e);
+    else product_wide_kernel<T, 32, 32, 2><<<grid, 256, 0, s>>>(g, tiles_n, t.k_slice, part, e);
+  }
+  if (part) product_join_kernel<T><<<(unsigned)ceil_div((int64_t)g.m * ((g.n + 3) / 4), 256), 256, 0, s>>>(part, t.slices, g.m, g.n, e);
 }
 
 // workgroups along the rows of the dz kernel
@@ -271,82 +504,145 @@ int64_t dz_groups(int64_t rows, int64_t cols_blocks, int rows_at_once) {
   return std::min<int64_t>(std::min<int64_t>(want, have), 512);
 }
 
-template <typename T>
-struct Backward {
-  typedef typename Wide<T>::type A;
-  bool need_dz, own_dz;          // dz is used by a product; dz is not dy itself
-  int lanes;
-  int64_t ldz, groups, dz_bytes, part_bytes, product_bytes_, total;
-  explicit Backward(const vmcpde_dense_args& a) {
-    need_dz = a.dx || a.dkernel;
-    own_dz = need_dz && (a.slope || a.scale != 1.0);
-    lanes = a.n_out <= 8 * vec_of<T>() ? 8 : 32;
-    ldz = own_dz ? a.n_out : a.ldd;
-    groups = dz_groups(a.rows, ceil_div(a.n_out, lanes * vec_of<T>()), 256 / lanes);
-    dz_bytes = own_dz ? round_up(a.rows * ldz * (int64_t)sizeof(T), 256) : 0;
-    part_bytes = a.dbias ? round_up(groups * a.n_out * (int64_t)sizeof(A), 256) : 0;
-    product_bytes_ = std::max(a.dx ? product_bytes<T>(a.rows, a.n_in, a.n_out) : 0, a.dkernel ? product_bytes<T>(a.n_in, a.n_out, a.rows) : 0);
-    total = dz_bytes + part_bytes + product_bytes_;
-  }
+// A matrix operand in memory: `lines` of `n` elements behind each other, `ld` apart.
+struct Lines {
+  const void* p;
+  int64_t lines, n, ld;
 };
+
+// Whether the 16-bit products can fetch it: 16-byte chunks at 16-byte addresses, and whole chunks where its lines lie along k.  What they cannot is
+// copied into lines of whole chunks first, zeros behind each line's end.
+template <typename T>
+bool fetchable(const Lines& o, bool along_k) {
+  return !is_half<T>() || (aligned16(o.p) && o.ld % 8 == 0 && (!along_k || o.n % 8 == 0));
+}
+
+template <typename T>
+void scaled_copy(const Lines& from, const typename Slope<T>::type* slope, double scale, T* to, int64_t ld_to, typename Wide<T>::type* partial, int64_t groups, hipStream_t s) {
+  typedef typename Wide<T>::type A;
+  const int64_t width = to ? ld_to : from.n;
+  if (from.n <= 8 * vec_of<T>())
+    dense_dz_kernel<T, 8><<<dim3((unsigned)ceil_div(width, 8 * vec_of<T>()), (unsigned)groups), 256, 0, s>>>(static_cast<const T*>(from.p), from.ld, slope, (A)scale, from.lines,
+                                                                                                          from.n, to, ld_to, partial);
+  else
+    dense_dz_kernel<T, 32><<<dim3((unsigned)ceil_div(width, 32 * vec_of<T>()), (unsigned)groups), 256, 0, s>>>(static_cast<const T*>(from.p), from.ld, slope, (A)scale,
+                                                                                                            from.lines, from.n, to, ld_to, partial);
+}
+
+template <typename T>
+int64_t copy_groups(const Lines& o) {
+  const int lanes = o.n <= 8 * vec_of<T>() ? 8 : 32;
+  return dz_groups(o.lines, ceil_div(o.n, lanes * vec_of<T>()), 256 / lanes);
+}
 
 template <typename T>
 struct Dense {
   typedef typename Wide<T>::type A;
   typedef typename Slope<T>::type S;
 
-  static int64_t bytes(const vmcpde_dense_args& a, bool backward) { return backward ? Backward<T>(a).total : product_bytes<T>(a.rows, a.n_out, a.n_in); }
+  // A walk over a call's launches.  Without a workspace it only adds up what they need of one.
+  char* workspace;
+  hipStream_t stream;
+  int64_t used = 0, most = 0;
+  bool launch;
+  Dense(void* w, hipStream_t s, bool l) : workspace(static_cast<char*>(w)), stream(s), launch(l) {}
 
-  static void forward(const vmcpde_dense_args& a, void* workspace, hipStream_t s) {
-    const Epilogue<T> e = {static_cast<const T*>(a.bias), static_cast<const T*>(a.residual), a.ldr, static_cast<T*>(a.y), a.ldy, static_cast<S*>(a.slope), a.n_out,
-                           (A)a.scale, a.activation};
-    product<T>({a.x, a.kernel, a.ldx, a.ldk, (int32_t)a.rows, (int32_t)a.n_out, (int32_t)a.n_in, 0, !a.kernel_t}, e, workspace, s);
+  void* take(int64_t bytes) {
+    void* p = workspace ? workspace + used : nullptr;
+    used += round_up(bytes, 256);
+    most = std::max(most, used);
+    return p;
   }
 
-  static void backward(const vmcpde_dense_args& a, void* workspace, hipStream_t s) {
-    const Backward<T> b(a);
-    char* at = static_cast<char*>(workspace);
-    T* own = b.own_dz ? reinterpret_cast<T*>(at) : nullptr;
-    A* partial = a.dbias ? reinterpret_cast<A*>(at + b.dz_bytes) : nullptr;
-    void* rest = at + b.dz_bytes + b.part_bytes;
-    if (own || partial) {
-      const T* dy = static_cast<const T*>(a.dy);
-      const S* slope = static_cast<const S*>(a.slope);
-      const dim3 grid((unsigned)ceil_div(a.n_out, b.lanes * vec_of<T>()), (unsigned)b.groups);
-      if (b.lanes == 8) dense_dz_kernel<T, 8><<<grid, 256, 0, s>>>(dy, a.ldd, slope, (A)a.scale, a.rows, a.n_out, own, b.ldz, partial);
-      else dense_dz_kernel<T, 32><<<grid, 256, 0, s>>>(dy, a.ldd, slope, (A)a.scale, a.rows, a.n_out, own, b.ldz, partial);
-      if (partial)
-        add_columns_kernel<A, T><<<dim3((unsigned)ceil_div(a.n_out, 64), 1), 1024, 0, s>>>(partial, (int)b.groups, a.n_out, a.n_out, static_cast<T*>(a.dbias), nullptr);
+  // an operand that the products can fetch; `k_held` is what it holds along k where its lines lie along it
+  Lines ready(Lines o, bool along_k) {
+    if (fetchable<T>(o, along_k)) return o;
+    const int64_t ld = round_up(o.n, 8);
+    T* to = static_cast<T*>(take(o.lines * ld * (int64_t)sizeof(T)));
+    if (launch && o.lines) scaled_copy<T>(o, nullptr, 1.0, to, ld, nullptr, copy_groups<T>(o), stream);
+    return {to, o.lines, along_k ? ld : o.n, ld};
+  }
+
+  void multiply(Lines p, bool p_across, Lines q, bool q_across, int64_t m, int64_t n, int64_t k, const Epilogue<T>& e) {
+    p = ready(p, !p_across);
+    q = ready(q, !q_across);
+    const int64_t kp = p_across ? p.lines : p.n, kq = q_across ? q.lines : q.n, k_all = std::max(k, std::max(kp, kq));
+    const int64_t bytes = product_bytes<T>(m, n, k_all);
+    void* rest = bytes ? take(bytes) : nullptr;
+    if (launch) product<T>({p.p, q.p, p.ld, q.ld, (int32_t)m, (int32_t)n, (int32_t)k_all, p_across, q_across, (int32_t)kp, (int32_t)kq}, e, rest, stream);
+    used -= round_up(bytes, 256);
+  }
+
+  void forward(const vmcpde_dense_args& a) {
+    if (!a.rows) return;
+    const Epilogue<T> e = {static_cast<const T*>(a.bias), static_cast<const T*>(a.residual), a.ldr, static_cast<T*>(a.y), a.ldy, static_cast<S*>(a.slope), a.n_out,
+                           (A)a.scale, a.activation};
+    multiply({a.x, a.rows, a.n_in, a.ldx}, false, kernel_lines(a), !a.kernel_t, a.rows, a.n_out, a.n_in, e);
+  }
+
+  static Lines kernel_lines(const vmcpde_dense_args& a) {
+    return a.kernel_t ? Lines{a.kernel, a.n_out, a.n_in, a.ldk} : Lines{a.kernel, a.n_in, a.n_out, a.ldk};
+  }
+
+  void backward(const vmcpde_dense_args& a) {
+    const Lines dy = {a.dy, a.rows, a.n_out, a.ldd};
+    Lines dz = dy;
+    const bool own = (a.dx || a.dkernel) && (a.slope || a.scale != 1.0 || !fetchable<T>(dy, a.dx));
+    T* to = nullptr;
+    if (own) {
+      const int64_t ld = is_half<T>() ? round_up(a.n_out, 8) : a.n_out;
+      to = static_cast<T*>(take(a.rows * ld * (int64_t)sizeof(T)));
+      dz = {to, a.rows, a.n_out, ld};
     }
-    const void* dz = own ? own : a.dy;
+    if (own || a.dbias) {
+      const int64_t groups = copy_groups<T>(dy);
+      A* partial = a.dbias ? static_cast<A*>(take(groups * a.n_out * (int64_t)sizeof(A))) : nullptr;
+      if (launch) {
+        scaled_copy<T>(dy, static_cast<const S*>(a.slope), a.scale, to, dz.ld, partial, groups, stream);
+        if (a.dbias)
+          add_columns_kernel<A, T><<<dim3((unsigned)ceil_div(a.n_out, 64), 1), 1024, 0, stream>>>(partial, (int)groups, a.n_out, a.n_out, static_cast<T*>(a.dbias), nullptr);
+      }
+    }
     if (a.dx && a.rows) {
       const Epilogue<T> e = {nullptr, nullptr, 0, static_cast<T*>(a.dx), a.n_in, nullptr, a.n_in, 1, VMCPDE_ACT_NONE};
-      product<T>({dz, a.kernel, b.ldz, a.ldk, (int32_t)a.rows, (int32_t)a.n_in, (int32_t)a.n_out, 0, a.kernel_t}, e, rest, s);
+      Lines z = dz;
+      if (own) z.n = is_half<T>() ? dz.ld : dz.n;           // (zeros behind the line's end)
+      multiply(z, false, kernel_lines(a), a.kernel_t, a.rows, a.n_in, a.n_out, e);
     }
     if (a.dkernel) {
       const Epilogue<T> e = {nullptr, nullptr, 0, static_cast<T*>(a.dkernel), a.n_out, nullptr, a.n_out, 1, VMCPDE_ACT_NONE};
-      product<T>({a.x, dz, a.ldx, b.ldz, (int32_t)a.n_in, (int32_t)a.n_out, (int32_t)a.rows, 1, 1}, e, rest, s);
+      multiply({a.x, a.rows, a.n_in, a.ldx}, true, dz, true, a.n_in, a.n_out, a.rows, e);
     }
   }
 };
 
-template <typename F>
-void by_type(int dtype, F f) {
-  switch (dtype) {
-    case VMCPDE_F64: f(Dense<double>()); break;
-    case VMCPDE_F32: f(Dense<float>()); break;
-    case VMCPDE_F16: f(Dense<f16_t>()); break;
-    default: f(Dense<bf16_t>());
+// the bytes of workspace that the call needs; `launch`: the call itself
+template <typename T>
+int64_t walk(const vmcpde_dense_args& a, bool backward, void* workspace, hipStream_t s, bool launch) {
+  Dense<T> d(workspace, s, launch);
+  if (backward) d.backward(a);
+  else d.forward(a);
+  return d.most;
+}
+
+int64_t walk_type(const vmcpde_dense_args& a, bool backward, void* workspace, hipStream_t s, bool launch) {
+  switch (a.dtype) {
+    case VMCPDE_F64: return walk<double>(a, backward, workspace, s, launch);
+    case VMCPDE_F32: return walk<float>(a, backward, workspace, s, launch);
+    case VMCPDE_F16: return walk<f16_t>(a, backward, workspace, s, launch);
+    default: return walk<bf16_t>(a, backward, workspace, s, launch);
   }
 }
 
 int check(const vmcpde_dense_args* a, bool backward) {
-  constexpr int64_t LIMIT = (int64_t)1 << 30;
+  constexpr int64_t LIMIT = (int64_t)1 << 30, HALF_LIMIT = (int64_t)1 << 22;
   VMC_REQUIRE(a, "dense: null arguments");
   VMC_REQUIRE(dtype_ok(a->dtype), "dense: type %d", a->dtype);
   VMC_REQUIRE(a->activation >= VMCPDE_ACT_NONE && a->activation <= VMCPDE_ACT_SILU, "dense: activation %d", a->activation);
   VMC_REQUIRE(a->rows >= 0 && a->rows < LIMIT && a->n_in >= 1 && a->n_in < LIMIT && a->n_out >= 1 && a->n_out < LIMIT,
               "dense: rows %lld, n_in %lld, n_out %lld (rows from 0, widths from 1, all below 2^30)", (long long)a->rows, (long long)a->n_in, (long long)a->n_out);
+  VMC_REQUIRE(dtype_size(a->dtype) > 2 || (std::max(a->n_in, a->n_out) < HALF_LIMIT && a->ldx < HALF_LIMIT && a->ldk < HALF_LIMIT && a->ldd < HALF_LIMIT),
+              "dense: widths and row pitches of 16-bit operands are below 2^22");     // (a tile's rows within 2^31 bytes of each other)
   VMC_REQUIRE(a->scale == a->scale, "dense: scale is NaN");
   VMC_REQUIRE(ceil_div(std::max(a->rows, a->n_in), 32) * ceil_div(std::max(a->n_in, a->n_out), 32) < (int64_t)1 << 31, "dense: more than 2^31 tiles");
   const int64_t kernel_row = a->kernel_t ? a->n_in : a->n_out;
@@ -368,9 +664,7 @@ extern "C" {
 
 int64_t vmcpde_dense_workspace_bytes(const vmcpde_dense_args* a, int32_t backward) {
   if (check(a, backward != 0)) return -1;
-  int64_t n = 0;
-  by_type(a->dtype, [&](auto d) { n = d.bytes(*a, backward != 0); });
-  return n;
+  return walk_type(*a, backward != 0, nullptr, nullptr, false);
 }
 
 static int run(const vmcpde_dense_args* a, bool backward, void* workspace, int64_t workspace_bytes, void* stream) {
@@ -378,10 +672,7 @@ static int run(const vmcpde_dense_args* a, bool backward, void* workspace, int64
   if (!backward && a->rows == 0) return 0;
   const int64_t need = vmcpde_dense_workspace_bytes(a, backward);
   VMC_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), "dense: workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)need);
-  by_type(a->dtype, [&](auto d) {
-    if (backward) d.backward(*a, workspace, static_cast<hipStream_t>(stream));
-    else d.forward(*a, workspace, static_cast<hipStream_t>(stream));
-  });
+  walk_type(*a, backward, workspace, static_cast<hipStream_t>(stream), true);
   VMC_CHECK_HIP(hipGetLastError());
   return 0;
 }

@@ -11,13 +11,11 @@ typedef _Float16 f16_t;
 // Arithmetic type of an element type: sums, statistics and epilogues of 16-bit elements are held in fp32, of fp64 in fp64.
 template <typename T> struct Wide { typedef float type; };
 template <> struct Wide<double> { typedef double type; };
-// act'(z) kept between the passes: fp16 for both 16-bit types.  Every slope lies in [-0.13, 1.13], where fp16 resolves 2^-11 relative
-// (6e-8 absolute near zero); bf16's 2^-8 would add an error as large as the output's own rounding to every gradient.
+// act'(z) kept between the passes, finer than the element type: fp16 for bf16, fp32 for fp16.  Every slope lies in [-0.13, 1.13]; rounded to the
+// element type itself it would add an error as large as the output's own rounding to every gradient.
 template <typename T> struct Slope { typedef T type; };
 template <> struct Slope<bf16_t> { typedef f16_t type; };
-
-template <typename T, int N>
-struct alignas(sizeof(T) * N) Pack { T v[N]; };
+template <> struct Slope<f16_t> { typedef float type; };
 
 inline int dtype_size(int dtype) { return dtype == VMCPDE_F64 ? 8 : dtype == VMCPDE_F32 ? 4 : 2; }
 inline bool dtype_ok(int dtype) { return dtype >= VMCPDE_F64 && dtype <= VMCPDE_BF16; }

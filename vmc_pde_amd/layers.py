@@ -20,6 +20,7 @@ from . import _native as nat
 DTYPE = {torch.float64: 0, torch.float32: 1, torch.float16: 2, torch.bfloat16: 3}
 ACTIVATION = {"none": 0, "tanh": 1, "gelu": 2, "silu": 3}
 _HALF = (torch.float16, torch.bfloat16)
+SLOPE = {torch.float64: torch.float64, torch.float32: torch.float32, torch.float16: torch.float32, torch.bfloat16: torch.float16}
 
 
 def _on(device):
@@ -102,8 +103,8 @@ def dense(x, kernel, bias=None, *, activation="none", scale=1.0, residual=None, 
 
     x (..., n_in); kernel (n_in, n_out), the layout of the flat parameter vector's leaves, or a transposed view of an (n_out, n_in) one; bias
     (n_out,); residual of y's shape.  activation: "none", "tanh", "gelu" (z Phi(z)), "silu".  `scale` is the output factor of the reference's
-    conditioners (net.py:50, 61: 10 * tanh).  With `want_slope` returns (y, slope): act'(z), which `dense_backward` takes (None for "none");
-    fp16 beside 16-bit elements, else of the element type."""
+    conditioners (net.py:50, 61: 10 * tanh).  Widths and row pitches of 16-bit operands are below 2^22.  With `want_slope` returns (y, slope): act'(z), which `dense_backward` takes (None for "none");
+    of the type SLOPE[x.dtype] (fp16 for bf16, fp32 for fp16, else the element type)."""
     _check(x, kernel=kernel, bias=bias, residual=residual)
     if activation not in ACTIVATION:
         raise ValueError(f"activation {activation!r}: one of {sorted(ACTIVATION)} is needed")
@@ -121,7 +122,7 @@ def dense(x, kernel, bias=None, *, activation="none", scale=1.0, residual=None, 
         y = torch.empty(shape, dtype=x.dtype, device=device)
         slope = None
         if want_slope and activation != "none":
-            slope = torch.empty(shape, dtype=torch.float16 if x.dtype in _HALF else x.dtype, device=device)
+            slope = torch.empty(shape, dtype=SLOPE[x.dtype], device=device)
         a = nat.DenseArgs(DTYPE[x.dtype], ACTIVATION[activation], kernel_t, 0, x.numel() // n_in, n_in, n_out, x.data_ptr(), ldx, kernel.data_ptr(), ldk,
                           _address(bias), _address(residual), ldr, float(scale), y.data_ptr(), n_out, _address(slope))
         ws, nbytes = _workspace(nat.lib().vmcpde_dense_workspace_bytes(a, 0), device)
@@ -141,7 +142,7 @@ def dense_backward(dy, x, kernel, slope=None, *, scale=1.0, want_x=True, want_ke
     x, ldx = _rows(x, n_in, "x")
     dy, ldd = _rows(dy, n_out, "dy")
     if slope is not None:
-        want = torch.float16 if x.dtype in _HALF else x.dtype
+        want = SLOPE[x.dtype]
         if slope.dtype != want or slope.device != x.device:
             raise TypeError(f"slope is {slope.dtype} on {slope.device}: {want} on {x.device} is needed, as dense(..., want_slope=True) returns it")
         _same_shape(slope, (*x_shape[:-1], n_out), "slope")
