@@ -9,13 +9,10 @@ namespace {
 
 // ---- the epilogue ------------------------------------------------------------------------------------------------------------------
 
-// act(z) and act'(z)
+// act(z) and act'(z), to a few units of the arithmetic type's last place
 template <typename A>
-__device__ __forceinline__ void activate(int act, A z, A& a, A& slope) {
-  if (act == VMCPDE_ACT_NONE) {
-    a = z;
-    slope = 1;
-  } else if (act == VMCPDE_ACT_TANH) {
+__device__ __forceinline__ void activate_exact(int act, A z, A& a, A& slope) {
+  if (act == VMCPDE_ACT_TANH) {
     a = sizeof(A) == 8 ? (A)tanh((double)z) : (A)tanhf((float)z);
     slope = 1 - a * a;
   } else if (act == VMCPDE_ACT_GELU) {
@@ -28,13 +25,49 @@ __device__ __forceinline__ void activate(int act, A z, A& a, A& slope) {
       density = 0.39894228f * expf(-0.5f * z * z);
     }
     a = z * cdf;
-    slope = density != 0 ? cdf + z * density : cdf;      // (z = -inf: no inf * 0)
+    slope = density != 0 ? cdf + z * density : cdf;      // (z = +-inf: no inf * 0)
     if (z == -(A)INFINITY) a = 0;
   } else {
     const A e = sizeof(A) == 8 ? (A)exp(-(double)z) : (A)expf(-(float)z);
     const A gate = 1 / (1 + e);
     a = z == -(A)INFINITY ? 0 : z * gate;
     slope = gate != 0 && gate != 1 ? gate * (1 + z * (1 - gate)) : gate;
+  }
+}
+
+// The same beside 16-bit elements, some 1e-7 absolute (2e-7 relative for small tanh), a tenth of the instructions: with the library's functions the
+// epilogue of a large product took as long as a quarter of its multiplications.  erf: the rational approximation 7.1.26 of Abramowitz and Stegun.
+__device__ __forceinline__ void activate_short(int act, float z, float& a, float& slope) {
+  const float x = fabsf(z);
+  if (act == VMCPDE_ACT_TANH) {
+    const float e = __expf(-2 * x), y = z * z;
+    const float large = copysignf((1 - e) * __builtin_amdgcn_rcpf(1 + e), z);
+    const float small = z * (1 + y * (-0.33333333f + y * (0.13333333f - y * 0.053968254f)));
+    a = x < 0.2f ? small : large;
+    slope = x < 0.2f ? 1 - a * a : 4 * e * __builtin_amdgcn_rcpf((1 + e) * (1 + e));
+  } else if (act == VMCPDE_ACT_GELU) {
+    const float e = __expf(-0.5f * z * z), t = __builtin_amdgcn_rcpf(1 + 0.3275911f * 0.70710678f * x);
+    const float tail = 0.5f * e * t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
+    const float cdf = z < 0 ? tail : 1 - tail;
+    a = z == -INFINITY ? 0 : z * cdf;
+    slope = e != 0 ? cdf + z * (0.39894228f * e) : cdf;
+    if (z != z) a = slope = z;
+  } else {
+    const float gate = __builtin_amdgcn_rcpf(1 + __expf(-z));
+    a = z == -INFINITY ? 0 : z * gate;
+    slope = gate != 0 && gate != 1 ? gate * (1 + z * (1 - gate)) : gate;
+  }
+}
+
+template <typename T, typename A>
+__device__ __forceinline__ void activate(int act, A z, A& a, A& slope) {
+  if (act == VMCPDE_ACT_NONE) {
+    a = z;
+    slope = 1;
+  } else if constexpr (sizeof(T) == 2) {
+    activate_short(act, z, a, slope);
+  } else {
+    activate_exact<A>(act, z, a, slope);
   }
 }
 
@@ -51,39 +84,24 @@ struct Epilogue {
   int32_t act;
 };
 
-template <typename T, typename A>
-__device__ __forceinline__ void finish(const Epilogue<T>& e, int64_t row, int64_t col, A z) {
-  A a, slope;
-  if (e.bias) z += (A)e.bias[col];
-  activate<A>(e.act, z, a, slope);
-  a *= e.scale;
-  if (e.residual) a += (A)e.residual[row * e.ldr + col];
-  e.y[row * e.ldy + col] = (T)a;
-  if (e.slope) e.slope[row * e.n + col] = (typename Slope<T>::type)slope;
-}
-
-// columns col .. col + 4 of a row (those inside it)
-template <typename T, typename A>
-__device__ __forceinline__ void finish4(const Epilogue<T>& e, int64_t row, int64_t col, const A (&z)[4]) {
-  A a[4], slope[4], more[4];
-#pragma unroll
-  for (int k = 0; k < 4; ++k) a[k] = z[k];
+// columns col .. col + N of a row (those inside it), from their sums
+template <typename T, int N, typename A>
+__device__ __forceinline__ void finish(const Epilogue<T>& e, int64_t row, int64_t col, A (&z)[N]) {
+  A slope[N], more[N];
   if (e.bias) {
-    load_vec<T, 4>(e.bias, col, e.n, more);
+    load_vec<T, N>(e.bias, col, e.n, more);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) a[k] += more[k];
+    for (int k = 0; k < N; ++k) z[k] += more[k];
   }
+  if (e.residual) load_vec<T, N>(e.residual + row * e.ldr, col, e.n, more);
 #pragma unroll
-  for (int k = 0; k < 4; ++k) activate<A>(e.act, a[k], a[k], slope[k]);
-#pragma unroll
-  for (int k = 0; k < 4; ++k) a[k] *= e.scale;
-  if (e.residual) {
-    load_vec<T, 4>(e.residual + row * e.ldr, col, e.n, more);
-#pragma unroll
-    for (int k = 0; k < 4; ++k) a[k] += more[k];
+  for (int k = 0; k < N; ++k) {
+    activate<T, A>(e.act, z[k], z[k], slope[k]);
+    z[k] *= e.scale;
+    if (e.residual) z[k] += more[k];
   }
-  store_vec<T, 4>(e.y + row * e.ldy, col, e.n, a);
-  if (e.slope) store_vec<typename Slope<T>::type, 4>(e.slope + row * e.n, col, e.n, slope);
+  store_vec<T, N>(e.y + row * e.ldy, col, e.n, z);
+  if (e.slope) store_vec<typename Slope<T>::type, N>(e.slope + row * e.n, col, e.n, slope);
 }
 
 // ---- products ----------------------------------------------------------------------------------------------------------------------
@@ -194,7 +212,10 @@ __global__ __launch_bounds__(256) void product_wide_kernel(Product g, int tiles_
         const int col = col0 + wc + b * 16 + i;
         if (col >= g.n) continue;
         if (part) part[((int64_t)blockIdx.y * g.m + row) * g.n + col] = acc[a][b][reg];
-        else finish<T, A>(e, row, col, acc[a][b][reg]);
+        else {
+          A z[1] = {acc[a][b][reg]};
+          finish<T, 1>(e, row, col, z);
+        }
       }
     }
 }
@@ -298,8 +319,8 @@ struct HalfTile {
 };
 
 // BM x BN of C by WM x WN waves; k in [k_begin, k_end) (k_begin a multiple of HK).  Two buffers: a step's fetches fly while the step before
-// is multiplied.  The column operand goes in as the matrix instruction's first, so a lane's four results lie along a row of C:
-// out(row, col, v): C[row][col .. col + 4].
+// is multiplied.  The column operand goes in as the matrix instruction's first, so a lane's four results lie along a row of C.
+// out(row, col, v): the sums of C[row][col .. col + N].
 template <typename H, int BM, int BN, int WM, int WN, bool PX, bool QX, typename F>
 __device__ __forceinline__ void half_product(const Product& g, int row0, int col0, int k_begin, int k_end, F out) {
   constexpr int THREADS = 64 * WM * WN, TM = BM / WM / 16, TN = BN / WN / 16;
@@ -351,14 +372,33 @@ __device__ __forceinline__ void half_product(const Product& g, int row0, int col
     step(lds + at, lds + at + P::BYTES, lds + other, lds + other + P::BYTES, k_end - k - HK);
     at = other;
   }
+  // Sixteen rows at a time through a piece of LDS of the wave's own, so that a lane ends with N columns of a row and a row's lanes write whole lines.
+  // The loop stays rolled (the epilogue is long); the registers are picked by number inside it.
+  constexpr int N = TN >= 2 ? 8 : 4, COLS = TN * 16, PITCH = COLS + 4;
+  static_assert(WM * WN * 16 * PITCH * 4 <= 2 * (P::BYTES + Q::BYTES), "the rows fit the tiles' LDS");
+  __syncthreads();
+  float* rows = reinterpret_cast<float*>(tiles) + wave * 16 * PITCH;
   const int i = lane & 15, quad = (lane >> 4) * 4;
+#pragma unroll 1
+  for (int turn = 0; turn < TM; ++turn) {
 #pragma unroll
-  for (int a = 0; a < TM; ++a)
+    for (int a = 0; a < TM; ++a)
+      if (a == turn) {
 #pragma unroll
-    for (int b = 0; b < TN; ++b) {
-      const float v[4] = {acc[a][b][0], acc[a][b][1], acc[a][b][2], acc[a][b][3]};
-      out(row0 + wr + a * 16 + i, col0 + wc + b * 16 + quad, v);
+        for (int b = 0; b < TN; ++b) *reinterpret_cast<float4v*>(rows + i * PITCH + b * 16 + quad) = acc[a][b];
+      }
+#pragma unroll
+    for (int j = 0; j < 16 * COLS / N / 64; ++j) {
+      const int u = j * 64 + lane, r = u / (COLS / N), c = u % (COLS / N) * N;
+      float v[N];
+#pragma unroll
+      for (int k = 0; k < N; k += 4) {
+        const float4v f = *reinterpret_cast<const float4v*>(rows + r * PITCH + c + k);
+        v[k] = f[0], v[k + 1] = f[1], v[k + 2] = f[2], v[k + 3] = f[3];
+      }
+      out(row0 + wr + turn * 16 + r, col0 + wc + c, v);
     }
+  }
 }
 
 // C in BM x BN tiles, slice blockIdx.y of the k range (`part` != null: its sums).  Workgroups go round the eight XCDs by their number: each
@@ -370,10 +410,11 @@ __global__ __launch_bounds__(64 * WM * WN) void product_half_kernel(Product g, i
   const int band = tile / (8 * tiles_n), in_band = tile - band * 8 * tiles_n, height = min(8, tiles_m - band * 8);
   const int row0 = (band * 8 + in_band % height) * BM, col0 = (in_band / height) * BN;
   const int k_begin = blockIdx.y * k_slice, k_end = min(k_begin + k_slice, g.k);
-  half_product<H, BM, BN, WM, WN, PX, QX>(g, row0, col0, k_begin, k_end, [&](int row, int col, const float (&v)[4]) {
+  half_product<H, BM, BN, WM, WN, PX, QX>(g, row0, col0, k_begin, k_end, [&](int row, int col, auto& v) {
+    constexpr int N = sizeof(v) / sizeof(float);
     if (row >= g.m || col >= g.n) return;
-    if (part) store_vec<float, 4>(part + ((int64_t)blockIdx.y * g.m + row) * g.n, col, g.n, v);
-    else finish4<H>(e, row, col, v);
+    if (part) store_vec<float, N>(part + ((int64_t)blockIdx.y * g.m + row) * g.n, col, g.n, v);
+    else finish<H, N>(e, row, col, v);
   });
 }
 
@@ -391,7 +432,7 @@ __global__ __launch_bounds__(256) void product_join_kernel(const typename Wide<T
 #pragma unroll
     for (int k = 0; k < 4; ++k) z[k] += v[k];
   }
-  finish4<T>(e, row, col, z);
+  finish<T, 4>(e, row, col, z);
 }
 
 // ---- the gradient before the activation ----------------------------------------------------------------------------------------------
