@@ -113,150 +113,79 @@ struct Product {
   const void* q;
   int64_t ldp, ldq;
   int32_t m, n, k;
-  int32_t p_across, q_across;
-  int32_t kp, kq;          // 16-bit products: k that P and Q hold (k may be rounded up to whole chunks; what lies behind is zero)
+  int32_t kp, kq;          // what P and Q hold along k (k may be rounded up to whole chunks; what lies behind is zero)
 };
-
-template <typename A> struct Acc;
-template <> struct Acc<float> { typedef float type __attribute__((ext_vector_type(4))); };
-template <> struct Acc<double> { typedef double type __attribute__((ext_vector_type(4))); };
-
-__device__ __forceinline__ Acc<float>::type mfma(float a, float b, Acc<float>::type c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
-__device__ __forceinline__ Acc<double>::type mfma(double a, double b, Acc<double>::type c) { return __builtin_amdgcn_mfma_f64_16x16x4f64(a, b, c, 0, 0, 0); }
-// row of the 16 x 16 block that register `reg` of a lane with lane / 16 = g holds (the column is lane % 16)
-template <typename A> __device__ __forceinline__ int block_row(int g, int reg) { return sizeof(A) == 8 ? g + 4 * reg : g * 4 + reg; }
-
-constexpr int WIDE_K = 16;
-
-// One step of an operand, 16 k x R rows: global -> registers, registers -> LDS [k][row].  Coalesced along whichever axis lies in memory.
-template <typename T, typename A, int R>
-struct WideStep {
-  static constexpr int E = R * WIDE_K / 256;
-  A v[E];
-  __device__ __forceinline__ void load(const T* __restrict__ base, int64_t ld, int across, int row0, int rows, int k0, int k_end) {
-    const int t = threadIdx.x;
-    const bool inside = row0 + R <= rows && k0 + WIDE_K <= k_end;
-#pragma unroll
-    for (int j = 0; j < E; ++j) {
-      const int r = row0 + (across ? t % R : t / WIDE_K + j * (256 / WIDE_K)), k = k0 + (across ? t / R + j * (256 / R) : t % WIDE_K);
-      v[j] = inside || (r < rows && k < k_end) ? (A)base[across ? k * ld + r : r * ld + k] : (A)0;
-    }
-  }
-  __device__ __forceinline__ void store(A* __restrict__ lds, int across) const {
-    const int t = threadIdx.x;
-#pragma unroll
-    for (int j = 0; j < E; ++j) {
-      const int r = across ? t % R : t / WIDE_K + j * (256 / WIDE_K), k = across ? t / R + j * (256 / R) : t % WIDE_K;
-      lds[k * (R + 16) + r] = v[j];
-    }
-  }
-};
-
-// BM x BN of C per workgroup of four waves, WM x WN blocks of 16 x 16 a wave; slice blockIdx.y of the k range, `part` != null: its sums
-template <typename T, int BM, int BN, int WAVES_M>
-__global__ __launch_bounds__(256) void product_wide_kernel(Product g, int tiles_n, int k_slice, typename Wide<T>::type* __restrict__ part, Epilogue<T> e) {
-  typedef typename Wide<T>::type A;
-  constexpr int WAVES_N = 4 / WAVES_M, WM = BM / WAVES_M / 16, WN = BN / WAVES_N / 16, LP = BM + 16, LQ = BN + 16;
-  __shared__ A lp[2][WIDE_K * LP], lq[2][WIDE_K * LQ];
-  const int row0 = (blockIdx.x / tiles_n) * BM, col0 = (blockIdx.x % tiles_n) * BN;
-  const int k_begin = blockIdx.y * k_slice, k_end = k_begin + k_slice < g.k ? k_begin + k_slice : g.k;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, q4 = lane >> 4;
-  const int wr = (wave / WAVES_N) * WM * 16, wc = (wave % WAVES_N) * WN * 16;
-  typename Acc<A>::type acc[WM][WN];
-#pragma unroll
-  for (int a = 0; a < WM; ++a)
-#pragma unroll
-    for (int b = 0; b < WN; ++b) acc[a][b] = {0, 0, 0, 0};
-  const T* p = static_cast<const T*>(g.p);
-  const T* q = static_cast<const T*>(g.q);
-  WideStep<T, A, BM> sp;
-  WideStep<T, A, BN> sq;
-  sp.load(p, g.ldp, g.p_across, row0, g.m, k_begin, k_end);
-  sq.load(q, g.ldq, g.q_across, col0, g.n, k_begin, k_end);
-  sp.store(lp[0], g.p_across);
-  sq.store(lq[0], g.q_across);
-  __syncthreads();
-  int buf = 0;
-  for (int k0 = k_begin; k0 < k_end; k0 += WIDE_K, buf ^= 1) {
-    const bool more = k0 + WIDE_K < k_end;
-    if (more) {
-      sp.load(p, g.ldp, g.p_across, row0, g.m, k0 + WIDE_K, k_end);
-      sq.load(q, g.ldq, g.q_across, col0, g.n, k0 + WIDE_K, k_end);
-    }
-#pragma unroll
-    for (int s = 0; s < WIDE_K / 4; ++s) {
-      A fp[WM], fq[WN];
-#pragma unroll
-      for (int a = 0; a < WM; ++a) fp[a] = lp[buf][(s * 4 + q4) * LP + wr + a * 16 + i];
-#pragma unroll
-      for (int b = 0; b < WN; ++b) fq[b] = lq[buf][(s * 4 + q4) * LQ + wc + b * 16 + i];
-#pragma unroll
-      for (int a = 0; a < WM; ++a)
-#pragma unroll
-        for (int b = 0; b < WN; ++b) acc[a][b] = mfma(fp[a], fq[b], acc[a][b]);
-    }
-    if (more) {
-      sp.store(lp[buf ^ 1], g.p_across);      // (the other buffer: its last readers passed the barrier of the step before)
-      sq.store(lq[buf ^ 1], g.q_across);
-    }
-    __syncthreads();
-  }
-#pragma unroll
-  for (int a = 0; a < WM; ++a)
-#pragma unroll
-    for (int reg = 0; reg < 4; ++reg) {
-      const int row = row0 + wr + a * 16 + block_row<A>(q4, reg);
-      if (row >= g.m) continue;
-#pragma unroll
-      for (int b = 0; b < WN; ++b) {
-        const int col = col0 + wc + b * 16 + i;
-        if (col >= g.n) continue;
-        if (part) part[((int64_t)blockIdx.y * g.m + row) * g.n + col] = acc[a][b][reg];
-        else {
-          A z[1] = {acc[a][b][reg]};
-          finish<T, 1>(e, row, col, z);
-        }
-      }
-    }
-}
-
-// ---- 16-bit products on the matrix pipe --------------------------------------------------------------------------------------------------
 
 typedef short short8 __attribute__((ext_vector_type(8)));
 typedef short short4v __attribute__((ext_vector_type(4)));
 typedef float float4v __attribute__((ext_vector_type(4)));
+typedef double double2v __attribute__((ext_vector_type(2)));
+typedef double double4v __attribute__((ext_vector_type(4)));
 typedef bf16_t bf16x8 __attribute__((ext_vector_type(8)));
 typedef f16_t f16x8 __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) char lds_char;
 typedef __attribute__((address_space(3))) short4v lds_short4;
-typedef __attribute__((address_space(3))) short8 lds_short8;
 
-constexpr int HK = 64;                    // k a step
+constexpr int LINE = 128;                 // bytes of k a step: 64 16-bit numbers, 32 fp32, 16 fp64
 constexpr int OUTSIDE = 0x7ffffff0;       // byte offset behind every record: such a lane reads zeros
+template <typename T> constexpr int step_of() { return LINE / (int)sizeof(T); }
 
-__device__ __forceinline__ float4v mfma16(bf16_t, short8 a, short8 b, float4v c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-}
-__device__ __forceinline__ float4v mfma16(f16_t, short8 a, short8 b, float4v c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-}
+// What a lane holds of 16 rows: 16 bytes, E numbers behind each other in k; four groups of 16 lanes hold 4 E of them.  One instruction of 32 k for
+// the 16-bit types; fp32 and fp64 instructions take four k, one of each group, so E of them take the numbers one by one.
+template <typename T> struct Matrix;
+template <> struct Matrix<bf16_t> {
+  typedef short8 Frag;
+  typedef float4v Acc;
+  static __device__ __forceinline__ Acc mfma(Frag a, Frag b, Acc c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  }
+};
+template <> struct Matrix<f16_t> {
+  typedef short8 Frag;
+  typedef float4v Acc;
+  static __device__ __forceinline__ Acc mfma(Frag a, Frag b, Acc c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  }
+};
+template <> struct Matrix<float> {
+  typedef float4v Frag;
+  typedef float4v Acc;
+  static __device__ __forceinline__ Acc mfma(Frag a, Frag b, Acc c) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], c, 0, 0, 0);
+    return c;
+  }
+};
+template <> struct Matrix<double> {
+  typedef double2v Frag;
+  typedef double4v Acc;
+  static __device__ __forceinline__ Acc mfma(Frag a, Frag b, Acc c) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) c = __builtin_amdgcn_mfma_f64_16x16x4f64(a[j], b[j], c, 0, 0, 0);
+    return c;
+  }
+};
 
-// One operand's tile, R rows x HK of k, 16-byte chunks straight from memory into LDS.  Along k: [row][8 chunks], chunk c of row r at
-// place c ^ (r & 7).  Across: [k][R / 8 chunks], chunk c of line k at place c ^ s(k); there the transposing LDS read hands a lane four k of
-// its row.  The places are permuted on the memory side (a lane fetches the chunk that belongs where it writes), so that the fragment
-// reads of a wave fall on different banks.
-template <int R, bool ACROSS, int THREADS>
-struct HalfTile {
-  static constexpr int LOADS = R * HK / 8 / THREADS;
-  static constexpr int BYTES = R * HK * 2;
-  static constexpr int PER_LINE = R / 8;                       // chunks of a line of k
+// One operand's tile, R rows x one step of k, 16-byte chunks straight from memory into LDS.  Along k: [row][8 chunks], chunk c of row r at
+// place c ^ (r & 7).  Across: [k][chunks of R rows], chunk c of line k at place c ^ swizzle(k); there a lane gathers its k line by line, by the
+// transposing LDS read for the 16-bit types.  The places are permuted on the memory side (a lane fetches the chunk that belongs where it
+// writes), so that the fragment reads of a wave fall on different banks.
+template <typename T, int R, bool ACROSS, int THREADS>
+struct Tile {
+  typedef typename Matrix<T>::Frag Frag;
+  static constexpr int SIZE = sizeof(T), E = 16 / SIZE, STEP = step_of<T>();
+  static constexpr int LOADS = R * 8 / THREADS, BYTES = R * LINE;
+  static constexpr int PER_LINE = R / E;                       // chunks of a line of k
+  static_assert(LOADS >= 1, "a chunk for every thread");
   const char* base;
   int64_t left, step;                                          // bytes from base to the operand's end; bytes a step of k moves on
   int offset[LOADS], chunk_k[LOADS];
-  int frag, line;                                              // this lane's place in a fragment read
+  int frag;                                                    // this lane's place in a fragment read
 
-  static __device__ __forceinline__ int swizzle(int k) {       // lines k whose reads meet: k & 3 and bit 3 of k
-    if constexpr (PER_LINE >= 16) return 2 * ((k & 3) | ((k >> 1) & 4));
+  static __device__ __forceinline__ int swizzle(int k) {       // lines whose reads meet on the same banks without it
+    if constexpr (SIZE == 8) return 8 * ((k >> 1) & 1);
+    else if constexpr (SIZE == 4) return PER_LINE >= 16 ? 4 * ((k >> 2) & 3) : 4 * ((k >> 2) & 1);
+    else if constexpr (PER_LINE >= 16) return 2 * ((k & 3) | ((k >> 1) & 4));
     else if constexpr (PER_LINE == 8) return 2 * (((k >> 1) & 1) | ((k >> 2) & 2));
     else return 2 * ((k >> 3) & 1);
   }
@@ -266,29 +195,30 @@ struct HalfTile {
     const int t = threadIdx.x, lane = t & 63, i = lane & 15, g = lane >> 4;
     const int64_t first = ACROSS ? (int64_t)k0 * ld + row0 : (int64_t)row0 * ld + k0;
     const int64_t end = ACROSS ? (int64_t)(k_total - 1) * ld + rows : (int64_t)(rows - 1) * ld + k_total;
-    base = static_cast<const char*>(p) + first * 2;
-    left = ((end - first) * 2 + 3) & ~(int64_t)3;              // the record ends with a whole dword (an odd width's last one: half of it is used)
-    step = (ACROSS ? HK * ld : HK) * 2;
+    base = static_cast<const char*>(p) + first * SIZE;
+    left = ((end - first) * SIZE + 3) & ~(int64_t)3;           // the record ends with a whole dword (of an odd 16-bit width's last one half is used)
+    step = ACROSS ? STEP * ld * SIZE : LINE;
 #pragma unroll
     for (int j = 0; j < LOADS; ++j) {
       const int u = j * THREADS + t;
       if constexpr (ACROSS) {
         const int k = u / PER_LINE, c = (u % PER_LINE) ^ swizzle(k);
-        offset[j] = k * (int)ld * 2 + c * 16;
+        offset[j] = k * (int)ld * SIZE + c * 16;
         chunk_k[j] = 0;
       } else {
         const int r = u / 8, c = (u % 8) ^ (r & 7);
-        offset[j] = r * (int)ld * 2 + c * 16;
-        chunk_k[j] = c * 8;
+        offset[j] = r * (int)ld * SIZE + c * 16;
+        chunk_k[j] = c * E;
       }
     }
-    if constexpr (ACROSS) {
-      line = g * 8 + (i >> 2);
-      const int c = row_w / 8 + ((i & 3) >> 1);
-      frag = line * (R * 2) + ((c ^ swizzle(line)) << 4) + (i & 1) * 8;
+    if constexpr (!ACROSS) {
+      frag = (row_w + i) * LINE + ((g ^ (i & 7)) << 4);
+    } else if constexpr (SIZE == 2) {
+      const int k = g * 8 + (i >> 2), c = row_w / 8 + ((i & 3) >> 1);
+      frag = k * (R * 2) + ((c ^ swizzle(k)) << 4) + (i & 1) * 8;
     } else {
-      line = 0;
-      frag = (row_w + i) * 128 + ((g ^ (i & 7)) << 4);
+      const int k = g * E, c = (row_w + i) / E;                // (the lane's E lines have one swizzle)
+      frag = k * (R * SIZE) + ((c ^ swizzle(k)) << 4) + (i % E) * SIZE;
     }
   }
 
@@ -306,26 +236,35 @@ struct HalfTile {
     left -= step;
   }
 
-  // rows row_w + 16 t .. + 16, k = 32 s + 8 (lane / 16) .. + 8 of the tile
-  __device__ __forceinline__ short8 fragment(const lds_char* tile, int t, int s) const {
-    if constexpr (ACROSS) {
+  // rows row_w + 16 t .. + 16, half s of the step's k
+  __device__ __forceinline__ Frag fragment(const lds_char* tile, int t, int s) const {
+    if constexpr (!ACROSS) {
+      return *(const __attribute__((address_space(3))) Frag*)(tile + ((frag ^ (s << 6)) + t * 16 * LINE));
+    } else if constexpr (SIZE == 2) {
       const lds_char* a = tile + ((frag ^ (t << 5)) + s * 32 * R * 2);
       const short4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)a), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(a + 4 * R * 2));
       return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
     } else {
-      return *(const lds_short8*)(tile + ((frag ^ (s << 6)) + t * 2048));
+      const lds_char* a = tile + ((frag ^ (t * 16 * SIZE)) + s * (STEP / 2) * R * SIZE);
+      Frag f;
+#pragma unroll
+      for (int j = 0; j < E; ++j) f[j] = *(const __attribute__((address_space(3))) T*)(a + j * R * SIZE);
+      return f;
     }
   }
 };
 
-// BM x BN of C by WM x WN waves; k in [k_begin, k_end) (k_begin a multiple of HK).  Two buffers: a step's fetches fly while the step before
-// is multiplied.  The column operand goes in as the matrix instruction's first, so a lane's four results lie along a row of C.
+// BM x BN of C by WM x WN waves; k in [k_begin, k_end) (k_begin a multiple of the step).  Two buffers: a step's fetches fly while the step before
+// is multiplied.  The column operand goes in as the matrix instruction's first, so a lane's results lie along a row of C.
 // out(row, col, v): the sums of C[row][col .. col + N].
-template <typename H, int BM, int BN, int WM, int WN, bool PX, bool QX, typename F>
-__device__ __forceinline__ void half_product(const Product& g, int row0, int col0, int k_begin, int k_end, F out) {
-  constexpr int THREADS = 64 * WM * WN, TM = BM / WM / 16, TN = BN / WN / 16;
-  typedef HalfTile<BM, PX, THREADS> P;
-  typedef HalfTile<BN, QX, THREADS> Q;
+template <typename T, int BM, int BN, int WM, int WN, bool PX, bool QX, typename F>
+__device__ __forceinline__ void tile_product(const Product& g, int row0, int col0, int k_begin, int k_end, F out) {
+  typedef typename Wide<T>::type A;
+  typedef typename Matrix<T>::Acc Acc;
+  typedef typename Matrix<T>::Frag Frag;
+  constexpr int THREADS = 64 * WM * WN, TM = BM / WM / 16, TN = BN / WN / 16, STEP = step_of<T>();
+  typedef Tile<T, BM, PX, THREADS> P;
+  typedef Tile<T, BN, QX, THREADS> Q;
   __shared__ __attribute__((aligned(16))) char tiles[2 * (P::BYTES + Q::BYTES)];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const int wr = (wave / WN) * TM * 16, wc = (wave % WN) * TN * 16;
@@ -333,23 +272,28 @@ __device__ __forceinline__ void half_product(const Product& g, int row0, int col
   Q q;
   p.init(g.p, g.ldp, g.m, min(k_end, g.kp), row0, k_begin, wr);
   q.init(g.q, g.ldq, g.n, min(k_end, g.kq), col0, k_begin, wc);
-  float4v acc[TM][TN];
+  Acc acc[TM][TN];
 #pragma unroll
   for (int a = 0; a < TM; ++a)
 #pragma unroll
     for (int b = 0; b < TN; ++b) acc[a][b] = {0, 0, 0, 0};
-  auto multiply = [&](const lds_char* tp, const lds_char* tq) {
+  // (the two buffers as parameters that do not overlap: otherwise every fragment read waits for the fetches into the other buffer)
+  auto step = [&](lds_char* __restrict__ now_p, lds_char* __restrict__ now_q, lds_char* __restrict__ next_p, lds_char* __restrict__ next_q, int k_left) {
+    if (k_left > 0) {
+      p.fetch(next_p, k_left);
+      q.fetch(next_q, k_left);
+    }
 #pragma unroll
-    for (int s = 0; s < HK / 32; ++s) {
-      short8 fp[TM], fq[TN];
+    for (int s = 0; s < 2; ++s) {
+      Frag fp[TM], fq[TN];
 #pragma unroll
-      for (int b = 0; b < TN; ++b) fq[b] = q.fragment(tq, b, s);
+      for (int b = 0; b < TN; ++b) fq[b] = q.fragment(now_q, b, s);
 #pragma unroll
-      for (int a = 0; a < TM; ++a) fp[a] = p.fragment(tp, a, s);
+      for (int a = 0; a < TM; ++a) fp[a] = p.fragment(now_p, a, s);
 #pragma unroll
       for (int a = 0; a < TM; ++a)
 #pragma unroll
-        for (int b = 0; b < TN; ++b) acc[a][b] = mfma16(H(), fq[b], fp[a], acc[a][b]);
+        for (int b = 0; b < TN; ++b) acc[a][b] = Matrix<T>::mfma(fq[b], fp[a], acc[a][b]);
     }
   };
   lds_char* const lds = (lds_char*)tiles;
@@ -358,44 +302,41 @@ __device__ __forceinline__ void half_product(const Product& g, int row0, int col
     p.fetch(lds, k_end - k_begin);
     q.fetch(lds + P::BYTES, k_end - k_begin);
   }
-  auto step = [&](lds_char* __restrict__ now_p, lds_char* __restrict__ now_q, lds_char* __restrict__ next_p, lds_char* __restrict__ next_q, int k_left) {
-    if (k_left > 0) {
-      p.fetch(next_p, k_left);
-      q.fetch(next_q, k_left);
-    }
-    multiply(now_p, now_q);
-  };
-  for (int k = k_begin; k < k_end; k += HK) {
+  for (int k = k_begin; k < k_end; k += STEP) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();                      // this step's tiles are there, and the other buffer's readers are done
     const int other = at ^ (P::BYTES + Q::BYTES);
-    step(lds + at, lds + at + P::BYTES, lds + other, lds + other + P::BYTES, k_end - k - HK);
+    step(lds + at, lds + at + P::BYTES, lds + other, lds + other + P::BYTES, k_end - k - STEP);
     at = other;
   }
   // Sixteen rows at a time through a piece of LDS of the wave's own, so that a lane ends with N columns of a row and a row's lanes write whole lines.
   // The loop stays rolled (the epilogue is long); the registers are picked by number inside it.
-  constexpr int N = TN >= 2 ? 8 : 4, COLS = TN * 16, PITCH = COLS + 4;
-  static_assert(WM * WN * 16 * PITCH * 4 <= 2 * (P::BYTES + Q::BYTES), "the rows fit the tiles' LDS");
+  constexpr int N = sizeof(T) == 8 ? 2 : sizeof(T) == 4 || TN == 1 ? 4 : 8, COLS = TN * 16, PITCH = COLS + 4;
+  static_assert(WM * WN * 16 * PITCH * (int)sizeof(A) <= 2 * (P::BYTES + Q::BYTES), "the rows fit the tiles' LDS");
   __syncthreads();
-  float* rows = reinterpret_cast<float*>(tiles) + wave * 16 * PITCH;
-  const int i = lane & 15, quad = (lane >> 4) * 4;
+  A* rows = reinterpret_cast<A*>(tiles) + wave * 16 * PITCH;
+  const int i = lane & 15, group = lane >> 4;
 #pragma unroll 1
   for (int turn = 0; turn < TM; ++turn) {
 #pragma unroll
     for (int a = 0; a < TM; ++a)
       if (a == turn) {
 #pragma unroll
-        for (int b = 0; b < TN; ++b) *reinterpret_cast<float4v*>(rows + i * PITCH + b * 16 + quad) = acc[a][b];
+        for (int b = 0; b < TN; ++b) {
+          if constexpr (sizeof(A) == 4) {
+            *reinterpret_cast<float4v*>(rows + i * PITCH + b * 16 + group * 4) = acc[a][b];
+          } else {                        // (the fp64 instruction's registers are four rows apart, not one)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) rows[i * PITCH + b * 16 + group + 4 * r] = acc[a][b][r];
+          }
+        }
       }
 #pragma unroll
     for (int j = 0; j < 16 * COLS / N / 64; ++j) {
       const int u = j * 64 + lane, r = u / (COLS / N), c = u % (COLS / N) * N;
-      float v[N];
+      A v[N];
 #pragma unroll
-      for (int k = 0; k < N; k += 4) {
-        const float4v f = *reinterpret_cast<const float4v*>(rows + r * PITCH + c + k);
-        v[k] = f[0], v[k + 1] = f[1], v[k + 2] = f[2], v[k + 3] = f[3];
-      }
+      for (int k = 0; k < N; ++k) v[k] = rows[r * PITCH + c + k];
       out(row0 + wr + turn * 16 + r, col0 + wc + c, v);
     }
   }
@@ -403,18 +344,21 @@ __device__ __forceinline__ void half_product(const Product& g, int row0, int col
 
 // C in BM x BN tiles, slice blockIdx.y of the k range (`part` != null: its sums).  Workgroups go round the eight XCDs by their number: each
 // XCD takes one contiguous eighth of the tiles, in bands of eight tile rows, so that the operands a band shares stay in its L2.
-template <typename H, int BM, int BN, int WM, int WN, bool PX, bool QX>
-__global__ __launch_bounds__(64 * WM * WN) void product_half_kernel(Product g, int tiles_m, int tiles_n, int k_slice, float* __restrict__ part, Epilogue<H> e) {
+template <typename T, int BM, int BN, int WM, int WN, bool PX, bool QX>
+__global__ __launch_bounds__(64 * WM * WN) void product_kernel(Product g, int tiles_m, int tiles_n, int k_slice, typename Wide<T>::type* __restrict__ part,
+                                                               Epilogue<T> e) {
+  typedef typename Wide<T>::type A;
   const int tiles = tiles_m * tiles_n, id = blockIdx.x, xcd = id & 7, each = tiles >> 3, more = tiles & 7;
   const int tile = xcd * each + (xcd < more ? xcd : more) + (id >> 3);
-  const int band = tile / (8 * tiles_n), in_band = tile - band * 8 * tiles_n, height = min(8, tiles_m - band * 8);
+  const int64_t per_band = (int64_t)8 * tiles_n;
+  const int band = (int)(tile / per_band), in_band = (int)(tile - band * per_band), height = min(8, tiles_m - band * 8);
   const int row0 = (band * 8 + in_band % height) * BM, col0 = (in_band / height) * BN;
   const int k_begin = blockIdx.y * k_slice, k_end = min(k_begin + k_slice, g.k);
-  half_product<H, BM, BN, WM, WN, PX, QX>(g, row0, col0, k_begin, k_end, [&](int row, int col, auto& v) {
-    constexpr int N = sizeof(v) / sizeof(float);
+  tile_product<T, BM, BN, WM, WN, PX, QX>(g, row0, col0, k_begin, k_end, [&](int row, int col, auto& v) {
+    constexpr int N = sizeof(v) / sizeof(A);
     if (row >= g.m || col >= g.n) return;
-    if (part) store_vec<float, N>(part + ((int64_t)blockIdx.y * g.m + row) * g.n, col, g.n, v);
-    else finish<H, N>(e, row, col, v);
+    if (part) store_vec<A, N>(part + ((int64_t)blockIdx.y * g.m + row) * g.n, col, g.n, v);
+    else finish<T, N>(e, row, col, v);
   });
 }
 
@@ -478,8 +422,6 @@ __global__ __launch_bounds__(256) void dense_dz_kernel(const T* __restrict__ dy,
 
 // ---- plans ---------------------------------------------------------------------------------------------------------------------------
 
-template <typename T> constexpr bool is_half() { return sizeof(T) == 2; }
-
 struct Tiles { int bm, bn, slices, k_slice; };
 
 // Tile and k slices of a product.  128 x 128 fills the matrix pipe; sides of at most 32 rows or columns take 32, so that little is multiplied for
@@ -487,11 +429,11 @@ struct Tiles { int bm, bn, slices, k_slice; };
 // idle the k range is cut, and the slices' sums are joined by a second launch.
 template <typename T>
 Tiles tiles_of(int64_t m, int64_t n, int64_t k) {
-  constexpr int64_t step = is_half<T>() ? HK : WIDE_K;
+  constexpr int64_t step = step_of<T>();
   Tiles t;
   t.bm = m <= 32 ? 32 : 128;
   t.bn = n <= 32 ? 32 : 128;
-  if (is_half<T>() && ceil_div(m, 256) * ceil_div(n, 256) >= 192) t.bm = t.bn = 256;
+  if (sizeof(T) == 2 && ceil_div(m, 256) * ceil_div(n, 256) >= 192) t.bm = t.bn = 256;
   const int64_t tiles = ceil_div(m, t.bm) * ceil_div(n, t.bn);
   int64_t slices = 1;
   if (tiles > 0 && tiles < 256) slices = std::min<int64_t>(std::min<int64_t>(ceil_div(512, tiles), ceil_div(k, 4 * step)), 512);
@@ -509,33 +451,24 @@ int64_t product_bytes(int64_t m, int64_t n, int64_t k) {
 }
 
 template <typename T, int BM, int BN, int WM, int WN>
-void product_half(const Product& g, const Tiles& t, float* part, const Epilogue<T>& e, hipStream_t s) {
+void product_as(const Product& g, bool p_across, bool q_across, const Tiles& t, typename Wide<T>::type* part, const Epilogue<T>& e, hipStream_t s) {
   const int tiles_m = (int)ceil_div(g.m, BM), tiles_n = (int)ceil_div(g.n, BN);
   const dim3 grid((unsigned)(tiles_m * tiles_n), (unsigned)t.slices);
-  if (!g.p_across && g.q_across) product_half_kernel<T, BM, BN, WM, WN, false, true><<<grid, 64 * WM * WN, 0, s>>>(g, tiles_m, tiles_n, t.k_slice, part, e);
-  else if (!g.p_across) product_half_kernel<T, BM, BN, WM, WN, false, false><<<grid, 64 * WM * WN, 0, s>>>(g, tiles_m, tiles_n, t.k_slice, part, e);
-  else product_half_kernel<T, BM, BN, WM, WN, true, true><<<grid, 64 * WM * WN, 0, s>>>(g, tiles_m, tiles_n, t.k_slice, part, e);
+  if (p_across) product_kernel<T, BM, BN, WM, WN, true, true><<<grid, 64 * WM * WN, 0, s>>>(g, tiles_m, tiles_n, t.k_slice, part, e);      // (P across: x^T dz, Q too)
+  else if (q_across) product_kernel<T, BM, BN, WM, WN, false, true><<<grid, 64 * WM * WN, 0, s>>>(g, tiles_m, tiles_n, t.k_slice, part, e);
+  else product_kernel<T, BM, BN, WM, WN, false, false><<<grid, 64 * WM * WN, 0, s>>>(g, tiles_m, tiles_n, t.k_slice, part, e);
 }
 
 template <typename T>
-void product(const Product& g, const Epilogue<T>& e, void* workspace, hipStream_t s) {
+void product(const Product& g, bool p_across, bool q_across, const Epilogue<T>& e, void* workspace, hipStream_t s) {
   typedef typename Wide<T>::type A;
   const Tiles t = tiles_of<T>(g.m, g.n, g.k);
   A* part = t.slices > 1 ? static_cast<A*>(workspace) : nullptr;
-  if constexpr (is_half<T>()) {
-    if (t.bm == 256) product_half<T, 256, 256, 2, 4>(g, t, part, e, s);
-    else if (t.bm == 128 && t.bn == 128) product_half<T, 128, 128, 2, 2>(g, t, part, e, s);
-    else if (t.bm == 128) product_half<T, 128, 32, 4, 1>(g, t, part, e, s);
-    else if (t.bn == 128) product_half<T, 32, 128, 1, 4>(g, t, part, e, s);
-    else product_half<T, 32, 32, 2, 2>(g, t, part, e, s);
-  } else {
-    const int tiles_n = (int)ceil_div(g.n, t.bn);
-    const dim3 grid((unsigned)(ceil_div(g.m, t.bm) * tiles_n), (unsigned)t.slices);
-    if (t.bm == 128 && t.bn == 128) product_wide_kernel<T, 128, 128, 2><<<grid, 256, 0, s>>>(g, tiles_n, t.k_slice, part, e);
-    else if (t.bm == 128) product_wide_kernel<T, 128, 32, 4><<<grid, 256, 0, s>>>(g, tiles_n, t.k_slice, part, e);
-    else if (t.bn == 128) product_wide_kernel<T, 32, 128, 1><<<grid, 256, 0, s>>>(g, tiles_n, t.k_slice, part, e);
-    else product_wide_kernel<T, 32, 32, 2><<<grid, 256, 0, s>>>(g, tiles_n, t.k_slice, part, e);
-  }
+  if (t.bm == 128 && t.bn == 128) product_as<T, 128, 128, 2, 2>(g, p_across, q_across, t, part, e, s);
+  else if (t.bm == 128) product_as<T, 128, 32, 4, 1>(g, p_across, q_across, t, part, e, s);
+  else if (t.bm == 32 && t.bn == 128) product_as<T, 32, 128, 1, 4>(g, p_across, q_across, t, part, e, s);
+  else if (t.bm == 32) product_as<T, 32, 32, 2, 2>(g, p_across, q_across, t, part, e, s);
+  else if constexpr (sizeof(T) == 2) product_as<T, 256, 256, 2, 4>(g, p_across, q_across, t, part, e, s);
   if (part) product_join_kernel<T><<<(unsigned)ceil_div((int64_t)g.m * ((g.n + 3) / 4), 256), 256, 0, s>>>(part, t.slices, g.m, g.n, e);
 }
 
@@ -551,11 +484,11 @@ struct Lines {
   int64_t lines, n, ld;
 };
 
-// Whether the 16-bit products can fetch it: 16-byte chunks at 16-byte addresses, and whole chunks where its lines lie along k.  What they cannot is
+// Whether the products can fetch it: 16-byte chunks at 16-byte addresses, and whole chunks where its lines lie along k.  What they cannot is
 // copied into lines of whole chunks first, zeros behind each line's end.
 template <typename T>
 bool fetchable(const Lines& o, bool along_k) {
-  return !is_half<T>() || (aligned16(o.p) && o.ld % 8 == 0 && (!along_k || o.n % 8 == 0));
+  return aligned16(o.p) && o.ld % vec_of<T>() == 0 && (!along_k || o.n % vec_of<T>() == 0);
 }
 
 template <typename T>
@@ -598,7 +531,7 @@ struct Dense {
   // an operand that the products can fetch; `k_held` is what it holds along k where its lines lie along it
   Lines ready(Lines o, bool along_k) {
     if (fetchable<T>(o, along_k)) return o;
-    const int64_t ld = round_up(o.n, 8);
+    const int64_t ld = round_up(o.n, vec_of<T>());
     T* to = static_cast<T*>(take(o.lines * ld * (int64_t)sizeof(T)));
     if (launch && o.lines) scaled_copy<T>(o, nullptr, 1.0, to, ld, nullptr, copy_groups<T>(o), stream);
     return {to, o.lines, along_k ? ld : o.n, ld};
@@ -610,7 +543,7 @@ struct Dense {
     const int64_t kp = p_across ? p.lines : p.n, kq = q_across ? q.lines : q.n, k_all = std::max(k, std::max(kp, kq));
     const int64_t bytes = product_bytes<T>(m, n, k_all);
     void* rest = bytes ? take(bytes) : nullptr;
-    if (launch) product<T>({p.p, q.p, p.ld, q.ld, (int32_t)m, (int32_t)n, (int32_t)k_all, p_across, q_across, (int32_t)kp, (int32_t)kq}, e, rest, stream);
+    if (launch) product<T>({p.p, q.p, p.ld, q.ld, (int32_t)m, (int32_t)n, (int32_t)k_all, (int32_t)kp, (int32_t)kq}, p_across, q_across, e, rest, stream);
     used -= round_up(bytes, 256);
   }
 
@@ -631,7 +564,7 @@ struct Dense {
     const bool own = (a.dx || a.dkernel) && (a.slope || a.scale != 1.0 || !fetchable<T>(dy, a.dx));
     T* to = nullptr;
     if (own) {
-      const int64_t ld = is_half<T>() ? round_up(a.n_out, 8) : a.n_out;
+      const int64_t ld = round_up(a.n_out, vec_of<T>());
       to = static_cast<T*>(take(a.rows * ld * (int64_t)sizeof(T)));
       dz = {to, a.rows, a.n_out, ld};
     }
@@ -647,7 +580,7 @@ struct Dense {
     if (a.dx && a.rows) {
       const Epilogue<T> e = {nullptr, nullptr, 0, static_cast<T*>(a.dx), a.n_in, nullptr, a.n_in, 1, VMCPDE_ACT_NONE};
       Lines z = dz;
-      if (own) z.n = is_half<T>() ? dz.ld : dz.n;           // (zeros behind the line's end)
+      if (own) z.n = dz.ld;           // (zeros behind the line's end)
       multiply(z, false, kernel_lines(a), a.kernel_t, a.rows, a.n_in, a.n_out, e);
     }
     if (a.dkernel) {
@@ -676,14 +609,15 @@ int64_t walk_type(const vmcpde_dense_args& a, bool backward, void* workspace, hi
 }
 
 int check(const vmcpde_dense_args* a, bool backward) {
-  constexpr int64_t LIMIT = (int64_t)1 << 30, HALF_LIMIT = (int64_t)1 << 22;
+  constexpr int64_t LIMIT = (int64_t)1 << 30;
   VMC_REQUIRE(a, "dense: null arguments");
   VMC_REQUIRE(dtype_ok(a->dtype), "dense: type %d", a->dtype);
   VMC_REQUIRE(a->activation >= VMCPDE_ACT_NONE && a->activation <= VMCPDE_ACT_SILU, "dense: activation %d", a->activation);
   VMC_REQUIRE(a->rows >= 0 && a->rows < LIMIT && a->n_in >= 1 && a->n_in < LIMIT && a->n_out >= 1 && a->n_out < LIMIT,
               "dense: rows %lld, n_in %lld, n_out %lld (rows from 0, widths from 1, all below 2^30)", (long long)a->rows, (long long)a->n_in, (long long)a->n_out);
-  VMC_REQUIRE(dtype_size(a->dtype) > 2 || (std::max(a->n_in, a->n_out) < HALF_LIMIT && a->ldx < HALF_LIMIT && a->ldk < HALF_LIMIT && a->ldd < HALF_LIMIT),
-              "dense: widths and row pitches of 16-bit operands are below 2^22");     // (a tile's rows within 2^31 bytes of each other)
+  const int64_t pitch = (int64_t)1 << (a->dtype == VMCPDE_F64 ? 21 : 22);
+  VMC_REQUIRE(std::max(std::max(a->n_in, a->n_out), std::max(a->ldx, std::max(a->ldk, a->ldd))) < pitch, "dense: widths and row pitches are below %lld for this type",
+              (long long)pitch);     // (a tile's rows lie within 2^31 bytes of each other)
   VMC_REQUIRE(a->scale == a->scale, "dense: scale is NaN");
   VMC_REQUIRE(ceil_div(std::max(a->rows, a->n_in), 32) * ceil_div(std::max(a->n_in, a->n_out), 32) < (int64_t)1 << 31, "dense: more than 2^31 tiles");
   const int64_t kernel_row = a->kernel_t ? a->n_in : a->n_out;

@@ -103,7 +103,7 @@ def dense(x, kernel, bias=None, *, activation="none", scale=1.0, residual=None, 
 
     x (..., n_in); kernel (n_in, n_out), the layout of the flat parameter vector's leaves, or a transposed view of an (n_out, n_in) one; bias
     (n_out,); residual of y's shape.  activation: "none", "tanh", "gelu" (z Phi(z)), "silu".  `scale` is the output factor of the reference's
-    conditioners (net.py:50, 61: 10 * tanh).  Widths and row pitches of 16-bit operands are below 2^22.  With `want_slope` returns (y, slope): act'(z), which `dense_backward` takes (None for "none");
+    conditioners (net.py:50, 61: 10 * tanh).  Widths and row pitches are below 2^22 (2^21 in fp64).  With `want_slope` returns (y, slope): act'(z), which `dense_backward` takes (None for "none");
     of the type SLOPE[x.dtype] (fp16 for bf16, fp32 for fp16, else the element type)."""
     _check(x, kernel=kernel, bias=bias, residual=residual)
     if activation not in ACTIVATION:
