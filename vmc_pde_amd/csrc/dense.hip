@@ -345,7 +345,7 @@ __device__ __forceinline__ void tile_product(const Product& g, int row0, int col
 // C in BM x BN tiles, slice blockIdx.y of the k range (`part` != null: its sums).  Workgroups go round the eight XCDs by their number: each
 // XCD takes one contiguous eighth of the tiles, in bands of eight tile rows, so that the operands a band shares stay in its L2.
 template <typename T, int BM, int BN, int WM, int WN, bool PX, bool QX>
-__global__ __launch_bounds__(64 * WM * WN) void product_kernel(Product g, int tiles_m, int tiles_n, int k_slice, typename Wide<T>::type* __restrict__ part,
+__global__ __launch_bounds__(64 * WM * WN, BM * BN >= 256 * 256 ? 1 : 2) void product_kernel(Product g, int tiles_m, int tiles_n, int k_slice, typename Wide<T>::type* __restrict__ part,
                                                                Epilogue<T> e) {
   typedef typename Wide<T>::type A;
   const int tiles = tiles_m * tiles_n, id = blockIdx.x, xcd = id & 7, each = tiles >> 3, more = tiles & 7;
@@ -362,21 +362,35 @@ __global__ __launch_bounds__(64 * WM * WN) void product_kernel(Product g, int ti
   });
 }
 
-// the slices' sums added in their order, and the epilogue: four columns a lane
-template <typename T>
+// the slices' sums and the epilogue: four columns a lane.  PARTS lanes share them where there are many slices of a small product; a part's slices, then
+// the parts, are added in their order.
+template <typename T, int PARTS>
 __global__ __launch_bounds__(256) void product_join_kernel(const typename Wide<T>::type* __restrict__ part, int slices, int64_t m, int64_t n, Epilogue<T> e) {
   typedef typename Wide<T>::type A;
-  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x, quads = (n + 3) / 4, row = at / quads, col = (at - row * quads) * 4;
-  if (row >= m) return;
+  constexpr int LANES = 256 / PARTS;
+  __shared__ A sh[PARTS > 1 ? PARTS : 1][LANES][4];
+  const int lane = threadIdx.x % LANES, p = threadIdx.x / LANES;
+  const int64_t at = (int64_t)blockIdx.x * LANES + lane, quads = (n + 3) / 4, row = at / quads, col = (at - row * quads) * 4;
   A z[4] = {0, 0, 0, 0};
+  if (row < m) {
 #pragma unroll 4
-  for (int s = 0; s < slices; ++s) {
-    A v[4];
-    load_vec<A, 4>(part + ((int64_t)s * m + row) * n, col, n, v);
+    for (int s = p; s < slices; s += PARTS) {
+      A v[4];
+      load_vec<A, 4>(part + ((int64_t)s * m + row) * n, col, n, v);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) z[k] += v[k];
+      for (int k = 0; k < 4; ++k) z[k] += v[k];
+    }
   }
-  finish<T, 4>(e, row, col, z);
+  if constexpr (PARTS > 1) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) sh[p][lane][k] = z[k];
+    __syncthreads();
+    if (p) return;
+    for (int q = 1; q < PARTS; ++q)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) z[k] += sh[q][lane][k];
+  }
+  if (row < m) finish<T, 4>(e, row, col, z);
 }
 
 // ---- the gradient before the activation ----------------------------------------------------------------------------------------------
@@ -424,19 +438,23 @@ __global__ __launch_bounds__(256) void dense_dz_kernel(const T* __restrict__ dy,
 
 struct Tiles { int bm, bn, slices, k_slice; };
 
+template <typename T> constexpr int64_t SMALL_TILES = sizeof(T) == 2 ? 256 : 1024;   // fewer tiles of 128 x 128 than this: 64 x 64
+
 // Tile and k slices of a product.  128 x 128 fills the matrix pipe; sides of at most 32 rows or columns take 32, so that little is multiplied for
-// nothing.  16-bit operands take 256 x 256, which reads each operand half as often, where such tiles still fill the card.  Where the tiles leave CUs
-// idle the k range is cut, and the slices' sums are joined by a second launch.
+// nothing.  16-bit operands take 256 x 256, which reads each operand half as often, where such tiles still fill the card.  Products of too few tiles
+// take 64 x 64, and where those leave CUs idle too the k range is cut, and the slices' sums are joined by a second launch.
 template <typename T>
 Tiles tiles_of(int64_t m, int64_t n, int64_t k) {
   constexpr int64_t step = step_of<T>();
   Tiles t;
   t.bm = m <= 32 ? 32 : 128;
   t.bn = n <= 32 ? 32 : 128;
+  int64_t tiles = ceil_div(m, t.bm) * ceil_div(n, t.bn);
   if (sizeof(T) == 2 && ceil_div(m, 256) * ceil_div(n, 256) >= 192) t.bm = t.bn = 256;
-  const int64_t tiles = ceil_div(m, t.bm) * ceil_div(n, t.bn);
+  else if (t.bm == 128 && t.bn == 128 && tiles < SMALL_TILES<T>) t.bm = t.bn = 64;
+  tiles = ceil_div(m, t.bm) * ceil_div(n, t.bn);
   int64_t slices = 1;
-  if (tiles > 0 && tiles < 256) slices = std::min<int64_t>(std::min<int64_t>(ceil_div(512, tiles), ceil_div(k, 4 * step)), 512);
+  if (tiles > 0 && tiles < 256) slices = std::min<int64_t>(std::min<int64_t>(ceil_div(512, tiles), ceil_div(k, 4 * step)), 256);
   if (slices < 1) slices = 1;
   t.k_slice = (int)round_up(ceil_div(k, slices), step);
   if (t.k_slice < step) t.k_slice = (int)step;
@@ -465,11 +483,15 @@ void product(const Product& g, bool p_across, bool q_across, const Epilogue<T>& 
   const Tiles t = tiles_of<T>(g.m, g.n, g.k);
   A* part = t.slices > 1 ? static_cast<A*>(workspace) : nullptr;
   if (t.bm == 128 && t.bn == 128) product_as<T, 128, 128, 2, 2>(g, p_across, q_across, t, part, e, s);
+  else if (t.bm == 64) product_as<T, 64, 64, 2, 2>(g, p_across, q_across, t, part, e, s);
   else if (t.bm == 128) product_as<T, 128, 32, 4, 1>(g, p_across, q_across, t, part, e, s);
   else if (t.bm == 32 && t.bn == 128) product_as<T, 32, 128, 1, 4>(g, p_across, q_across, t, part, e, s);
   else if (t.bm == 32) product_as<T, 32, 32, 2, 2>(g, p_across, q_across, t, part, e, s);
   else if constexpr (sizeof(T) == 2) product_as<T, 256, 256, 2, 4>(g, p_across, q_across, t, part, e, s);
-  if (part) product_join_kernel<T><<<(unsigned)ceil_div((int64_t)g.m * ((g.n + 3) / 4), 256), 256, 0, s>>>(part, t.slices, g.m, g.n, e);
+  if (!part) return;
+  const int64_t lanes = (int64_t)g.m * ((g.n + 3) / 4);
+  if (t.slices > 16) product_join_kernel<T, 32><<<(unsigned)ceil_div(lanes, 8), 256, 0, s>>>(part, t.slices, g.m, g.n, e);
+  else product_join_kernel<T, 1><<<(unsigned)ceil_div(lanes, 256), 256, 0, s>>>(part, t.slices, g.m, g.n, e);
 }
 
 // workgroups along the rows of the dz kernel

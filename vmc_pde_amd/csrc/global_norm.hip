@@ -20,7 +20,7 @@ constexpr int TABLE = 112;             // tensors a launch: 112 x 32 bytes of ke
 constexpr int THREADS = 256;
 constexpr int SMALL_THREADS = 1024;
 constexpr int64_t SMALL_TOTAL = 32768; // up to here one workgroup reads, reduces and scales: one launch instead of three
-constexpr int64_t SMALL_SHARED = 1024; // a tensor of that launch that all its waves share
+constexpr int64_t SMALL_SHARED = 512;  // a tensor of that launch that all its waves share
 constexpr int64_t MIN_CHUNK = 8192;
 constexpr int64_t GROUPS = 2048;       // workgroups a launch aims at: eight a CU
 
@@ -35,7 +35,7 @@ struct Entry {
 };
 struct Table {
   Entry e[TABLE];
-  int32_t count, groups;
+  int32_t count, groups, shared;
   int64_t chunk;
 };
 
@@ -200,9 +200,8 @@ __global__ __launch_bounds__(SMALL_THREADS) void small_kernel(Table tab, int cli
   Bins b = {0, 0, 0};
   // leaves are mostly shorter than a wave: a wave takes every sixteenth tensor, and all of them share one that is long
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  for (int k = 0; k < tab.count; ++k)
-    if (tab.e[k].n > SMALL_SHARED) square_any(tab.e[k], 0, tab.e[k].n, threadIdx.x, SMALL_THREADS, b);
-    else if (k % (SMALL_THREADS / 64) == wave) square_any(tab.e[k], 0, tab.e[k].n, lane, 64, b);
+  for (int k = 0; k < tab.shared; ++k) square_any(tab.e[k], 0, tab.e[k].n, threadIdx.x, SMALL_THREADS, b);
+  for (int k = tab.shared + wave; k < tab.count; k += SMALL_THREADS / 64) square_any(tab.e[k], 0, tab.e[k].n, lane, 64, b);
   b = group_bins<SMALL_THREADS / 64>(b);
   if (threadIdx.x == 0) {
     const double v = join(b);
@@ -212,11 +211,8 @@ __global__ __launch_bounds__(SMALL_THREADS) void small_kernel(Table tab, int cli
   __syncthreads();
   if (!clip) return;
   const double f = shared_factor;
-  for (int k = 0; k < tab.count; ++k) {
-    if (f == 1.0 && tab.e[k].in == tab.e[k].out) continue;
-    if (tab.e[k].n > SMALL_SHARED) scale_any(tab.e[k], 0, tab.e[k].n, threadIdx.x, SMALL_THREADS, f);
-    else if (k % (SMALL_THREADS / 64) == wave) scale_any(tab.e[k], 0, tab.e[k].n, lane, 64, f);
-  }
+  for (int k = 0; k < tab.shared; ++k) scale_any(tab.e[k], 0, tab.e[k].n, threadIdx.x, SMALL_THREADS, f);
+  for (int k = tab.shared + wave; k < tab.count; k += SMALL_THREADS / 64) scale_any(tab.e[k], 0, tab.e[k].n, lane, 64, f);
 }
 
 struct Plan {
@@ -326,8 +322,11 @@ int vmcpde_global_norm(const vmcpde_tensor* tensors, int32_t count, int32_t clip
   if (p.small) {
     Table tab;
     tab.count = 0;
-    for (int32_t k = 0; k < count; ++k)
-      if (tensors[k].n) tab.e[tab.count++] = {tensors[k].in, tensors[k].out, tensors[k].n, tensors[k].dtype, 0};
+    for (bool shared : {true, false}) {      // the tensors that all waves share come first
+      for (int32_t k = 0; k < count; ++k)
+        if (tensors[k].n && (tensors[k].n > SMALL_SHARED) == shared) tab.e[tab.count++] = {tensors[k].in, tensors[k].out, tensors[k].n, tensors[k].dtype, 0};
+      if (shared) tab.shared = tab.count;
+    }
     small_kernel<<<1, SMALL_THREADS, 0, s>>>(tab, clip, max_norm, norm);
     VMC_CHECK_HIP(hipGetLastError());
     return 0;

@@ -7,10 +7,14 @@ a function of its own, and takes no part in torch's automatic differentiation (t
 
 All run on the current HIP stream, allocate through torch, never synchronise with the host, and can be captured into a graph.  Sums, statistics
 and epilogues are held in fp32 for fp32 and 16-bit elements, in fp64 for fp64.  None uses atomics: the same call gives the same bits.
+
+Small calls are bound by the host: arguments travel as one packed record per call (`vmcpde_dense_args`, `vmcpde_norm_args` of include/vmcpde.h)
+and every tensor attribute is read once.
 """
 from __future__ import annotations
 
-import contextlib
+import ctypes as C
+import struct
 
 import numpy as np
 import torch
@@ -19,36 +23,66 @@ from . import _native as nat
 
 DTYPE = {torch.float64: 0, torch.float32: 1, torch.float16: 2, torch.bfloat16: 3}
 ACTIVATION = {"none": 0, "tanh": 1, "gelu": 2, "silu": 3}
-_HALF = (torch.float16, torch.bfloat16)
 SLOPE = {torch.float64: torch.float64, torch.float32: torch.float32, torch.float16: torch.float32, torch.bfloat16: torch.float16}
+WIDE = {torch.float64: torch.float64, torch.float32: torch.float32, torch.float16: torch.float32, torch.bfloat16: torch.float32}
+_HALF = (torch.float16, torch.bfloat16)
+_AUTOGRAD = "the layer operators are no autograd functions: call them under torch.no_grad() and use their *_backward"
+_HOST = "the layer operators run on device (HBM) tensors only"
+
+_pack_dense = struct.Struct("@4i3qPqPqPPqdPqPPqPPP").pack       # vmcpde_dense_args
+_pack_norm = struct.Struct("@2i2qPqPPdPqPPPqPPP").pack          # vmcpde_norm_args
+
+_empty, _device, _stream, _recording = torch.empty, torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream, torch.is_grad_enabled
+_entry = {}
 
 
-def _on(device):
-    return contextlib.nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+def _entries():
+    """The entry points with packed records as their first argument (bound on first use: the library may not be built yet)."""
+    library = nat.lib()
+    for name, (result, arguments) in nat._PROTOS.items():
+        if name.startswith(("vmcpde_dense", "vmcpde_layer_norm", "vmcpde_global_norm")):
+            f = library[name]
+            f.restype, f.argtypes = result, [C.c_void_p, *arguments[1:]]
+            _entry[name] = f
+    return _entry
 
 
-def _check(first, **others):
-    """Element type and device of `first`, which every other tensor must share."""
-    if not isinstance(first, torch.Tensor):
-        raise TypeError(f"a tensor is needed, not {type(first).__name__}")
-    if first.dtype not in DTYPE:
-        raise TypeError(f"element type {first.dtype}: fp64, fp32, fp16 and bf16 are supported")
-    recording = torch.is_grad_enabled()
-    if recording and first.requires_grad:
-        raise ValueError("the layer operators are no autograd functions: call them under torch.no_grad() and use their *_backward")
-    for name, t in others.items():
-        if t is None:
-            continue
-        if not isinstance(t, torch.Tensor):
-            raise TypeError(f"{name}: a tensor is needed, not {type(t).__name__}")
-        if t.dtype != first.dtype:
-            raise TypeError(f"{name} has type {t.dtype} beside {first.dtype}")
-        if t.device != first.device:
-            raise ValueError(f"{name} is on {t.device}, not on {first.device}")
-        if recording and t.requires_grad:
-            raise ValueError("the layer operators are no autograd functions: call them under torch.no_grad() and use their *_backward")
-    if not first.is_cuda:
-        raise ValueError("the layer operators run on device (HBM) tensors only")
+def _call(name, *arguments):
+    rc = (_entry or _entries())[name](*arguments)
+    if rc != 0:
+        nat.check(rc, name)
+
+
+def _workspace(name, device, *arguments):
+    nbytes = (_entry or _entries())[name](*arguments)
+    if nbytes == 0:
+        return None, 0
+    if nbytes < 0:
+        nat.check(-1, name)
+    return _empty(nbytes, dtype=torch.uint8, device=device), nbytes
+
+
+def _first(t):
+    """Element type and device index of the tensor that every other one has to agree with."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"a tensor is needed, not {type(t).__name__}")
+    dtype = t.dtype
+    if dtype not in DTYPE:
+        raise TypeError(f"element type {dtype}: fp64, fp32, fp16 and bf16 are supported")
+    if t.requires_grad and _recording():
+        raise ValueError(_AUTOGRAD)
+    return dtype, t.get_device()
+
+
+def _agrees(t, name, dtype, index):
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name}: a tensor is needed, not {type(t).__name__}")
+    if t.dtype != dtype:
+        raise TypeError(f"{name} has type {t.dtype}: {dtype} is needed")
+    if t.get_device() != index:
+        raise ValueError(f"{name} is on {t.device}, not on " + (f"cuda:{index}" if index >= 0 else "cpu"))
+    if t.requires_grad and _recording():
+        raise ValueError(_AUTOGRAD)
 
 
 def _rows(t, cols, name):
@@ -64,38 +98,23 @@ def _rows(t, cols, name):
 
 
 def _same_shape(t, shape, name):
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f"{name} has shape {tuple(t.shape)}: {tuple(shape)} is needed")
 
 
-def _vector(t, n, name):
-    if t is None:
-        return None
-    _same_shape(t, (n,), name)
-    return t.contiguous()
-
-
-def _address(t):
-    return None if t is None else t.data_ptr()
-
-
-def _workspace(nbytes, device):
-    if nbytes < 0:
-        nat.check(-1, "layers")
-    return (None, 0) if nbytes == 0 else (torch.empty(nbytes, dtype=torch.uint8, device=device), nbytes)
-
-
 def _kernel_layout(kernel):
-    """(tensor, row pitch, whether it is stored (n_out, n_in)) of a kernel of shape (n_in, n_out)."""
-    if kernel.dim() != 2 or 0 in kernel.shape:
-        raise ValueError(f"kernel has shape {tuple(kernel.shape)}: (n_in, n_out), neither of them 0, is needed")
+    """(tensor, n_in, n_out, row pitch, whether it is stored (n_out, n_in)) of a kernel of shape (n_in, n_out)."""
+    if kernel.dim() != 2:
+        raise ValueError(f"kernel has shape {tuple(kernel.shape)}: (n_in, n_out) is needed")
     n_in, n_out = kernel.shape
+    if n_in == 0 or n_out == 0:
+        raise ValueError(f"kernel has shape {(n_in, n_out)}: no axis may be empty")
     s0, s1 = kernel.stride()
     if (s1 == 1 or n_out == 1) and (s0 >= n_out or n_in == 1):
-        return kernel, max(s0, n_out), 0
+        return kernel, n_in, n_out, max(s0, n_out), 0
     if (s0 == 1 or n_in == 1) and (s1 >= n_in or n_out == 1):
-        return kernel, max(s1, n_in), 1
-    return kernel.contiguous(), n_out, 0
+        return kernel, n_in, n_out, max(s1, n_in), 1
+    return kernel.contiguous(), n_in, n_out, n_out, 0
 
 
 def dense(x, kernel, bias=None, *, activation="none", scale=1.0, residual=None, want_slope=False):
@@ -103,30 +122,39 @@ def dense(x, kernel, bias=None, *, activation="none", scale=1.0, residual=None, 
 
     x (..., n_in); kernel (n_in, n_out), the layout of the flat parameter vector's leaves, or a transposed view of an (n_out, n_in) one; bias
     (n_out,); residual of y's shape.  activation: "none", "tanh", "gelu" (z Phi(z)), "silu".  `scale` is the output factor of the reference's
-    conditioners (net.py:50, 61: 10 * tanh).  Widths and row pitches are below 2^22 (2^21 in fp64).  With `want_slope` returns (y, slope): act'(z), which `dense_backward` takes (None for "none");
-    of the type SLOPE[x.dtype] (fp16 for bf16, fp32 for fp16, else the element type)."""
-    _check(x, kernel=kernel, bias=bias, residual=residual)
-    if activation not in ACTIVATION:
+    conditioners (net.py:50, 61: 10 * tanh).  Widths and row pitches are below 2^22 (2^21 in fp64).  With `want_slope` returns (y, slope): act'(z),
+    which `dense_backward` takes (None for "none"), of the type SLOPE[x.dtype] (fp16 for bf16, fp32 for fp16, else the element type)."""
+    dtype, index = _first(x)
+    _agrees(kernel, "kernel", dtype, index)
+    if bias is not None:
+        _agrees(bias, "bias", dtype, index)
+    if residual is not None:
+        _agrees(residual, "residual", dtype, index)
+    if index < 0:
+        raise ValueError(_HOST)
+    if _device() != index:
+        with torch.cuda.device(index):
+            return dense(x, kernel, bias, activation=activation, scale=scale, residual=residual, want_slope=want_slope)
+    act = ACTIVATION.get(activation)
+    if act is None:
         raise ValueError(f"activation {activation!r}: one of {sorted(ACTIVATION)} is needed")
-    kernel, ldk, kernel_t = _kernel_layout(kernel)
-    n_in, n_out = kernel.shape
-    shape = (*x.shape[:-1], n_out)
+    kernel, n_in, n_out, ldk, kernel_t = _kernel_layout(kernel)
+    shape, device = (*x.shape[:-1], n_out), x.device
     x, ldx = _rows(x, n_in, "x")
-    bias = _vector(bias, n_out, "bias")
+    if bias is not None:
+        _same_shape(bias, (n_out,), "bias")
+        bias = bias.contiguous()
     ldr = 0
     if residual is not None:
         _same_shape(residual, shape, "residual")
         residual, ldr = _rows(residual, n_out, "residual")
-    device = x.device
-    with _on(device):
-        y = torch.empty(shape, dtype=x.dtype, device=device)
-        slope = None
-        if want_slope and activation != "none":
-            slope = torch.empty(shape, dtype=SLOPE[x.dtype], device=device)
-        a = nat.DenseArgs(DTYPE[x.dtype], ACTIVATION[activation], kernel_t, 0, x.numel() // n_in, n_in, n_out, x.data_ptr(), ldx, kernel.data_ptr(), ldk,
-                          _address(bias), _address(residual), ldr, float(scale), y.data_ptr(), n_out, _address(slope))
-        ws, nbytes = _workspace(nat.lib().vmcpde_dense_workspace_bytes(a, 0), device)
-        nat.call("vmcpde_dense", a, _address(ws), nbytes, nat.stream())
+    y = _empty(shape, dtype=dtype, device=device)
+    slope = _empty(shape, dtype=SLOPE[dtype], device=device) if want_slope and act else None
+    record = _pack_dense(DTYPE[dtype], act, kernel_t, 0, x.numel() // n_in, n_in, n_out, x.data_ptr(), ldx, kernel.data_ptr(), ldk,
+                         0 if bias is None else bias.data_ptr(), 0 if residual is None else residual.data_ptr(), ldr, float(scale), y.data_ptr(), n_out,
+                         0 if slope is None else slope.data_ptr(), 0, 0, 0, 0, 0)
+    ws, nbytes = _workspace("vmcpde_dense_workspace_bytes", device, record, 0)
+    _call("vmcpde_dense", record, None if ws is None else ws.data_ptr(), nbytes, _stream(index))
     return (y, slope) if want_slope else y
 
 
@@ -134,46 +162,50 @@ def dense_backward(dy, x, kernel, slope=None, *, scale=1.0, want_x=True, want_ke
     """(dx, dkernel, dbias) of `dense` for the gradient dy of y, None where not wanted: with dz = scale * slope * dy, dx = dz @ kernel^T,
     dkernel = x^T @ dz (n_in, n_out), dbias = the sum of dz over the rows.  `slope` and `scale` as the forward call had them; the residual's
     gradient is dy itself.  dz is rounded to the element type, in which the matrix pipe takes it."""
-    _check(dy, x=x, kernel=kernel)
-    kernel, ldk, kernel_t = _kernel_layout(kernel)
-    n_in, n_out = kernel.shape
-    _same_shape(dy, (*x.shape[:-1], n_out), "dy")
-    x_shape = x.shape
+    dtype, index = _first(dy)
+    _agrees(x, "x", dtype, index)
+    _agrees(kernel, "kernel", dtype, index)
+    if index < 0:
+        raise ValueError(_HOST)
+    if _device() != index:
+        with torch.cuda.device(index):
+            return dense_backward(dy, x, kernel, slope, scale=scale, want_x=want_x, want_kernel=want_kernel, want_bias=want_bias)
+    kernel, n_in, n_out, ldk, kernel_t = _kernel_layout(kernel)
+    x_shape, device = x.shape, x.device
+    shape = (*x_shape[:-1], n_out)
+    _same_shape(dy, shape, "dy")
     x, ldx = _rows(x, n_in, "x")
     dy, ldd = _rows(dy, n_out, "dy")
     if slope is not None:
-        want = SLOPE[x.dtype]
-        if slope.dtype != want or slope.device != x.device:
-            raise TypeError(f"slope is {slope.dtype} on {slope.device}: {want} on {x.device} is needed, as dense(..., want_slope=True) returns it")
-        _same_shape(slope, (*x_shape[:-1], n_out), "slope")
+        _agrees(slope, "slope", SLOPE[dtype], index)
+        _same_shape(slope, shape, "slope")
         slope = slope.contiguous()
-    device = x.device
-    with _on(device):
-        dx = torch.empty(x_shape, dtype=x.dtype, device=device) if want_x else None
-        dkernel = torch.empty((n_in, n_out), dtype=x.dtype, device=device) if want_kernel else None
-        dbias = torch.empty(n_out, dtype=x.dtype, device=device) if want_bias else None
-        a = nat.DenseArgs(DTYPE[x.dtype], 0, kernel_t, 0, x.numel() // n_in, n_in, n_out, x.data_ptr(), ldx, kernel.data_ptr(), ldk, None, None, 0,
-                          float(scale), None, 0, _address(slope), dy.data_ptr(), ldd, _address(dx), _address(dkernel), _address(dbias))
-        ws, nbytes = _workspace(nat.lib().vmcpde_dense_workspace_bytes(a, 1), device)
-        nat.call("vmcpde_dense_backward", a, _address(ws), nbytes, nat.stream())
+    dx = _empty(x_shape, dtype=dtype, device=device) if want_x else None
+    dkernel = _empty((n_in, n_out), dtype=dtype, device=device) if want_kernel else None
+    dbias = _empty(n_out, dtype=dtype, device=device) if want_bias else None
+    record = _pack_dense(DTYPE[dtype], 0, kernel_t, 0, x.numel() // n_in, n_in, n_out, x.data_ptr(), ldx, kernel.data_ptr(), ldk, 0, 0, 0, float(scale), 0, 0,
+                         0 if slope is None else slope.data_ptr(), dy.data_ptr(), ldd, 0 if dx is None else dx.data_ptr(),
+                         0 if dkernel is None else dkernel.data_ptr(), 0 if dbias is None else dbias.data_ptr())
+    ws, nbytes = _workspace("vmcpde_dense_workspace_bytes", device, record, 1)
+    _call("vmcpde_dense_backward", record, None if ws is None else ws.data_ptr(), nbytes, _stream(index))
     return dx, dkernel, dbias
 
 
-def _norm_weights(x, weight, bias):
-    """The weights' element type: x's, or fp32 beside 16-bit elements."""
-    for name, t in (("weight", weight), ("bias", bias)):
-        if t is None:
-            continue
-        if t.dtype != x.dtype and not (x.dtype in _HALF and t.dtype == torch.float32):
-            raise TypeError(f"{name} has type {t.dtype} beside {x.dtype}: the same, or fp32 beside 16-bit elements")
-        if t.device != x.device:
-            raise ValueError(f"{name} is on {t.device}, not on {x.device}")
-        if torch.is_grad_enabled() and t.requires_grad:
-            raise ValueError("the layer operators are no autograd functions: call them under torch.no_grad() and use their *_backward")
-    if weight is not None and bias is not None and weight.dtype != bias.dtype:
-        raise TypeError(f"weight has type {weight.dtype} and bias {bias.dtype}")
-    first = weight if weight is not None else bias
-    return x.dtype if first is None else first.dtype
+def _weights(t, name, dtype, index, cols):
+    """A weight or bias of the layer norm: x's element type, or fp32 beside 16-bit elements."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name}: a tensor is needed, not {type(t).__name__}")
+    if t.dtype != dtype and not (t.dtype == torch.float32 and dtype in _HALF):
+        raise TypeError(f"{name} has type {t.dtype} beside {dtype}: the same, or fp32 beside 16-bit elements")
+    _agrees(t, name, t.dtype, index)
+    _same_shape(t, (cols,), name)
+    return t.contiguous()
+
+
+def _columns(x):
+    if x.dim() == 0 or x.shape[-1] == 0:
+        raise ValueError(f"x has shape {tuple(x.shape)}: a last axis of one or more is needed")
+    return x.shape[-1]
 
 
 def layer_norm(x, weight=None, bias=None, *, eps=1e-6, want_stats=False):
@@ -181,61 +213,71 @@ def layer_norm(x, weight=None, bias=None, *, eps=1e-6, want_stats=False):
 
     weight, bias (cols,): x's element type, or fp32 beside 16-bit elements.  With `want_stats` returns (y, mean, rstd), which
     `layer_norm_backward` takes: of the leading shape, fp32 (fp64 for fp64)."""
-    _check(x)
-    if x.dim() == 0 or x.shape[-1] == 0:
-        raise ValueError(f"x has shape {tuple(x.shape)}: a last axis of one or more is needed")
+    dtype, index = _first(x)
+    cols = _columns(x)
+    weights = None
+    if weight is not None:
+        weight = _weights(weight, "weight", dtype, index, cols)
+        weights = weight.dtype
+    if bias is not None:
+        bias = _weights(bias, "bias", dtype, index, cols)
+        if weights is not None and bias.dtype != weights:
+            raise TypeError(f"weight has type {weights} and bias {bias.dtype}")
+        weights = bias.dtype
     if not eps >= 0:
         raise ValueError(f"eps = {eps}")
-    weights = _norm_weights(x, weight, bias)
-    shape, cols = x.shape, x.shape[-1]
-    weight, bias = _vector(weight, cols, "weight"), _vector(bias, cols, "bias")
+    if index < 0:
+        raise ValueError(_HOST)
+    if _device() != index:
+        with torch.cuda.device(index):
+            return layer_norm(x, weight, bias, eps=eps, want_stats=want_stats)
+    shape, device = x.shape, x.device
     x, ldx = _rows(x, cols, "x")
-    device = x.device
-    with _on(device):
-        y = torch.empty(shape, dtype=x.dtype, device=device)
-        mean = rstd = None
-        if want_stats:
-            wide = torch.float64 if x.dtype == torch.float64 else torch.float32
-            mean, rstd = torch.empty(shape[:-1], dtype=wide, device=device), torch.empty(shape[:-1], dtype=wide, device=device)
-        a = nat.NormArgs(DTYPE[x.dtype], DTYPE[weights], x.numel() // cols, cols, x.data_ptr(), ldx, _address(weight), _address(bias), float(eps),
-                         y.data_ptr(), cols, _address(mean), _address(rstd))
-        nat.call("vmcpde_layer_norm", a, nat.stream())
+    y = _empty(shape, dtype=dtype, device=device)
+    mean = rstd = None
+    if want_stats:
+        mean, rstd = _empty(shape[:-1], dtype=WIDE[dtype], device=device), _empty(shape[:-1], dtype=WIDE[dtype], device=device)
+    _call("vmcpde_layer_norm", _pack_norm(DTYPE[dtype], DTYPE[weights or dtype], x.numel() // cols, cols, x.data_ptr(), ldx, 0 if weight is None else weight.data_ptr(),
+                                          0 if bias is None else bias.data_ptr(), float(eps), y.data_ptr(), cols, 0 if mean is None else mean.data_ptr(),
+                                          0 if rstd is None else rstd.data_ptr(), 0, 0, 0, 0, 0), _stream(index))
     return (y, mean, rstd) if want_stats else y
 
 
 def layer_norm_backward(dy, x, mean, rstd, weight=None, *, want_x=True, want_weight=True, want_bias=True, weight_dtype=None):
     """(dx, dweight, dbias) of `layer_norm` for the gradient dy of y, None where not wanted; mean, rstd from `layer_norm(..., want_stats=True)`.
     dweight and dbias have the weight's type (without a weight `weight_dtype`, else x's)."""
-    _check(dy, x=x)
-    weights = _norm_weights(x, weight, None)
-    if weight is None and weight_dtype is not None:
-        if weight_dtype != x.dtype and not (x.dtype in _HALF and weight_dtype == torch.float32):
-            raise TypeError(f"weight_dtype {weight_dtype} beside {x.dtype}: the same, or fp32 beside 16-bit elements")
+    dtype, index = _first(dy)
+    _agrees(x, "x", dtype, index)
+    cols = _columns(x)
+    weights = dtype
+    if weight is not None:
+        weight = _weights(weight, "weight", dtype, index, cols)
+        weights = weight.dtype
+    elif weight_dtype is not None:
+        if weight_dtype != dtype and not (dtype in _HALF and weight_dtype == torch.float32):
+            raise TypeError(f"weight_dtype {weight_dtype} beside {dtype}: the same, or fp32 beside 16-bit elements")
         weights = weight_dtype
-    if x.dim() == 0 or x.shape[-1] == 0:
-        raise ValueError(f"x has shape {tuple(x.shape)}: a last axis of one or more is needed")
-    shape, cols = x.shape, x.shape[-1]
+    shape, device = x.shape, x.device
     _same_shape(dy, shape, "dy")
-    wide = torch.float64 if x.dtype == torch.float64 else torch.float32
     for name, t in (("mean", mean), ("rstd", rstd)):
+        _agrees(t, name, WIDE[dtype], index)
         _same_shape(t, shape[:-1], name)
-        if t.dtype != wide or t.device != x.device:
-            raise TypeError(f"{name} is {t.dtype} on {t.device}: {wide} on {x.device} is needed")
-    weight = _vector(weight, cols, "weight")
+    if index < 0:
+        raise ValueError(_HOST)
+    if _device() != index:
+        with torch.cuda.device(index):
+            return layer_norm_backward(dy, x, mean, rstd, weight, want_x=want_x, want_weight=want_weight, want_bias=want_bias, weight_dtype=weight_dtype)
     x, ldx = _rows(x, cols, "x")
     dy, ldd = _rows(dy, cols, "dy")
     mean, rstd = mean.contiguous(), rstd.contiguous()
-    device = x.device
-    with _on(device):
-        dx = torch.empty(shape, dtype=x.dtype, device=device) if want_x else None
-        dweight = torch.empty(cols, dtype=weights, device=device) if want_weight else None
-        dbias = torch.empty(cols, dtype=weights, device=device) if want_bias else None
-        a = nat.NormArgs(DTYPE[x.dtype], DTYPE[weights], x.numel() // cols, cols, x.data_ptr(), ldx, _address(weight), None, 0.0, None, 0, mean.data_ptr(),
-                         rstd.data_ptr(), dy.data_ptr(), ldd, _address(dx), _address(dweight), _address(dbias))
-        ws, nbytes = (None, 0)
-        if want_weight or want_bias:
-            ws, nbytes = _workspace(nat.lib().vmcpde_layer_norm_backward_workspace_bytes(a), device)
-        nat.call("vmcpde_layer_norm_backward", a, _address(ws), nbytes, nat.stream())
+    dx = _empty(shape, dtype=dtype, device=device) if want_x else None
+    dweight = _empty(cols, dtype=weights, device=device) if want_weight else None
+    dbias = _empty(cols, dtype=weights, device=device) if want_bias else None
+    record = _pack_norm(DTYPE[dtype], DTYPE[weights], x.numel() // cols, cols, x.data_ptr(), ldx, 0 if weight is None else weight.data_ptr(), 0, 0.0, 0, 0,
+                        mean.data_ptr(), rstd.data_ptr(), dy.data_ptr(), ldd, 0 if dx is None else dx.data_ptr(), 0 if dweight is None else dweight.data_ptr(),
+                        0 if dbias is None else dbias.data_ptr())
+    ws, nbytes = _workspace("vmcpde_layer_norm_backward_workspace_bytes", device, record) if want_weight or want_bias else (None, 0)
+    _call("vmcpde_layer_norm_backward", record, None if ws is None else ws.data_ptr(), nbytes, _stream(index))
     return dx, dweight, dbias
 
 
@@ -263,37 +305,51 @@ def _fills_memory(t):
     return True
 
 
+def _codes(leaves):
+    try:
+        return [DTYPE[t.dtype] for t in leaves]
+    except KeyError as unknown:
+        raise TypeError(f"element type {unknown.args[0]}: fp64, fp32, fp16 and bf16 are supported") from None
+
+
 def _global_norm(tensors, max_norm, out):
     leaves = _leaves(tensors, [])
     if not leaves:
         raise ValueError("no tensors")
-    device = leaves[0].device
-    if not leaves[0].is_cuda:
-        raise ValueError("the layer operators run on device (HBM) tensors only")
-    for t in leaves:
-        if t.device != device:
-            raise ValueError(f"tensors on {device} and {t.device}")
-        if t.dtype not in DTYPE:
-            raise TypeError(f"element type {t.dtype}: fp64, fp32, fp16 and bf16 are supported")
-        if not (t.is_contiguous() or t.numel() == 0 or _fills_memory(t)):
-            raise ValueError(f"a tensor of shape {tuple(t.shape)} and strides {t.stride()} does not fill its memory: pass a contiguous one")
+    index, codes = leaves[0].get_device(), _codes(leaves)
+    if index < 0:
+        raise ValueError(_HOST)
+    if any([t.get_device() != index for t in leaves]):
+        raise ValueError(f"tensors on several devices: {sorted({str(t.device) for t in leaves})}")
+    if _device() != index:
+        with torch.cuda.device(index):
+            return _global_norm(tensors, max_norm, out)
+    plain = all([t.is_contiguous() for t in leaves])
+    if not plain:
+        for t in leaves:
+            if t.numel() and not t.is_contiguous() and not _fills_memory(t):
+                raise ValueError(f"a tensor of shape {tuple(t.shape)} and strides {t.stride()} does not fill its memory: pass a contiguous one")
+    places = [t.data_ptr() for t in leaves]
     targets = leaves
-    if out is not None:
+    if out is None:
+        to = places
+    else:
         targets = _leaves(out, [])
         if len(targets) != len(leaves):
             raise ValueError(f"{len(leaves)} tensors and {len(targets)} to write them to")
-        for t, o in zip(leaves, targets):
-            if o.shape != t.shape or o.dtype != t.dtype or o.device != device or o.stride() != t.stride():
-                raise ValueError(f"out: shape {tuple(o.shape)}, strides {o.stride()}, {o.dtype} on {o.device} beside {tuple(t.shape)}, {t.stride()}, {t.dtype} on {device}")
-    if max_norm is not None and torch.is_grad_enabled() and any(t.requires_grad for t in targets):
+        if [t.shape for t in targets] != [t.shape for t in leaves] or _codes(targets) != codes or any([t.get_device() != index for t in targets]) \
+                or not (plain and all([t.is_contiguous() for t in targets])) and [t.stride() for t in targets] != [t.stride() for t in leaves]:
+            raise ValueError("out: shapes, strides, element types and devices have to be those of the tensors")
+        to = [t.data_ptr() for t in targets]
+    if max_norm is not None and _recording() and any([t.requires_grad for t in targets]):
         raise ValueError("clipping writes into tensors that automatic differentiation records: call it under torch.no_grad()")
-    table = np.array([(t.data_ptr(), o.data_ptr(), t.numel(), DTYPE[t.dtype]) for t, o in zip(leaves, targets)], dtype=np.int64)   # vmcpde_tensor
-    address, count = table.ctypes.data, len(leaves)
-    with _on(device):
-        norm = torch.empty((), dtype=torch.float64, device=device)
-        ws, nbytes = _workspace(nat.lib().vmcpde_global_norm_workspace_bytes(address, count), device)
-        nat.call("vmcpde_global_norm", address, count, 0 if max_norm is None else 1, 0.0 if max_norm is None else max_norm, norm.data_ptr(), _address(ws), nbytes,
-                 nat.stream())
+    count = len(leaves)
+    table = np.array((places, to, [t.numel() for t in leaves], codes), dtype=np.int64).T.copy()        # vmcpde_tensor: in, out, n, dtype
+    address, device = table.ctypes.data, leaves[0].device
+    norm = _empty((), dtype=torch.float64, device=device)
+    ws, nbytes = _workspace("vmcpde_global_norm_workspace_bytes", device, address, count)
+    _call("vmcpde_global_norm", address, count, 0 if max_norm is None else 1, 0.0 if max_norm is None else max_norm, norm.data_ptr(),
+          None if ws is None else ws.data_ptr(), nbytes, _stream(index))
     return norm
 
 
