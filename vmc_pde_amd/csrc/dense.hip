@@ -136,34 +136,30 @@ template <typename T> struct Matrix;
 template <> struct Matrix<bf16_t> {
   typedef short8 Frag;
   typedef float4v Acc;
-  static __device__ __forceinline__ Acc mfma(Frag a, Frag b, Acc c) {
+  static constexpr int TURNS = 1;
+  static __device__ __forceinline__ Acc mfma(Frag a, Frag b, Acc c, int) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
   }
 };
 template <> struct Matrix<f16_t> {
   typedef short8 Frag;
   typedef float4v Acc;
-  static __device__ __forceinline__ Acc mfma(Frag a, Frag b, Acc c) {
+  static constexpr int TURNS = 1;
+  static __device__ __forceinline__ Acc mfma(Frag a, Frag b, Acc c, int) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
   }
 };
 template <> struct Matrix<float> {
   typedef float4v Frag;
   typedef float4v Acc;
-  static __device__ __forceinline__ Acc mfma(Frag a, Frag b, Acc c) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], c, 0, 0, 0);
-    return c;
-  }
+  static constexpr int TURNS = 4;
+  static __device__ __forceinline__ Acc mfma(Frag a, Frag b, Acc c, int j) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], c, 0, 0, 0); }
 };
 template <> struct Matrix<double> {
   typedef double2v Frag;
   typedef double4v Acc;
-  static __device__ __forceinline__ Acc mfma(Frag a, Frag b, Acc c) {
-#pragma unroll
-    for (int j = 0; j < 2; ++j) c = __builtin_amdgcn_mfma_f64_16x16x4f64(a[j], b[j], c, 0, 0, 0);
-    return c;
-  }
+  static constexpr int TURNS = 2;
+  static __device__ __forceinline__ Acc mfma(Frag a, Frag b, Acc c, int j) { return __builtin_amdgcn_mfma_f64_16x16x4f64(a[j], b[j], c, 0, 0, 0); }
 };
 
 // One operand's tile, R rows x one step of k, 16-byte chunks straight from memory into LDS.  Along k: [row][8 chunks], chunk c of row r at
@@ -291,9 +287,11 @@ __device__ __forceinline__ void tile_product(const Product& g, int row0, int col
 #pragma unroll
       for (int a = 0; a < TM; ++a) fp[a] = p.fragment(now_p, a, s);
 #pragma unroll
-      for (int a = 0; a < TM; ++a)
+      for (int j = 0; j < Matrix<T>::TURNS; ++j)
 #pragma unroll
-        for (int b = 0; b < TN; ++b) acc[a][b] = Matrix<T>::mfma(fq[b], fp[a], acc[a][b]);
+        for (int a = 0; a < TM; ++a)
+#pragma unroll
+          for (int b = 0; b < TN; ++b) acc[a][b] = Matrix<T>::mfma(fq[b], fp[a], acc[a][b], j);
     }
   };
   lds_char* const lds = (lds_char*)tiles;
@@ -438,23 +436,24 @@ __global__ __launch_bounds__(256) void dense_dz_kernel(const T* __restrict__ dy,
 
 struct Tiles { int bm, bn, slices, k_slice; };
 
-template <typename T> constexpr int64_t SMALL_TILES = sizeof(T) == 2 ? 256 : 1024;   // fewer tiles of 128 x 128 than this: 64 x 64
-
-// Tile and k slices of a product.  128 x 128 fills the matrix pipe; sides of at most 32 rows or columns take 32, so that little is multiplied for
-// nothing.  16-bit operands take 256 x 256, which reads each operand half as often, where such tiles still fill the card.  Products of too few tiles
-// take 64 x 64, and where those leave CUs idle too the k range is cut, and the slices' sums are joined by a second launch.
+// Tile and k slices of a product.  Sides of at most 32 rows or columns take 32, so that little is multiplied for nothing.  16-bit operands take
+// 256 x 256, which reads each operand half as often, where such tiles fill the card, else 128 x 128; fp32 and fp64 take 128 x 64, of which a CU holds
+// three.  Products of too few tiles take 64 x 64, and where those leave CUs idle too the k range is cut, and the slices' sums are joined by a second launch.
 template <typename T>
 Tiles tiles_of(int64_t m, int64_t n, int64_t k) {
   constexpr int64_t step = step_of<T>();
+  constexpr bool half = sizeof(T) == 2;
   Tiles t;
   t.bm = m <= 32 ? 32 : 128;
-  t.bn = n <= 32 ? 32 : 128;
-  int64_t tiles = ceil_div(m, t.bm) * ceil_div(n, t.bn);
-  if (sizeof(T) == 2 && ceil_div(m, 256) * ceil_div(n, 256) >= 192) t.bm = t.bn = 256;
-  else if (t.bm == 128 && t.bn == 128 && tiles < SMALL_TILES<T>) t.bm = t.bn = 64;
+  t.bn = n <= 32 ? 32 : half || t.bm == 32 ? 128 : 64;
+  int64_t tiles = ceil_div(m, t.bm) * ceil_div(n, t.bn), fill = 512;
+  if (half && ceil_div(m, 256) * ceil_div(n, 256) >= 192) t.bm = t.bn = 256;
+  else if (t.bm == 128 && t.bn == 128 && tiles < 256) t.bm = t.bn = 64;
+  else if (t.bm == 128 && t.bn == 64 && tiles < 128) t.bm = 64;
+  else if (!half && t.bn == 64) fill = 768;
   tiles = ceil_div(m, t.bm) * ceil_div(n, t.bn);
   int64_t slices = 1;
-  if (tiles > 0 && tiles < 256) slices = std::min<int64_t>(std::min<int64_t>(ceil_div(512, tiles), ceil_div(k, 4 * step)), 256);
+  if (tiles > 0 && tiles < 256) slices = std::min<int64_t>(std::min<int64_t>(ceil_div(fill, tiles), ceil_div(k, 4 * step)), 256);
   if (slices < 1) slices = 1;
   t.k_slice = (int)round_up(ceil_div(k, slices), step);
   if (t.k_slice < step) t.k_slice = (int)step;
@@ -482,12 +481,16 @@ void product(const Product& g, bool p_across, bool q_across, const Epilogue<T>& 
   typedef typename Wide<T>::type A;
   const Tiles t = tiles_of<T>(g.m, g.n, g.k);
   A* part = t.slices > 1 ? static_cast<A*>(workspace) : nullptr;
-  if (t.bm == 128 && t.bn == 128) product_as<T, 128, 128, 2, 2>(g, p_across, q_across, t, part, e, s);
-  else if (t.bm == 64) product_as<T, 64, 64, 2, 2>(g, p_across, q_across, t, part, e, s);
-  else if (t.bm == 128) product_as<T, 128, 32, 4, 1>(g, p_across, q_across, t, part, e, s);
+  if constexpr (sizeof(T) == 2) {
+    if (t.bm == 256) product_as<T, 256, 256, 2, 4>(g, p_across, q_across, t, part, e, s);
+    if (t.bm == 128 && t.bn == 128) product_as<T, 128, 128, 2, 2>(g, p_across, q_across, t, part, e, s);
+  } else {
+    if (t.bm == 128 && t.bn == 64) product_as<T, 128, 64, 2, 2>(g, p_across, q_across, t, part, e, s);
+  }
+  if (t.bm == 64) product_as<T, 64, 64, 2, 2>(g, p_across, q_across, t, part, e, s);
+  else if (t.bm == 128 && t.bn == 32) product_as<T, 128, 32, 4, 1>(g, p_across, q_across, t, part, e, s);
   else if (t.bm == 32 && t.bn == 128) product_as<T, 32, 128, 1, 4>(g, p_across, q_across, t, part, e, s);
   else if (t.bm == 32) product_as<T, 32, 32, 2, 2>(g, p_across, q_across, t, part, e, s);
-  else if constexpr (sizeof(T) == 2) product_as<T, 256, 256, 2, 4>(g, p_across, q_across, t, part, e, s);
   if (!part) return;
   const int64_t lanes = (int64_t)g.m * ((g.n + 3) / 4);
   if (t.slices > 16) product_join_kernel<T, 32><<<(unsigned)ceil_div(lanes, 8), 256, 0, s>>>(part, t.slices, g.m, g.n, e);
