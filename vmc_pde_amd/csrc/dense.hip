@@ -119,6 +119,7 @@ struct Product {
 typedef short short8 __attribute__((ext_vector_type(8)));
 typedef short short4v __attribute__((ext_vector_type(4)));
 typedef float float4v __attribute__((ext_vector_type(4)));
+typedef int int4v __attribute__((ext_vector_type(4)));
 typedef double double2v __attribute__((ext_vector_type(2)));
 typedef double double4v __attribute__((ext_vector_type(4)));
 typedef bf16_t bf16x8 __attribute__((ext_vector_type(8)));
@@ -172,6 +173,7 @@ struct Tile {
   static constexpr int SIZE = sizeof(T), E = 16 / SIZE, STEP = step_of<T>();
   static constexpr int LOADS = R * 8 / THREADS, BYTES = R * LINE;
   static constexpr int PER_LINE = R / E;                       // chunks of a line of k
+  static constexpr int READS = !ACROSS ? 1 : SIZE == 2 ? 2 : E;   // LDS instructions of a fragment
   static_assert(LOADS >= 1, "a chunk for every thread");
   const char* base;
   int64_t left, step;                                          // bytes from base to the operand's end; bytes a step of k moves on
@@ -218,15 +220,17 @@ struct Tile {
     }
   }
 
-  // fetch the tile at k (k_left of it inside the operand) and move on
-  __device__ __forceinline__ void fetch(lds_char* to, int k_left) {
+  // Fetch the tile at k (k_left of it inside the operand) and move on.  In assembly because the compiler, which cannot tell the buffers apart, makes every
+  // fragment read wait for the fetches into the other one; nothing is returned in registers, and `arrived` waits for what lands in LDS.
+  __device__ __forceinline__ void fetch(unsigned to, int k_left) {
     const int64_t l = left < 0 ? 0 : left;
-    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, l < OUTSIDE ? (int)l : OUTSIDE, 0x00020000);
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint64_t b = reinterpret_cast<uint64_t>(base);
+    const int4v r = {(int)(uint32_t)b, (int)((b >> 32) & 0xffff), l < OUTSIDE ? (int)l : OUTSIDE, 0x00020000};
+    const unsigned first = to + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 1024;
 #pragma unroll
     for (int j = 0; j < LOADS; ++j) {
       const int at = ACROSS || chunk_k[j] < k_left ? offset[j] : OUTSIDE;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, to + (j * THREADS + wave * 64) * 16, 16, at, 0, 0, 0);
+      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(first + j * THREADS * 16), "v"(at), "s"(r) : "memory", "m0");
     }
     base += step;
     left -= step;
@@ -250,8 +254,7 @@ struct Tile {
   }
 };
 
-// BM x BN of C by WM x WN waves; k in [k_begin, k_end) (k_begin a multiple of the step).  Two buffers: a step's fetches fly while the step before
-// is multiplied.  The column operand goes in as the matrix instruction's first, so a lane's results lie along a row of C.
+// BM x BN of C by WM x WN waves; k in [k_begin, k_end) (k_begin a multiple of the step).  The column operand goes in as the matrix instruction's first, so a lane's results lie along a row of C.
 // out(row, col, v): the sums of C[row][col .. col + N].
 template <typename T, int BM, int BN, int WM, int WN, bool PX, bool QX, typename F>
 __device__ __forceinline__ void tile_product(const Product& g, int row0, int col0, int k_begin, int k_end, F out) {
@@ -273,39 +276,67 @@ __device__ __forceinline__ void tile_product(const Product& g, int row0, int col
   for (int a = 0; a < TM; ++a)
 #pragma unroll
     for (int b = 0; b < TN; ++b) acc[a][b] = {0, 0, 0, 0};
-  // (the two buffers as parameters that do not overlap: otherwise every fragment read waits for the fetches into the other buffer)
-  auto step = [&](lds_char* __restrict__ now_p, lds_char* __restrict__ now_q, lds_char* __restrict__ next_p, lds_char* __restrict__ next_q, int k_left) {
-    if (k_left > 0) {
-      p.fetch(next_p, k_left);
-      q.fetch(next_q, k_left);
-    }
+  // A step's k is multiplied in two halves.  While the first half is multiplied the second's fragments are read; then the next step's tiles have arrived
+  // and everyone has read this step's: the buffer is free for the step after next, and while the second half is multiplied the next step's first
+  // fragments are read.  One barrier a step, and the matrix pipe has work on both sides of it.
+  Frag p0[TM], q0[TN], p1[TM], q1[TN];
+  auto read = [&](const lds_char* from, int s, Frag (&fp)[TM], Frag (&fq)[TN]) {
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      Frag fp[TM], fq[TN];
+    for (int b = 0; b < TN; ++b) fq[b] = q.fragment(from + P::BYTES, b, s);
 #pragma unroll
-      for (int b = 0; b < TN; ++b) fq[b] = q.fragment(now_q, b, s);
-#pragma unroll
-      for (int a = 0; a < TM; ++a) fp[a] = p.fragment(now_p, a, s);
-#pragma unroll
-      for (int j = 0; j < Matrix<T>::TURNS; ++j)
-#pragma unroll
-        for (int a = 0; a < TM; ++a)
-#pragma unroll
-          for (int b = 0; b < TN; ++b) acc[a][b] = Matrix<T>::mfma(fq[b], fp[a], acc[a][b], j);
-    }
+    for (int a = 0; a < TM; ++a) fp[a] = p.fragment(from, a, s);
   };
-  lds_char* const lds = (lds_char*)tiles;
-  int at = 0;
+  auto multiply = [&](const Frag (&fp)[TM], const Frag (&fq)[TN]) {
+#pragma unroll
+    for (int j = 0; j < Matrix<T>::TURNS; ++j)
+#pragma unroll
+      for (int a = 0; a < TM; ++a)
+#pragma unroll
+        for (int b = 0; b < TN; ++b) acc[a][b] = Matrix<T>::mfma(fq[b], fp[a], acc[a][b], j);
+  };
+  // a half's reads spread between the multiplications that run meanwhile (left alone, the compiler puts them behind)
+  constexpr int READS = TM * P::READS + TN * Q::READS, PRODUCTS = TM * TN * Matrix<T>::TURNS, EACH = PRODUCTS / READS > 2 ? 2 : 1;
+  auto interleave = [&]() {
+#pragma unroll
+    for (int r = 0; r < READS; ++r) {
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);      // an LDS read
+      __builtin_amdgcn_sched_group_barrier(0x008, EACH, 0);   // matrix instructions
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  constexpr int BUFFER = P::BYTES + Q::BYTES;
+  const lds_char* const lds = (const lds_char*)tiles;
+  const unsigned place = __builtin_amdgcn_readfirstlane((unsigned)reinterpret_cast<uintptr_t>(lds));
+  auto fetch = [&](int buffer, int k_left) {
+    p.fetch(place + buffer, k_left);
+    q.fetch(place + buffer + P::BYTES, k_left);
+  };
   if (k_begin < k_end) {
-    p.fetch(lds, k_end - k_begin);
-    q.fetch(lds + P::BYTES, k_end - k_begin);
-  }
-  for (int k = k_begin; k < k_end; k += STEP) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();                      // this step's tiles are there, and the other buffer's readers are done
-    const int other = at ^ (P::BYTES + Q::BYTES);
-    step(lds + at, lds + at + P::BYTES, lds + other, lds + other + P::BYTES, k_end - k - STEP);
-    at = other;
+    const int steps = (k_end - k_begin + STEP - 1) / STEP;
+    int k_left = k_end - k_begin, now = 0;
+    fetch(0, k_left);
+    if (steps > 1) {
+      fetch(BUFFER, k_left - STEP);
+      asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(P::LOADS + Q::LOADS) : "memory");
+    } else {
+      asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+    }
+    read(lds, 0, p0, q0);
+    for (int left = steps - 1; left > 0; --left) {
+      read(lds + now, 1, p1, q1);
+      multiply(p0, q0);
+      interleave();
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      if (left > 1) fetch(now, k_left - 2 * STEP);
+      k_left -= STEP;
+      now ^= BUFFER;
+      read(lds + now, 0, p0, q0);
+      multiply(p1, q1);
+      interleave();
+    }
+    read(lds + now, 1, p1, q1);
+    multiply(p0, q0);
+    multiply(p1, q1);
   }
   // Sixteen rows at a time through a piece of LDS of the wave's own, so that a lane ends with N columns of a row and a row's lanes write whole lines.
   // The loop stays rolled (the epilogue is long); the registers are picked by number inside it.
