@@ -463,6 +463,174 @@ __global__ __launch_bounds__(256) void dense_dz_kernel(const T* __restrict__ dy,
   }
 }
 
+// ---- thin layers ---------------------------------------------------------------------------------------------------------------------
+
+// At most 32 inputs and outputs in fp32 or fp64 (the flow's own conditioners): bound by reading and writing the rows once.  The kernel's fragments
+// stay in registers, a wave takes sixteen rows at a time straight from memory, nothing passes through LDS, and no operand is copied.
+constexpr int THIN = 32, THIN_THREADS = 512, THIN_GROUPS = 256;
+
+__device__ __forceinline__ float4v mfma4(float a, float b, float4v c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ double4v mfma4(double a, double b, double4v c) { return __builtin_amdgcn_mfma_f64_16x16x4f64(a, b, c, 0, 0, 0); }
+// row of a 16 x 16 result that register r of a lane of group g holds
+template <typename T> __device__ __forceinline__ int result_row(int g, int r) { return sizeof(T) == 8 ? g + 4 * r : g * 4 + r; }
+
+// The kernel's element (k, n) is at w[k * sk + n * sn].  KS: steps of four inputs, NT: tiles of sixteen outputs.
+template <typename T, int KS, int NT>
+__global__ __launch_bounds__(256) void thin_forward_kernel(const T* __restrict__ x, int64_t ldx, const T* __restrict__ w, int64_t sk, int64_t sn, int64_t rows, int n_in,
+                                                           Epilogue<T> e) {
+  typedef typename Matrix<T>::Acc Acc;
+  const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+  const int64_t tiles = (rows + 15) / 16, stride = (int64_t)gridDim.x * 4;
+  int64_t tile = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (tile >= tiles) return;
+  T wf[KS][NT], bias[NT], xf[KS];
+#pragma unroll
+  for (int b = 0; b < NT; ++b) {
+    const int n = b * 16 + i;
+    bias[b] = e.bias && n < e.n ? e.bias[n] : (T)0;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) wf[s][b] = 4 * s + g < n_in && n < e.n ? w[(4 * s + g) * sk + n * sn] : (T)0;
+  }
+  auto load = [&](int64_t at) {
+#pragma unroll
+    for (int s = 0; s < KS; ++s) xf[s] = at * 16 + i < rows && 4 * s + g < n_in ? x[(at * 16 + i) * ldx + 4 * s + g] : (T)0;
+  };
+  load(tile);
+  for (; tile < tiles; tile += stride) {
+    Acc acc[NT];
+#pragma unroll
+    for (int b = 0; b < NT; ++b) acc[b] = {0, 0, 0, 0};
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int b = 0; b < NT; ++b) acc[b] = mfma4(xf[s], wf[s][b], acc[b]);
+    if (tile + stride < tiles) load(tile + stride);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int64_t row = tile * 16 + result_row<T>(g, r);
+#pragma unroll
+      for (int b = 0; b < NT; ++b) {
+        const int n = b * 16 + i;
+        if (row < rows && n < e.n) {
+          T a, slope;
+          activate<T, T>(e.act, acc[b][r] + bias[b], a, slope);
+          a *= e.scale;
+          if (e.residual) a += e.residual[row * e.ldr + n];
+          e.y[row * e.ldy + n] = a;
+          if (e.slope) e.slope[row * e.n + n] = slope;
+        }
+      }
+    }
+  }
+}
+
+// dx (may be null) and this workgroup's sums partial[blockIdx.x][n_in * n_out + n_out] of x^T dz and dz (null: not wanted).  dz = scale * slope * dy is
+// taken twice from memory (the second time from the caches), once for each product's lane layout.
+template <typename T, int KT, int NT>
+__global__ __launch_bounds__(THIN_THREADS) void thin_backward_kernel(const T* __restrict__ dy, int64_t ldd, const T* __restrict__ slope, T scale,
+                                                                     const T* __restrict__ x, int64_t ldx, const T* __restrict__ w, int64_t sk, int64_t sn, int64_t rows,
+                                                                     int n_in, int n_out, T* __restrict__ dx, T* __restrict__ partial) {
+  typedef typename Matrix<T>::Acc Acc;
+  constexpr int NS = NT * 4, WAVES = THIN_THREADS / 64, SUMS = KT * 16 * NT * 16 + NT * 16;
+  __shared__ T sh[WAVES / 2][SUMS];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
+  const int64_t tiles = (rows + 15) / 16, stride = (int64_t)gridDim.x * WAVES;
+  T wf[NS][KT];
+#pragma unroll
+  for (int s = 0; s < NS; ++s)
+#pragma unroll
+    for (int a = 0; a < KT; ++a) wf[s][a] = dx && a * 16 + i < n_in && 4 * s + g < n_out ? w[(a * 16 + i) * sk + (4 * s + g) * sn] : (T)0;
+  Acc sum[KT][NT];
+  T bias[NT];
+#pragma unroll
+  for (int b = 0; b < NT; ++b) {
+    bias[b] = 0;
+#pragma unroll
+    for (int a = 0; a < KT; ++a) sum[a][b] = {0, 0, 0, 0};
+  }
+  auto dz = [&](int64_t row, int n) {
+    if (row >= rows || n >= n_out) return (T)0;
+    const T v = dy[row * ldd + n] * scale;
+    return slope ? v * slope[row * n_out + n] : v;
+  };
+  for (int64_t tile = (int64_t)blockIdx.x * WAVES + wave; tile < tiles; tile += stride) {
+    T zr[NS], zc[4][NT], xc[4][KT];
+    if (dx) {
+#pragma unroll
+      for (int s = 0; s < NS; ++s) zr[s] = dz(tile * 16 + i, 4 * s + g);
+    }
+    if (partial) {
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        const int64_t row = tile * 16 + 4 * s + g;
+#pragma unroll
+        for (int b = 0; b < NT; ++b) zc[s][b] = dz(row, b * 16 + i);
+#pragma unroll
+        for (int a = 0; a < KT; ++a) xc[s][a] = x && row < rows && a * 16 + i < n_in ? x[row * ldx + a * 16 + i] : (T)0;
+      }
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+#pragma unroll
+        for (int b = 0; b < NT; ++b) {
+          bias[b] += zc[s][b];
+#pragma unroll
+          for (int a = 0; a < KT; ++a) sum[a][b] = mfma4(xc[s][a], zc[s][b], sum[a][b]);
+        }
+    }
+    if (dx) {
+      Acc acc[KT];
+#pragma unroll
+      for (int a = 0; a < KT; ++a) acc[a] = {0, 0, 0, 0};
+#pragma unroll
+      for (int s = 0; s < NS; ++s)
+#pragma unroll
+        for (int a = 0; a < KT; ++a) acc[a] = mfma4(zr[s], wf[s][a], acc[a]);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int64_t row = tile * 16 + result_row<T>(g, r);
+#pragma unroll
+        for (int a = 0; a < KT; ++a)
+          if (row < rows && a * 16 + i < n_in) dx[row * n_in + a * 16 + i] = acc[a][r];
+      }
+    }
+  }
+  if (!partial) return;
+#pragma unroll
+  for (int b = 0; b < NT; ++b) {
+    bias[b] += __shfl_xor(bias[b], 16);
+    bias[b] += __shfl_xor(bias[b], 32);
+  }
+  // the upper waves' sums onto the lower ones', then those in their order
+  for (int half = 0; half < 2; ++half) {
+    if (wave / (WAVES / 2) == half) {
+      T* to = sh[wave % (WAVES / 2)];
+#pragma unroll
+      for (int b = 0; b < NT; ++b) {
+#pragma unroll
+        for (int a = 0; a < KT; ++a)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            T& at = to[(a * 16 + result_row<T>(g, r)) * (NT * 16) + b * 16 + i];
+            at = half ? at + sum[a][b][r] : sum[a][b][r];
+          }
+        T& at = to[KT * 16 * NT * 16 + b * 16 + i];
+        if (g == 0) at = half ? at + bias[b] : bias[b];
+      }
+    }
+    __syncthreads();
+  }
+  T* out = partial + (int64_t)blockIdx.x * (n_in + 1) * n_out;
+  for (int u = threadIdx.x; u < SUMS; u += THIN_THREADS) {
+    const int k = u / (NT * 16), n = u % (NT * 16);
+    const bool is_bias = k == KT * 16;
+    if (n < n_out && (is_bias || k < n_in)) {
+      T v = sh[0][u];
+      for (int s = 1; s < WAVES / 2; ++s) v += sh[s][u];
+      out[(is_bias ? n_in : k) * n_out + n] = v;
+    }
+  }
+}
+
 // ---- plans ---------------------------------------------------------------------------------------------------------------------------
 
 struct Tiles { int bm, bn, slices, k_slice; };
@@ -603,10 +771,51 @@ struct Dense {
     used -= round_up(bytes, 256);
   }
 
+  // The thin kernels' layers.  They read operands where they lie, so nothing else is asked of these.
+  static bool thin(const vmcpde_dense_args& a) { return sizeof(T) > 2 && a.n_in <= THIN && a.n_out <= THIN; }
+
+  template <int NT>
+  void thin_forward(const vmcpde_dense_args& a, const Epilogue<T>& e) {
+    const unsigned groups = (unsigned)std::min<int64_t>(ceil_div(a.rows, 64), 2048);
+    const T* x = static_cast<const T*>(a.x);
+    const T* w = static_cast<const T*>(a.kernel);
+    const int64_t sk = a.kernel_t ? 1 : a.ldk, sn = a.kernel_t ? a.ldk : 1;
+    if (a.n_in <= 8) thin_forward_kernel<T, 2, NT><<<groups, 256, 0, stream>>>(x, a.ldx, w, sk, sn, a.rows, (int)a.n_in, e);
+    else if (a.n_in <= 16) thin_forward_kernel<T, 4, NT><<<groups, 256, 0, stream>>>(x, a.ldx, w, sk, sn, a.rows, (int)a.n_in, e);
+    else if (a.n_in <= 24) thin_forward_kernel<T, 6, NT><<<groups, 256, 0, stream>>>(x, a.ldx, w, sk, sn, a.rows, (int)a.n_in, e);
+    else thin_forward_kernel<T, 8, NT><<<groups, 256, 0, stream>>>(x, a.ldx, w, sk, sn, a.rows, (int)a.n_in, e);
+  }
+
+  template <int KT, int NT>
+  void thin_backward(const vmcpde_dense_args& a, unsigned groups, T* partial) {
+    thin_backward_kernel<T, KT, NT><<<groups, THIN_THREADS, 0, stream>>>(
+        static_cast<const T*>(a.dy), a.ldd, static_cast<const T*>(a.slope), (T)a.scale, a.dkernel ? static_cast<const T*>(a.x) : nullptr, a.ldx,
+        static_cast<const T*>(a.kernel), a.kernel_t ? 1 : a.ldk, a.kernel_t ? a.ldk : 1, a.rows, (int)a.n_in, (int)a.n_out, static_cast<T*>(a.dx), partial);
+  }
+
+  void thin_backward(const vmcpde_dense_args& a) {
+    const int64_t groups = std::max<int64_t>(1, std::min<int64_t>(ceil_div(a.rows, 16 * (THIN_THREADS / 64)), THIN_GROUPS)), sums = (a.n_in + 1) * a.n_out;
+    T* partial = a.dkernel || a.dbias ? static_cast<T*>(take(groups * sums * (int64_t)sizeof(T))) : nullptr;
+    if (!launch || (!partial && !(a.dx && a.rows))) return;
+    if (a.n_in <= 16 && a.n_out <= 16) thin_backward<1, 1>(a, (unsigned)groups, partial);
+    else if (a.n_in <= 16) thin_backward<1, 2>(a, (unsigned)groups, partial);
+    else if (a.n_out <= 16) thin_backward<2, 1>(a, (unsigned)groups, partial);
+    else thin_backward<2, 2>(a, (unsigned)groups, partial);
+    if (partial)
+      add_columns_kernel<T, T><<<(unsigned)ceil_div(sums, 64), 1024, 0, stream>>>(partial, (int)groups, sums, a.n_in * a.n_out, a.n_out, static_cast<T*>(a.dkernel),
+                                                                                 static_cast<T*>(a.dbias));
+  }
+
   void forward(const vmcpde_dense_args& a) {
     if (!a.rows) return;
     const Epilogue<T> e = {static_cast<const T*>(a.bias), static_cast<const T*>(a.residual), a.ldr, static_cast<T*>(a.y), a.ldy, static_cast<S*>(a.slope), a.n_out,
                            (A)a.scale, a.activation};
+    if constexpr (sizeof(T) > 2) {
+      if (thin(a)) {
+        if (launch) a.n_out <= 16 ? thin_forward<1>(a, e) : thin_forward<2>(a, e);
+        return;
+      }
+    }
     multiply({a.x, a.rows, a.n_in, a.ldx}, false, kernel_lines(a), !a.kernel_t, a.rows, a.n_out, a.n_in, e);
   }
 
@@ -615,6 +824,9 @@ struct Dense {
   }
 
   void backward(const vmcpde_dense_args& a) {
+    if constexpr (sizeof(T) > 2) {
+      if (thin(a)) return thin_backward(a);
+    }
     const Lines dy = {a.dy, a.rows, a.n_out, a.ldd};
     Lines dz = dy;
     const bool own = (a.dx || a.dkernel) && (a.slope || a.scale != 1.0 || !fetchable<T>(dy, a.dx));
@@ -630,7 +842,7 @@ struct Dense {
       if (launch) {
         scaled_copy<T>(dy, static_cast<const S*>(a.slope), a.scale, to, dz.ld, partial, groups, stream);
         if (a.dbias)
-          add_columns_kernel<A, T><<<dim3((unsigned)ceil_div(a.n_out, 64), 1), 1024, 0, stream>>>(partial, (int)groups, a.n_out, a.n_out, static_cast<T*>(a.dbias), nullptr);
+          add_columns_kernel<A, T><<<(unsigned)ceil_div(a.n_out, 64), 1024, 0, stream>>>(partial, (int)groups, a.n_out, a.n_out, 0, static_cast<T*>(a.dbias), nullptr);
       }
     }
     if (a.dx && a.rows) {

@@ -373,8 +373,8 @@ struct Norm {
             partial);
     }
     if (partial)
-      add_columns_kernel<A, W><<<dim3((unsigned)ceil_div(a.cols, 64), 2), 1024, 0, s>>>(partial, (int)groups, 2 * a.cols, a.cols, static_cast<W*>(a.dweight),
-                                                                                          static_cast<W*>(a.dbias));
+      add_columns_kernel<A, W><<<(unsigned)ceil_div(2 * a.cols, 64), 1024, 0, s>>>(partial, (int)groups, 2 * a.cols, a.cols, a.cols, static_cast<W*>(a.dweight),
+                                                                                   static_cast<W*>(a.dbias));
   }
 };
 

@@ -73,26 +73,28 @@ __device__ __forceinline__ void store_vec(T* __restrict__ row, int64_t col, int6
   }
 }
 
-// out_w[col] = sum_g partial[g * pitch + w * cols + col] for w = blockIdx.y (a null out is skipped): the last step of a sum over rows.
-// 64 columns x 16 parts of the groups a workgroup; the parts are added in their order.
+// Last step of a sum over rows: columns col < cols0 of sum_g partial[g * pitch + col] go to out0, the cols1 behind them to out1 (a null one is skipped).
+// 64 columns x 16 parts of the groups a workgroup; a part's groups, then the parts, are added in their order.
 template <typename A, typename W>
-static __global__ __launch_bounds__(1024) void add_columns_kernel(const A* __restrict__ partial, int groups, int64_t pitch, int64_t cols, W* __restrict__ out0,
-                                                           W* __restrict__ out1) {
+static __global__ __launch_bounds__(1024) void add_columns_kernel(const A* __restrict__ partial, int groups, int64_t pitch, int64_t cols0, int64_t cols1,
+                                                                  W* __restrict__ out0, W* __restrict__ out1) {
   __shared__ A sh[16][64];
-  const int which = blockIdx.y, part = threadIdx.x >> 6, c = threadIdx.x & 63;
-  W* out = which ? out1 : out0;
-  if (!out) return;
+  const int part = threadIdx.x >> 6, c = threadIdx.x & 63;
   const int64_t col = (int64_t)blockIdx.x * 64 + c;
   A v = 0;
-  if (col < cols) {
+  if (col < cols0 + cols1) {
 #pragma unroll 8
-    for (int g = part; g < groups; g += 16) v += partial[(int64_t)g * pitch + which * cols + col];
+    for (int g = part; g < groups; g += 16) v += partial[(int64_t)g * pitch + col];
   }
   sh[part][c] = v;
   __syncthreads();
-  if (part == 0 && col < cols) {
+  if (part == 0 && col < cols0 + cols1) {
     for (int p = 1; p < 16; ++p) v += sh[p][c];
-    out[col] = (W)v;
+    if (col < cols0) {
+      if (out0) out0[col] = (W)v;
+    } else if (out1) {
+      out1[col - cols0] = (W)v;
+    }
   }
 }
 
