@@ -9,12 +9,60 @@ namespace {
 
 // ---- the epilogue ------------------------------------------------------------------------------------------------------------------
 
+// tanh(z) and 1 - tanh(z)^2, to a few units in the last place (of the smallest numbers too): with e^(-2|z|) - 1 = m, tanh|z| = -m / (2 + m) and the slope
+// is 4 (1 + m) / (2 + m)^2.  m from a range reduction by ln 2 and the Taylor series of e^r - 1 on |r| <= ln 2 / 2 (degree 13: remainder 4e-18 r, fp32
+// degree 7: 1e-9 r).  A quarter of the library function's instructions, and no branches.
+__device__ __forceinline__ void tanh_slope(double z, double& a, double& slope) {
+  const double x = fabs(z) > 25.0 ? 25.0 : fabs(z), y = -2.0 * x, n = rint(y * 1.4426950408889634074);      // (NaN stays)
+  double r = fma(n, -6.93147180369123816490e-01, y);
+  r = fma(n, -1.90821492927058770002e-10, r);
+  double p = 1.0 / 6227020800.0;
+  p = fma(p, r, 1.0 / 479001600.0);
+  p = fma(p, r, 1.0 / 39916800.0);
+  p = fma(p, r, 1.0 / 3628800.0);
+  p = fma(p, r, 1.0 / 362880.0);
+  p = fma(p, r, 1.0 / 40320.0);
+  p = fma(p, r, 1.0 / 5040.0);
+  p = fma(p, r, 1.0 / 720.0);
+  p = fma(p, r, 1.0 / 120.0);
+  p = fma(p, r, 1.0 / 24.0);
+  p = fma(p, r, 1.0 / 6.0);
+  p = fma(p, r, 0.5);
+  p = fma(p * r, r, r);
+  const double two_n = ldexp(1.0, (int)n), m = fma(two_n, p, two_n - 1.0), den = 2.0 + m;
+  double q = __builtin_amdgcn_rcp(den);
+  q = fma(fma(-den, q, 1.0), q, q);
+  q = fma(fma(-den, q, 1.0), q, q);
+  double h = -m * q;
+  h = fma(fma(-den, h, -m), q, h);
+  a = copysign(h, z);
+  slope = 4.0 * fma(two_n, p, two_n) * q * q;
+}
+__device__ __forceinline__ void tanh_slope(float z, float& a, float& slope) {
+  const float x = fabsf(z) > 15.0f ? 15.0f : fabsf(z), y = -2.0f * x, n = rintf(y * 1.44269504f);
+  float r = fmaf(n, -0.693359375f, y);
+  r = fmaf(n, 2.12194440e-4f, r);
+  float p = 1.0f / 5040.0f;
+  p = fmaf(p, r, 1.0f / 720.0f);
+  p = fmaf(p, r, 1.0f / 120.0f);
+  p = fmaf(p, r, 1.0f / 24.0f);
+  p = fmaf(p, r, 1.0f / 6.0f);
+  p = fmaf(p, r, 0.5f);
+  p = fmaf(p * r, r, r);
+  const float two_n = ldexpf(1.0f, (int)n), m = fmaf(two_n, p, two_n - 1.0f), den = 2.0f + m;
+  float q = __builtin_amdgcn_rcpf(den);
+  q = fmaf(fmaf(-den, q, 1.0f), q, q);
+  float h = -m * q;
+  h = fmaf(fmaf(-den, h, -m), q, h);
+  a = copysignf(h, z);
+  slope = 4.0f * fmaf(two_n, p, two_n) * q * q;
+}
+
 // act(z) and act'(z), to a few units of the arithmetic type's last place
 template <typename A>
 __device__ __forceinline__ void activate_exact(int act, A z, A& a, A& slope) {
   if (act == VMCPDE_ACT_TANH) {
-    a = sizeof(A) == 8 ? (A)tanh((double)z) : (A)tanhf((float)z);
-    slope = 1 - a * a;
+    tanh_slope(z, a, slope);
   } else if (act == VMCPDE_ACT_GELU) {
     A cdf, density;
     if constexpr (sizeof(A) == 8) {
@@ -51,7 +99,6 @@ __device__ __forceinline__ void activate_short(int act, float z, float& a, float
     const float cdf = z < 0 ? tail : 1 - tail;
     a = z == -INFINITY ? 0 : z * cdf;
     slope = e != 0 ? cdf + z * (0.39894228f * e) : cdf;
-    if (z != z) a = slope = z;
   } else {
     const float gate = __builtin_amdgcn_rcpf(1 + __expf(-z));
     a = z == -INFINITY ? 0 : z * gate;
@@ -466,132 +513,186 @@ __global__ __launch_bounds__(256) void dense_dz_kernel(const T* __restrict__ dy,
 // ---- thin layers ---------------------------------------------------------------------------------------------------------------------
 
 // At most 32 inputs and outputs in fp32 or fp64 (the flow's own conditioners): bound by reading and writing the rows once.  The kernel's fragments
-// stay in registers, a wave takes sixteen rows at a time straight from memory, nothing passes through LDS, and no operand is copied.
-constexpr int THIN = 32, THIN_THREADS = 512, THIN_GROUPS = 256;
+// stay in registers, a wave takes sixteen rows at a time, and no operand is copied.  Between memory and the matrix instruction's lane layout a tile
+// passes through a piece of LDS of the wave's own: its elements are fetched and written in the order of the rows (whole lines at any pitch), and the
+// epilogue runs over them in that order too, so that no lane evaluates an activation for a column that is not there.
+constexpr int THIN = 32, THIN_THREADS = 512, THIN_GROUPS = 256, THIN_PITCH = 36, THIN_TILE = 16 * THIN_PITCH;
 
 __device__ __forceinline__ float4v mfma4(float a, float b, float4v c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ double4v mfma4(double a, double b, double4v c) { return __builtin_amdgcn_mfma_f64_16x16x4f64(a, b, c, 0, 0, 0); }
 // row of a 16 x 16 result that register r of a lane of group g holds
 template <typename T> __device__ __forceinline__ int result_row(int g, int r) { return sizeof(T) == 8 ? g + 4 * r : g * 4 + r; }
 
+// Element u < 16 n of sixteen rows of n <= 32 (the product is off by far less than the half that keeps it from a whole number)
+struct InOrder {
+  int n;
+  float inv;
+  __device__ __forceinline__ explicit InOrder(int n_) : n(n_), inv(1.0f / (float)n_) {}
+  __device__ __forceinline__ int row(int u) const { return (int)(((float)u + 0.5f) * inv); }
+  __device__ __forceinline__ int place(int u, int r) const { return r * THIN_PITCH + u - r * n; }
+};
+
 // The kernel's element (k, n) is at w[k * sk + n * sn].  KS: steps of four inputs, NT: tiles of sixteen outputs.
 template <typename T, int KS, int NT>
 __global__ __launch_bounds__(256) void thin_forward_kernel(const T* __restrict__ x, int64_t ldx, const T* __restrict__ w, int64_t sk, int64_t sn, int64_t rows, int n_in,
                                                            Epilogue<T> e) {
   typedef typename Matrix<T>::Acc Acc;
-  const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+  __shared__ T sh[4][2][THIN_TILE];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4, n_out = (int)e.n;
   const int64_t tiles = (rows + 15) / 16, stride = (int64_t)gridDim.x * 4;
-  int64_t tile = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  int64_t tile = (int64_t)blockIdx.x * 4 + wave;
   if (tile >= tiles) return;
-  T wf[KS][NT], bias[NT], xf[KS];
+  T* tx = sh[wave][0];
+  T* tz = sh[wave][1];
+  const InOrder in(n_in), out(n_out);
+  T wf[KS][NT], bias[NT], xv[KS];
 #pragma unroll
   for (int b = 0; b < NT; ++b) {
-    const int n = b * 16 + i;
-    bias[b] = e.bias && n < e.n ? e.bias[n] : (T)0;
+    bias[b] = e.bias && b * 16 + i < n_out ? e.bias[b * 16 + i] : (T)0;
 #pragma unroll
-    for (int s = 0; s < KS; ++s) wf[s][b] = 4 * s + g < n_in && n < e.n ? w[(4 * s + g) * sk + n * sn] : (T)0;
+    for (int s = 0; s < KS; ++s) wf[s][b] = 4 * s + g < n_in && b * 16 + i < n_out ? w[(4 * s + g) * sk + (b * 16 + i) * sn] : (T)0;
   }
+  for (int u = lane; u < THIN_TILE; u += 64) tx[u] = 0;          // (behind the inputs it stays zero)
   auto load = [&](int64_t at) {
 #pragma unroll
-    for (int s = 0; s < KS; ++s) xf[s] = at * 16 + i < rows && 4 * s + g < n_in ? x[(at * 16 + i) * ldx + 4 * s + g] : (T)0;
+    for (int j = 0; j < KS; ++j) {
+      const int u = lane + 64 * j, r = in.row(u);
+      xv[j] = r < 16 && at * 16 + r < rows ? x[(at * 16 + r) * ldx + u - r * n_in] : (T)0;
+    }
   };
   load(tile);
   for (; tile < tiles; tile += stride) {
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int j = 0; j < KS; ++j) {
+      const int u = lane + 64 * j, r = in.row(u);
+      if (r < 16) tx[in.place(u, r)] = xv[j];
+    }
+    if (tile + stride < tiles) load(tile + stride);
+    __builtin_amdgcn_wave_barrier();
     Acc acc[NT];
 #pragma unroll
-    for (int b = 0; b < NT; ++b) acc[b] = {0, 0, 0, 0};
+    for (int b = 0; b < NT; ++b) acc[b] = {bias[b], bias[b], bias[b], bias[b]};
 #pragma unroll
-    for (int s = 0; s < KS; ++s)
+    for (int s = 0; s < KS; ++s) {
+      const T xf = tx[i * THIN_PITCH + 4 * s + g];
 #pragma unroll
-      for (int b = 0; b < NT; ++b) acc[b] = mfma4(xf[s], wf[s][b], acc[b]);
-    if (tile + stride < tiles) load(tile + stride);
+      for (int b = 0; b < NT; ++b) acc[b] = mfma4(xf, wf[s][b], acc[b]);
+    }
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int64_t row = tile * 16 + result_row<T>(g, r);
+    for (int b = 0; b < NT; ++b)
 #pragma unroll
-      for (int b = 0; b < NT; ++b) {
-        const int n = b * 16 + i;
-        if (row < rows && n < e.n) {
-          T a, slope;
-          activate<T, T>(e.act, acc[b][r] + bias[b], a, slope);
-          a *= e.scale;
-          if (e.residual) a += e.residual[row * e.ldr + n];
-          e.y[row * e.ldy + n] = a;
-          if (e.slope) e.slope[row * e.n + n] = slope;
-        }
-      }
+      for (int r = 0; r < 4; ++r) tz[result_row<T>(g, r) * THIN_PITCH + b * 16 + i] = acc[b][r];
+    __builtin_amdgcn_wave_barrier();
+    const int live = (int)min((int64_t)16, rows - tile * 16) * n_out;
+#pragma unroll 1
+    for (int u = lane; u < live; u += 64) {                      // (rolled: the activations' code is longer than the loop saves)
+      const int r = out.row(u), n = u - r * n_out;
+      const int64_t row = tile * 16 + r;
+      T a, slope;
+      activate<T, T>(e.act, tz[out.place(u, r)], a, slope);
+      a *= e.scale;
+      if (e.residual) a += e.residual[row * e.ldr + n];
+      e.y[row * e.ldy + n] = a;
+      if (e.slope) e.slope[row * n_out + n] = slope;
     }
   }
 }
 
-// dx (may be null) and this workgroup's sums partial[blockIdx.x][n_in * n_out + n_out] of x^T dz and dz (null: not wanted).  dz = scale * slope * dy is
-// taken twice from memory (the second time from the caches), once for each product's lane layout.
+// dx (may be null) and this workgroup's sums partial[blockIdx.x][n_in * n_out + n_out] of x^T dz and dz (null: not wanted).
 template <typename T, int KT, int NT>
 __global__ __launch_bounds__(THIN_THREADS) void thin_backward_kernel(const T* __restrict__ dy, int64_t ldd, const T* __restrict__ slope, T scale,
                                                                      const T* __restrict__ x, int64_t ldx, const T* __restrict__ w, int64_t sk, int64_t sn, int64_t rows,
                                                                      int n_in, int n_out, T* __restrict__ dx, T* __restrict__ partial) {
   typedef typename Matrix<T>::Acc Acc;
   constexpr int NS = NT * 4, WAVES = THIN_THREADS / 64, SUMS = KT * 16 * NT * 16 + NT * 16;
-  __shared__ T sh[WAVES / 2][SUMS];
+  __shared__ T sh[WAVES * 2 * THIN_TILE];
+  static_assert(WAVES / 2 * SUMS <= WAVES * 2 * THIN_TILE, "the sums fit the tiles' LDS");
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
   const int64_t tiles = (rows + 15) / 16, stride = (int64_t)gridDim.x * WAVES;
+  T* tx = sh + wave * 2 * THIN_TILE;
+  T* tz = tx + THIN_TILE;
+  const InOrder in(n_in), out(n_out);
   T wf[NS][KT];
 #pragma unroll
   for (int s = 0; s < NS; ++s)
 #pragma unroll
     for (int a = 0; a < KT; ++a) wf[s][a] = dx && a * 16 + i < n_in && 4 * s + g < n_out ? w[(a * 16 + i) * sk + (4 * s + g) * sn] : (T)0;
   Acc sum[KT][NT];
-  T bias[NT];
+  T bias[NT], xv[KT * 4], zv[NS];
 #pragma unroll
   for (int b = 0; b < NT; ++b) {
     bias[b] = 0;
 #pragma unroll
     for (int a = 0; a < KT; ++a) sum[a][b] = {0, 0, 0, 0};
   }
-  auto dz = [&](int64_t row, int n) {
-    if (row >= rows || n >= n_out) return (T)0;
-    const T v = dy[row * ldd + n] * scale;
-    return slope ? v * slope[row * n_out + n] : v;
-  };
-  for (int64_t tile = (int64_t)blockIdx.x * WAVES + wave; tile < tiles; tile += stride) {
-    T zr[NS], zc[4][NT], xc[4][KT];
-    if (dx) {
+  for (int u = lane; u < 2 * THIN_TILE; u += 64) tx[u] = 0;      // (behind dz's columns it stays zero: they are summed over)
+  auto load = [&](int64_t at) {
 #pragma unroll
-      for (int s = 0; s < NS; ++s) zr[s] = dz(tile * 16 + i, 4 * s + g);
+    for (int j = 0; j < NS; ++j) {
+      const int u = lane + 64 * j, r = out.row(u);
+      const int64_t row = at * 16 + r;
+      zv[j] = 0;
+      if (r < 16 && row < rows) {
+        zv[j] = dy[row * ldd + u - r * n_out] * scale;
+        if (slope) zv[j] *= slope[at * 16 * n_out + u];
+      }
     }
+#pragma unroll
+    for (int j = 0; j < KT * 4; ++j) {
+      const int u = lane + 64 * j, r = in.row(u);
+      xv[j] = x && r < 16 && at * 16 + r < rows ? x[(at * 16 + r) * ldx + u - r * n_in] : (T)0;
+    }
+  };
+  int64_t tile = (int64_t)blockIdx.x * WAVES + wave;
+  if (tile < tiles) load(tile);
+  for (; tile < tiles; tile += stride) {
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int j = 0; j < NS; ++j) {
+      const int u = lane + 64 * j, r = out.row(u);
+      if (r < 16) tz[out.place(u, r)] = zv[j];
+    }
+#pragma unroll
+    for (int j = 0; j < KT * 4; ++j) {
+      const int u = lane + 64 * j, r = in.row(u);
+      if (r < 16) tx[in.place(u, r)] = xv[j];
+    }
+    if (tile + stride < tiles) load(tile + stride);
+    __builtin_amdgcn_wave_barrier();
     if (partial) {
 #pragma unroll
       for (int s = 0; s < 4; ++s) {
-        const int64_t row = tile * 16 + 4 * s + g;
+        T xc[KT];
 #pragma unroll
-        for (int b = 0; b < NT; ++b) zc[s][b] = dz(row, b * 16 + i);
-#pragma unroll
-        for (int a = 0; a < KT; ++a) xc[s][a] = x && row < rows && a * 16 + i < n_in ? x[row * ldx + a * 16 + i] : (T)0;
-      }
-#pragma unroll
-      for (int s = 0; s < 4; ++s)
+        for (int a = 0; a < KT; ++a) xc[a] = tx[(4 * s + g) * THIN_PITCH + a * 16 + i];
 #pragma unroll
         for (int b = 0; b < NT; ++b) {
-          bias[b] += zc[s][b];
+          const T zc = tz[(4 * s + g) * THIN_PITCH + b * 16 + i];
+          bias[b] += zc;
 #pragma unroll
-          for (int a = 0; a < KT; ++a) sum[a][b] = mfma4(xc[s][a], zc[s][b], sum[a][b]);
+          for (int a = 0; a < KT; ++a) sum[a][b] = mfma4(xc[a], zc, sum[a][b]);
         }
+      }
     }
     if (dx) {
       Acc acc[KT];
 #pragma unroll
       for (int a = 0; a < KT; ++a) acc[a] = {0, 0, 0, 0};
 #pragma unroll
-      for (int s = 0; s < NS; ++s)
+      for (int s = 0; s < NS; ++s) {
+        const T zr = tz[i * THIN_PITCH + 4 * s + g];
 #pragma unroll
-        for (int a = 0; a < KT; ++a) acc[a] = mfma4(zr[s], wf[s][a], acc[a]);
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int64_t row = tile * 16 + result_row<T>(g, r);
-#pragma unroll
-        for (int a = 0; a < KT; ++a)
-          if (row < rows && a * 16 + i < n_in) dx[row * n_in + a * 16 + i] = acc[a][r];
+        for (int a = 0; a < KT; ++a) acc[a] = mfma4(zr, wf[s][a], acc[a]);
       }
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int a = 0; a < KT; ++a)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) tx[result_row<T>(g, r) * THIN_PITCH + a * 16 + i] = acc[a][r];
+      __builtin_amdgcn_wave_barrier();
+      const int live = (int)min((int64_t)16, rows - tile * 16) * n_in;
+      for (int u = lane; u < live; u += 64) dx[tile * 16 * n_in + u] = tx[in.place(u, in.row(u))];
     }
   }
   if (!partial) return;
@@ -600,10 +701,11 @@ __global__ __launch_bounds__(THIN_THREADS) void thin_backward_kernel(const T* __
     bias[b] += __shfl_xor(bias[b], 16);
     bias[b] += __shfl_xor(bias[b], 32);
   }
+  __syncthreads();
   // the upper waves' sums onto the lower ones', then those in their order
   for (int half = 0; half < 2; ++half) {
     if (wave / (WAVES / 2) == half) {
-      T* to = sh[wave % (WAVES / 2)];
+      T* to = sh + wave % (WAVES / 2) * SUMS;
 #pragma unroll
       for (int b = 0; b < NT; ++b) {
 #pragma unroll
@@ -619,14 +721,14 @@ __global__ __launch_bounds__(THIN_THREADS) void thin_backward_kernel(const T* __
     }
     __syncthreads();
   }
-  T* out = partial + (int64_t)blockIdx.x * (n_in + 1) * n_out;
+  T* to = partial + (int64_t)blockIdx.x * (n_in + 1) * n_out;
   for (int u = threadIdx.x; u < SUMS; u += THIN_THREADS) {
     const int k = u / (NT * 16), n = u % (NT * 16);
     const bool is_bias = k == KT * 16;
     if (n < n_out && (is_bias || k < n_in)) {
-      T v = sh[0][u];
-      for (int s = 1; s < WAVES / 2; ++s) v += sh[s][u];
-      out[(is_bias ? n_in : k) * n_out + n] = v;
+      T v = sh[u];
+      for (int s = 1; s < WAVES / 2; ++s) v += sh[s * SUMS + u];
+      to[(is_bias ? n_in : k) * n_out + n] = v;
     }
   }
 }
@@ -776,7 +878,7 @@ struct Dense {
 
   template <int NT>
   void thin_forward(const vmcpde_dense_args& a, const Epilogue<T>& e) {
-    const unsigned groups = (unsigned)std::min<int64_t>(ceil_div(a.rows, 64), 2048);
+    const unsigned groups = (unsigned)std::min<int64_t>(ceil_div(a.rows, 64), 512);
     const T* x = static_cast<const T*>(a.x);
     const T* w = static_cast<const T*>(a.kernel);
     const int64_t sk = a.kernel_t ? 1 : a.ldk, sn = a.kernel_t ? a.ldk : 1;
