@@ -601,64 +601,55 @@ __global__ __launch_bounds__(256) void thin_forward_kernel(const T* __restrict__
 
 // dx (may be null) and this workgroup's sums partial[blockIdx.x][n_in * n_out + n_out] of x^T dz and dz (null: not wanted).
 template <typename T, int KT, int NT>
-__global__ __launch_bounds__(THIN_THREADS) void thin_backward_kernel(const T* __restrict__ dy, int64_t ldd, const T* __restrict__ slope, T scale,
+__global__ __launch_bounds__(THIN_THREADS, 4) void thin_backward_kernel(const T* __restrict__ dy, int64_t ldd, const T* __restrict__ slope, T scale,
                                                                      const T* __restrict__ x, int64_t ldx, const T* __restrict__ w, int64_t sk, int64_t sn, int64_t rows,
                                                                      int n_in, int n_out, T* __restrict__ dx, T* __restrict__ partial) {
   typedef typename Matrix<T>::Acc Acc;
   constexpr int NS = NT * 4, WAVES = THIN_THREADS / 64, SUMS = KT * 16 * NT * 16 + NT * 16;
-  __shared__ T sh[WAVES * 2 * THIN_TILE];
+  __shared__ T sh[WAVES * 2 * THIN_TILE], wt[KT * 16 * THIN_PITCH];
   static_assert(WAVES / 2 * SUMS <= WAVES * 2 * THIN_TILE, "the sums fit the tiles' LDS");
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
   const int64_t tiles = (rows + 15) / 16, stride = (int64_t)gridDim.x * WAVES;
   T* tx = sh + wave * 2 * THIN_TILE;
   T* tz = tx + THIN_TILE;
   const InOrder in(n_in), out(n_out);
-  T wf[NS][KT];
-#pragma unroll
-  for (int s = 0; s < NS; ++s)
-#pragma unroll
-    for (int a = 0; a < KT; ++a) wf[s][a] = dx && a * 16 + i < n_in && 4 * s + g < n_out ? w[(a * 16 + i) * sk + (4 * s + g) * sn] : (T)0;
+  for (int u = threadIdx.x; u < KT * 16 * NT * 16; u += THIN_THREADS) {
+    const int k = u / (NT * 16), n = u % (NT * 16);
+    wt[k * THIN_PITCH + n] = dx && k < n_in && n < n_out ? w[k * sk + n * sn] : (T)0;
+  }
+  for (int u = lane; u < 2 * THIN_TILE; u += 64) tx[u] = 0;      // (behind dz's columns it stays zero: they are summed over)
+  __syncthreads();
   Acc sum[KT][NT];
-  T bias[NT], xv[KT * 4], zv[NS];
+  T bias[NT];
 #pragma unroll
   for (int b = 0; b < NT; ++b) {
     bias[b] = 0;
 #pragma unroll
     for (int a = 0; a < KT; ++a) sum[a][b] = {0, 0, 0, 0};
   }
-  for (int u = lane; u < 2 * THIN_TILE; u += 64) tx[u] = 0;      // (behind dz's columns it stays zero: they are summed over)
-  auto load = [&](int64_t at) {
-#pragma unroll
-    for (int j = 0; j < NS; ++j) {
-      const int u = lane + 64 * j, r = out.row(u);
-      const int64_t row = at * 16 + r;
-      zv[j] = 0;
-      if (r < 16 && row < rows) {
-        zv[j] = dy[row * ldd + u - r * n_out] * scale;
-        if (slope) zv[j] *= slope[at * 16 * n_out + u];
+  for (int64_t tile = (int64_t)blockIdx.x * WAVES + wave; tile < tiles; tile += stride) {
+    const int live = (int)min((int64_t)16, rows - tile * 16);
+    const T* dyt = dy + tile * 16 * ldd;
+    const T* st = slope + tile * 16 * n_out;
+    const T* xt = x + tile * 16 * ldx;
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll 4
+    for (int u = lane; u < 16 * n_out; u += 64) {
+      const int r = out.row(u);
+      T v = 0;
+      if (r < live) {
+        v = dyt[r * (int)ldd + u - r * n_out] * scale;
+        if (slope) v *= st[u];
+      }
+      tz[out.place(u, r)] = v;
+    }
+    if (partial && x) {
+#pragma unroll 4
+      for (int u = lane; u < 16 * n_in; u += 64) {
+        const int r = in.row(u);
+        tx[in.place(u, r)] = r < live ? xt[r * (int)ldx + u - r * n_in] : (T)0;
       }
     }
-#pragma unroll
-    for (int j = 0; j < KT * 4; ++j) {
-      const int u = lane + 64 * j, r = in.row(u);
-      xv[j] = x && r < 16 && at * 16 + r < rows ? x[(at * 16 + r) * ldx + u - r * n_in] : (T)0;
-    }
-  };
-  int64_t tile = (int64_t)blockIdx.x * WAVES + wave;
-  if (tile < tiles) load(tile);
-  for (; tile < tiles; tile += stride) {
-    __builtin_amdgcn_wave_barrier();
-#pragma unroll
-    for (int j = 0; j < NS; ++j) {
-      const int u = lane + 64 * j, r = out.row(u);
-      if (r < 16) tz[out.place(u, r)] = zv[j];
-    }
-#pragma unroll
-    for (int j = 0; j < KT * 4; ++j) {
-      const int u = lane + 64 * j, r = in.row(u);
-      if (r < 16) tx[in.place(u, r)] = xv[j];
-    }
-    if (tile + stride < tiles) load(tile + stride);
     __builtin_amdgcn_wave_barrier();
     if (partial) {
 #pragma unroll
@@ -683,7 +674,7 @@ __global__ __launch_bounds__(THIN_THREADS) void thin_backward_kernel(const T* __
       for (int s = 0; s < NS; ++s) {
         const T zr = tz[i * THIN_PITCH + 4 * s + g];
 #pragma unroll
-        for (int a = 0; a < KT; ++a) acc[a] = mfma4(zr, wf[s][a], acc[a]);
+        for (int a = 0; a < KT; ++a) acc[a] = mfma4(zr, wt[(a * 16 + i) * THIN_PITCH + 4 * s + g], acc[a]);
       }
       __builtin_amdgcn_wave_barrier();
 #pragma unroll
@@ -691,8 +682,9 @@ __global__ __launch_bounds__(THIN_THREADS) void thin_backward_kernel(const T* __
 #pragma unroll
         for (int r = 0; r < 4; ++r) tx[result_row<T>(g, r) * THIN_PITCH + a * 16 + i] = acc[a][r];
       __builtin_amdgcn_wave_barrier();
-      const int live = (int)min((int64_t)16, rows - tile * 16) * n_in;
-      for (int u = lane; u < live; u += 64) dx[tile * 16 * n_in + u] = tx[in.place(u, in.row(u))];
+      T* dxt = dx + tile * 16 * n_in;
+#pragma unroll 4
+      for (int u = lane; u < live * n_in; u += 64) dxt[u] = tx[in.place(u, in.row(u))];
     }
   }
   if (!partial) return;
