@@ -553,11 +553,13 @@ __global__ __launch_bounds__(256) void thin_forward_kernel(const T* __restrict__
     for (int s = 0; s < KS; ++s) wf[s][b] = 4 * s + g < n_in && b * 16 + i < n_out ? w[(4 * s + g) * sk + (b * 16 + i) * sn] : (T)0;
   }
   for (int u = lane; u < THIN_TILE; u += 64) tx[u] = 0;          // (behind the inputs it stays zero)
-  auto load = [&](int64_t at) {
+  auto load = [&](int64_t at) {                                  // (no branches: a lane without an element reads the tile's first one, so that all loads fly at once)
+    const T* p = x + at * 16 * ldx;
+    const int live = (int)min((int64_t)16, rows - at * 16);
 #pragma unroll
     for (int j = 0; j < KS; ++j) {
       const int u = lane + 64 * j, r = in.row(u);
-      xv[j] = r < 16 && at * 16 + r < rows ? x[(at * 16 + r) * ldx + u - r * n_in] : (T)0;
+      xv[j] = p[r < live ? r * (int)ldx + u - r * n_in : 0];
     }
   };
   load(tile);
@@ -566,7 +568,7 @@ __global__ __launch_bounds__(256) void thin_forward_kernel(const T* __restrict__
 #pragma unroll
     for (int j = 0; j < KS; ++j) {
       const int u = lane + 64 * j, r = in.row(u);
-      if (r < 16) tx[in.place(u, r)] = xv[j];
+      if (r < 16) tx[in.place(u, r)] = xv[j];                   // (a row that is not there takes any numbers: its results are not written)
     }
     if (tile + stride < tiles) load(tile + stride);
     __builtin_amdgcn_wave_barrier();
@@ -601,7 +603,7 @@ __global__ __launch_bounds__(256) void thin_forward_kernel(const T* __restrict__
 
 // dx (may be null) and this workgroup's sums partial[blockIdx.x][n_in * n_out + n_out] of x^T dz and dz (null: not wanted).
 template <typename T, int KT, int NT>
-__global__ __launch_bounds__(THIN_THREADS, 4) void thin_backward_kernel(const T* __restrict__ dy, int64_t ldd, const T* __restrict__ slope, T scale,
+__global__ __launch_bounds__(THIN_THREADS) void thin_backward_kernel(const T* __restrict__ dy, int64_t ldd, const T* __restrict__ slope, T scale,
                                                                      const T* __restrict__ x, int64_t ldx, const T* __restrict__ w, int64_t sk, int64_t sn, int64_t rows,
                                                                      int n_in, int n_out, T* __restrict__ dx, T* __restrict__ partial) {
   typedef typename Matrix<T>::Acc Acc;
@@ -627,29 +629,42 @@ __global__ __launch_bounds__(THIN_THREADS, 4) void thin_backward_kernel(const T*
 #pragma unroll
     for (int a = 0; a < KT; ++a) sum[a][b] = {0, 0, 0, 0};
   }
-  for (int64_t tile = (int64_t)blockIdx.x * WAVES + wave; tile < tiles; tile += stride) {
+  T dv[NS], sv[NS], xv[KT * 4];
+  auto load = [&](int64_t at) {                                  // (no branches: see above)
+    const T* pd = dy + at * 16 * ldd;
+    const T* ps = slope + at * 16 * n_out;
+    const T* px = x + at * 16 * ldx;
+    const int live = (int)min((int64_t)16, rows - at * 16);
+#pragma unroll
+    for (int j = 0; j < NS; ++j) {
+      const int u = lane + 64 * j, r = out.row(u);
+      dv[j] = pd[r < live ? r * (int)ldd + u - r * n_out : 0];
+      sv[j] = slope ? ps[r < live ? u : 0] : (T)1;
+    }
+    if (x)
+#pragma unroll
+      for (int j = 0; j < KT * 4; ++j) {
+        const int u = lane + 64 * j, r = in.row(u);
+        xv[j] = px[r < live ? r * (int)ldx + u - r * n_in : 0];
+      }
+  };
+  int64_t tile = (int64_t)blockIdx.x * WAVES + wave;
+  if (tile < tiles) load(tile);
+  for (; tile < tiles; tile += stride) {
     const int live = (int)min((int64_t)16, rows - tile * 16);
-    const T* dyt = dy + tile * 16 * ldd;
-    const T* st = slope + tile * 16 * n_out;
-    const T* xt = x + tile * 16 * ldx;
     __builtin_amdgcn_wave_barrier();
-#pragma unroll 4
-    for (int u = lane; u < 16 * n_out; u += 64) {
-      const int r = out.row(u);
-      T v = 0;
-      if (r < live) {
-        v = dyt[r * (int)ldd + u - r * n_out] * scale;
-        if (slope) v *= st[u];
-      }
-      tz[out.place(u, r)] = v;
+#pragma unroll
+    for (int j = 0; j < NS; ++j) {
+      const int u = lane + 64 * j, r = out.row(u);
+      if (r < 16) tz[out.place(u, r)] = r < live ? dv[j] * scale * sv[j] : (T)0;
     }
-    if (partial && x) {
-#pragma unroll 4
-      for (int u = lane; u < 16 * n_in; u += 64) {
-        const int r = in.row(u);
-        tx[in.place(u, r)] = r < live ? xt[r * (int)ldx + u - r * n_in] : (T)0;
+    if (x)
+#pragma unroll
+      for (int j = 0; j < KT * 4; ++j) {
+        const int u = lane + 64 * j, r = in.row(u);
+        if (r < 16) tx[in.place(u, r)] = r < live ? xv[j] : (T)0;
       }
-    }
+    if (tile + stride < tiles) load(tile + stride);
     __builtin_amdgcn_wave_barrier();
     if (partial) {
 #pragma unroll
