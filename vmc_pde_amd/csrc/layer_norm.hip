@@ -4,10 +4,14 @@
 //
 // Bound by memory.  A row is read once and stays in registers (fp32, fp64 rows in fp64): the mean is taken first and the variance from the
 // deviations, so a row far from zero loses nothing.  16, 64, 256 or 1024 lanes share a row, so that a lane holds at most four 16-byte
-// vectors; longer rows go through the kernels that read them again.  Loads and stores are 16 bytes a lane at any alignment (global memory
-// takes them unaligned; only a row's last, partial vector goes element by element), so odd widths cost one path, not another kernel.
+// vectors; longer rows (and those shorter than a vector) go through the kernels that read them again.  Loads and stores are 16 bytes a lane at any
+// alignment (global memory takes them unaligned).  A row's last, partial vector is moved back to end with the row: it repeats columns of the lane before,
+// which it leaves out of the row's sums and otherwise computes and writes a second time, with the same result.  So a row is loaded without a branch, and
+// the next row's loads fly while one is reduced.
 // The weights' gradients: every workgroup takes every gridDim-th group of rows and adds its columns in registers; the workgroups' sums are
 // added in index order by a second launch -- no atomics, the same bits every time.
+#include <algorithm>
+
 #include "layers.hpp"
 
 using namespace vmcpde;
@@ -42,58 +46,114 @@ __device__ __forceinline__ void row_sum(A (&v)[K], A* sh) {
   }
 }
 
-template <typename T, typename W, int LANES, int ITER, int THREADS>
+// Where a lane's vectors lie in a row of cols >= V: from column base[i], of which the first skip[i] belong to the lane before (V or more: all of them).
+template <int LANES, int ITER, int V>
+struct Span {
+  int base[ITER], skip[ITER];
+  __device__ __forceinline__ explicit Span(int64_t cols) {
+    const int lane = threadIdx.x % LANES;
+#pragma unroll
+    for (int i = 0; i < ITER; ++i) {
+      const int col = (i * LANES + lane) * V;
+      base[i] = min(col, (int)cols - V);
+      skip[i] = col - base[i];
+    }
+  }
+};
+template <typename T, int V>
+struct __attribute__((packed, aligned(sizeof(T)))) Raw { T v[V]; };
+template <typename T, int V>
+__device__ __forceinline__ Raw<T, V> raw_at(const T* p) { return *reinterpret_cast<const Raw<T, V>*>(p); }
+template <typename T, int V, typename A>
+__device__ __forceinline__ void put(T* p, const A (&v)[V]) {
+  Raw<T, V> r;
+#pragma unroll
+  for (int k = 0; k < V; ++k) r.v[k] = (T)v[k];
+  *reinterpret_cast<Raw<T, V>*>(p) = r;
+}
+// a weight's or bias' vector; `none` where there is none
+template <typename W, int V, typename A>
+__device__ __forceinline__ void weights_at(const W* p, int base, A none, A (&out)[V]) {
+  if (p) {
+    const Raw<W, V> r = raw_at<W, V>(p + base);
+#pragma unroll
+    for (int k = 0; k < V; ++k) out[k] = (A)r.v[k];
+  } else {
+#pragma unroll
+    for (int k = 0; k < V; ++k) out[k] = none;
+  }
+}
+
+// Every workgroup takes every gridDim-th group of rows.  The weights stay in registers where a lane holds at most 16 elements: read anew for every row
+// they are up to four times the row's own traffic, from the caches.  EXACT: the row is LANES * ITER vectors.
+template <typename T, typename W, int LANES, int ITER, int THREADS, bool EXACT>
 __global__ __launch_bounds__(THREADS) void norm_forward_kernel(const T* __restrict__ x, int64_t ldx, const W* __restrict__ weight, const W* __restrict__ bias,
                                                                typename Wide<T>::type eps, int64_t rows, int64_t cols, T* __restrict__ y, int64_t ldy,
                                                                typename Wide<T>::type* __restrict__ mean_out, typename Wide<T>::type* __restrict__ rstd_out) {
   typedef typename Wide<T>::type A;
-  constexpr int V = vec_of<T>(), GROUPS = THREADS / LANES;
-  __shared__ A sh[2][THREADS / 64];
+  constexpr int V = vec_of<T>(), GROUPS = THREADS / LANES, WAVES = THREADS / 64;
+  constexpr bool KEEP = ITER * V <= 16;
+  __shared__ A sh[2][2][WAVES];                // (two sets of slots in turn: a wave may be a row ahead of the slowest)
   const int lane = threadIdx.x % LANES;
-  const int64_t row = (int64_t)blockIdx.x * GROUPS + threadIdx.x / LANES;
-  const bool live = row < rows;              // (a whole group of lanes; the sums below need every lane of a wave)
-  const T* xr = x + (live ? row : 0) * ldx;
-  A v[ITER][V];
-  A s[1] = {0};
+  const Span<LANES, ITER, V> at(cols);
+  A w[KEEP ? ITER : 1][V], b[KEEP ? ITER : 1][V];
+  if constexpr (KEEP) {
 #pragma unroll
-  for (int i = 0; i < ITER; ++i) {
-    load_vec<T, V>(xr, ((int64_t)i * LANES + lane) * V, cols, v[i]);
-#pragma unroll
-    for (int k = 0; k < V; ++k) s[0] += v[i][k];
-  }
-  row_sum<LANES>(s, sh[0]);
-  const A mean = s[0] / (A)cols;
-  A q[1] = {0};
-#pragma unroll
-  for (int i = 0; i < ITER; ++i)
-#pragma unroll
-    for (int k = 0; k < V; ++k) {
-      v[i][k] -= mean;
-      if (((int64_t)i * LANES + lane) * V + k < cols) q[0] += v[i][k] * v[i][k];
+    for (int i = 0; i < ITER; ++i) {
+      weights_at<W, V>(weight, at.base[i], (A)1, w[i]);
+      weights_at<W, V>(bias, at.base[i], (A)0, b[i]);
     }
-  row_sum<LANES>(q, sh[1]);
-  const A rstd = reciprocal_root<A>(q[0] / (A)cols + eps);
-  if (!live) return;
-  if (lane == 0 && mean_out) {
-    mean_out[row] = mean;
-    rstd_out[row] = rstd;
   }
-  T* yr = y + row * ldy;
+  Raw<T, V> next[ITER];
+  auto fetch = [&](int64_t row) {
+    const T* xr = x + (GROUPS == 1 || row < rows ? row : 0) * ldx;
 #pragma unroll
-  for (int i = 0; i < ITER; ++i) {
-    const int64_t col = ((int64_t)i * LANES + lane) * V;
-    if (col < cols) {
-      A w[V], b[V];
-      if (weight) load_vec<W, V>(weight, col, cols, w);
-      if (bias) load_vec<W, V>(bias, col, cols, b);
+    for (int i = 0; i < ITER; ++i) next[i] = raw_at<T, V>(xr + at.base[i]);
+  };
+  int64_t first = (int64_t)blockIdx.x * GROUPS;
+  fetch(first + threadIdx.x / LANES);
+  for (int turn = 0; first < rows; turn ^= 1) {
+    const int64_t row = first + threadIdx.x / LANES;
+    first += (int64_t)gridDim.x * GROUPS;
+    A v[ITER][V], s[1] = {0}, q[1] = {0};
+#pragma unroll
+    for (int i = 0; i < ITER; ++i)
 #pragma unroll
       for (int k = 0; k < V; ++k) {
-        A h = v[i][k] * rstd;
-        if (weight) h *= w[k];
-        if (bias) h += b[k];
-        v[i][k] = h;
+        v[i][k] = (A)next[i].v[k];
+        s[0] += EXACT || k >= at.skip[i] ? v[i][k] : (A)0;
       }
-      store_vec<T, V>(yr, col, cols, v[i]);
+    if (first < rows) fetch(first + threadIdx.x / LANES);
+    row_sum<LANES>(s, sh[turn][0]);
+    const A mean = s[0] / (A)cols;
+#pragma unroll
+    for (int i = 0; i < ITER; ++i)
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        v[i][k] -= mean;
+        q[0] += EXACT || k >= at.skip[i] ? v[i][k] * v[i][k] : (A)0;
+      }
+    row_sum<LANES>(q, sh[turn][1]);
+    const A rstd = reciprocal_root<A>(q[0] / (A)cols + eps);
+    if (GROUPS > 1 && row >= rows) continue;   // (a whole group of lanes; the sums above need every lane of a wave)
+    if (lane == 0 && mean_out) {
+      mean_out[row] = mean;
+      rstd_out[row] = rstd;
+    }
+    T* yr = y + row * ldy;
+#pragma unroll
+    for (int i = 0; i < ITER; ++i) {
+      A wi[V], bi[V];
+      if constexpr (KEEP) {
+#pragma unroll
+        for (int k = 0; k < V; ++k) wi[k] = w[i][k], bi[k] = b[i][k];
+      } else {
+        weights_at<W, V>(weight, at.base[i], (A)1, wi);
+        weights_at<W, V>(bias, at.base[i], (A)0, bi);
+      }
+#pragma unroll
+      for (int k = 0; k < V; ++k) v[i][k] = v[i][k] * rstd * wi[k] + bi[k];
+      if (EXACT || at.skip[i] < V) put<T, V>(yr + at.base[i], v[i]);
     }
   }
 }
@@ -144,7 +204,7 @@ __global__ __launch_bounds__(1024) void norm_forward_wide_kernel(const T* __rest
 }
 
 // dx (may be null) and, with `partial`, this workgroup's column sums: partial[group][2][cols] = { sum dy h, sum dy }
-template <typename T, typename W, int LANES, int ITER, int THREADS>
+template <typename T, typename W, int LANES, int ITER, int THREADS, bool EXACT>
 __global__ __launch_bounds__(THREADS) void norm_backward_kernel(const T* __restrict__ dy, int64_t ldd, const T* __restrict__ x, int64_t ldx,
                                                                 const typename Wide<T>::type* __restrict__ mean_in,
                                                                 const typename Wide<T>::type* __restrict__ rstd_in, const W* __restrict__ weight,
@@ -152,38 +212,62 @@ __global__ __launch_bounds__(THREADS) void norm_backward_kernel(const T* __restr
   typedef typename Wide<T>::type A;
   constexpr int V = vec_of<T>(), GROUPS = THREADS / LANES, WAVES = THREADS / 64;
   constexpr int SHARED = LANES <= 64 ? WAVES * LANES * ITER * V : 4 * WAVES;   // column sums of every wave, or the slots of the row sums
+  constexpr bool KEEP = LANES < 1024 || ITER * V <= 8;           // (1024 lanes have 128 registers each)
   __shared__ A sh[SHARED];
   const int lane = threadIdx.x % LANES;
   const A inv = (A)1 / (A)cols;
-  A dw[ITER][V], db[ITER][V];
+  const Span<LANES, ITER, V> at(cols);
+  A dw[ITER][V], db[ITER][V], w[KEEP ? ITER : 1][V];
 #pragma unroll
-  for (int i = 0; i < ITER; ++i)
+  for (int i = 0; i < ITER; ++i) {
+    if constexpr (KEEP) weights_at<W, V>(weight, at.base[i], (A)1, w[i]);
 #pragma unroll
     for (int k = 0; k < V; ++k) dw[i][k] = db[i][k] = 0;
-  int turn = 0;
-  for (int64_t first = (int64_t)blockIdx.x * GROUPS; first < rows; first += (int64_t)gridDim.x * GROUPS, turn ^= 1) {
-    const int64_t row = first + threadIdx.x / LANES;
-    const bool live = row < rows;
-    const int64_t r = live ? row : 0;
-    const int64_t width = live ? cols : 0;      // lanes of no row read nothing and add zeros
-    const A mean = mean_in[r], rstd = rstd_in[r];
-    A h[ITER][V], g[ITER][V];
-    A s[2] = {0, 0};
+  }
+  Raw<T, V> next_x[ITER], next_d[ITER];
+  A next_mean, next_rstd;
+  auto fetch = [&](int64_t row) {
+    const int64_t r = GROUPS == 1 || row < rows ? row : 0;
+    next_mean = mean_in[r], next_rstd = rstd_in[r];
 #pragma unroll
     for (int i = 0; i < ITER; ++i) {
-      const int64_t col = ((int64_t)i * LANES + lane) * V;
-      A w[V];
-      load_vec<T, V>(dy + r * ldd, col, width, g[i]);
-      load_vec<T, V>(x + r * ldx, col, width, h[i]);
-      if (weight) load_vec<W, V>(weight, col, cols, w);
+      next_d[i] = raw_at<T, V>(dy + r * ldd + at.base[i]);
+      next_x[i] = raw_at<T, V>(x + r * ldx + at.base[i]);
+    }
+  };
+  int64_t first = (int64_t)blockIdx.x * GROUPS;
+  if (first < rows) fetch(first + threadIdx.x / LANES);
+  for (int turn = 0; first < rows; turn ^= 1) {
+    const int64_t row = first + threadIdx.x / LANES;
+    const bool live = GROUPS == 1 || row < rows;                 // lanes of no row add zeros
+    first += (int64_t)gridDim.x * GROUPS;
+    const A mean = next_mean, rstd = next_rstd;
+    A h[ITER][V], g[ITER][V], s[2] = {0, 0};
+#pragma unroll
+    for (int i = 0; i < ITER; ++i)
 #pragma unroll
       for (int k = 0; k < V; ++k) {
-        h[i][k] = col + k < width ? (h[i][k] - mean) * rstd : (A)0;
+        h[i][k] = live ? ((A)next_x[i].v[k] - mean) * rstd : (A)0;
+        g[i][k] = live ? (A)next_d[i].v[k] : (A)0;
+      }
+    if (first < rows) fetch(first + threadIdx.x / LANES);
+#pragma unroll
+    for (int i = 0; i < ITER; ++i) {
+      A wi[V];
+      if constexpr (KEEP) {
+#pragma unroll
+        for (int k = 0; k < V; ++k) wi[k] = w[i][k];
+      } else {
+        weights_at<W, V>(weight, at.base[i], (A)1, wi);
+      }
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
         dw[i][k] += g[i][k] * h[i][k];
         db[i][k] += g[i][k];
-        if (weight) g[i][k] *= w[k];
-        s[0] += g[i][k];
-        s[1] += g[i][k] * h[i][k];
+        g[i][k] *= wi[k];
+        const bool mine = EXACT || k >= at.skip[i];
+        s[0] += mine ? g[i][k] : (A)0;
+        s[1] += mine ? g[i][k] * h[i][k] : (A)0;
       }
     }
     if (dx) {
@@ -191,12 +275,9 @@ __global__ __launch_bounds__(THREADS) void norm_backward_kernel(const T* __restr
       const A c1 = s[0] * inv, c2 = s[1] * inv;
 #pragma unroll
       for (int i = 0; i < ITER; ++i) {
-        const int64_t col = ((int64_t)i * LANES + lane) * V;
-        if (col < width) {
 #pragma unroll
-          for (int k = 0; k < V; ++k) g[i][k] = rstd * (g[i][k] - c1 - h[i][k] * c2);
-          store_vec<T, V>(dx + r * cols, col, cols, g[i]);
-        }
+        for (int k = 0; k < V; ++k) g[i][k] = rstd * (g[i][k] - c1 - h[i][k] * c2);
+        if (live && (EXACT || at.skip[i] < V)) put<T, V>(dx + row * cols + at.base[i], g[i]);
       }
     }
   }
@@ -206,7 +287,8 @@ __global__ __launch_bounds__(THREADS) void norm_backward_kernel(const T* __restr
   for (int which = 0; which < 2; ++which) {
     if constexpr (LANES > 64) {
 #pragma unroll
-      for (int i = 0; i < ITER; ++i) store_vec<A, V>(out + which * cols, ((int64_t)i * LANES + lane) * V, cols, which ? db[i] : dw[i]);
+      for (int i = 0; i < ITER; ++i)
+        if (EXACT || at.skip[i] < V) put<A, V>(out + which * cols + at.base[i], which ? db[i] : dw[i]);
     } else {
       const int wave = threadIdx.x >> 6;
       __syncthreads();
@@ -219,13 +301,14 @@ __global__ __launch_bounds__(THREADS) void norm_backward_kernel(const T* __restr
             v += __shfl_xor(v, 16);
             v += __shfl_xor(v, 32);
           }
-          if ((threadIdx.x & 63) < LANES) sh[(wave * ITER + i) * LANES * V + lane * V + k] = v;
+          if ((threadIdx.x & 63) < LANES) sh[((wave * ITER + i) * LANES + lane) * V + k] = v;
         }
       __syncthreads();
       for (int c = threadIdx.x; c < ITER * LANES * V; c += THREADS) {
         A v = 0;
         for (int w = 0; w < WAVES; ++w) v += sh[w * ITER * LANES * V + c];
-        if (c < cols) out[which * cols + c] = v;
+        const int col = c / V * V;
+        if (col < cols) out[which * cols + min(col, (int)cols - V) + c % V] = v;
       }
     }
   }
@@ -296,10 +379,12 @@ __global__ __launch_bounds__(256) void norm_columns_kernel(const T* __restrict__
 // lanes that share a row, vectors a lane holds of it, workgroup size; lanes = 0: the kernels for wide rows
 struct Shape { int lanes, iter, threads; };
 
-// most: vectors a lane may hold below 1024 lanes.  4 forward (one array of the row in registers), 2 backward (four arrays of it)
-Shape shape_of(int64_t cols, int vec, int most) {
+// Vectors that a lane may hold, below 1024 lanes and with them (128 registers each).  Forward (the row and two weights): two of 16-bit elements, else four;
+// backward (five arrays of the row): two, four of fp32 at 1024 lanes.
+Shape shape_of(int64_t cols, int vec, int most, int most_1024) {
+  if (cols < vec) return {0, 0, 1024};
   for (int lanes : {16, 64, 256, 1024}) {
-    const int limit = lanes == 1024 ? 4 : most;
+    const int limit = lanes == 1024 ? most_1024 : most;
     const int64_t vectors = ceil_div(cols, (int64_t)lanes * vec);
     if (vectors <= limit) return {lanes, vectors <= 1 ? 1 : vectors <= 2 ? 2 : 4, lanes <= 256 ? 256 : 1024};
   }
@@ -321,7 +406,12 @@ struct Norm {
 
   template <int LANES, int ITER, int THREADS>
   static void forward_as(const vmcpde_norm_args& a, hipStream_t s) {
-    norm_forward_kernel<T, W, LANES, ITER, THREADS><<<(unsigned)ceil_div(a.rows, THREADS / LANES), THREADS, 0, s>>>(
+    if (a.cols == (int64_t)LANES * ITER * V) forward_exactly<LANES, ITER, THREADS, true>(a, s);
+    else forward_exactly<LANES, ITER, THREADS, false>(a, s);
+  }
+  template <int LANES, int ITER, int THREADS, bool EXACT>
+  static void forward_exactly(const vmcpde_norm_args& a, hipStream_t s) {
+    norm_forward_kernel<T, W, LANES, ITER, THREADS, EXACT><<<(unsigned)std::min<int64_t>(ceil_div(a.rows, THREADS / LANES), THREADS == 1024 ? 512 : 2048), THREADS, 0, s>>>(
         static_cast<const T*>(a.x), a.ldx, static_cast<const W*>(a.weight), static_cast<const W*>(a.bias), (A)a.eps, a.rows, a.cols, static_cast<T*>(a.y), a.ldy,
         static_cast<A*>(a.mean), static_cast<A*>(a.rstd));
   }
@@ -329,10 +419,10 @@ struct Norm {
   static void forward_iter(int iter, const vmcpde_norm_args& a, hipStream_t s) {
     if (iter == 1) forward_as<LANES, 1, THREADS>(a, s);
     else if (iter == 2) forward_as<LANES, 2, THREADS>(a, s);
-    else forward_as<LANES, 4, THREADS>(a, s);
+    else if constexpr (sizeof(T) > 2) forward_as<LANES, 4, THREADS>(a, s);
   }
   static void forward(const vmcpde_norm_args& a, hipStream_t s) {
-    const Shape p = shape_of(a.cols, V, 4);
+    const Shape p = shape_of(a.cols, V, sizeof(T) == 2 ? 2 : 4, sizeof(T) == 2 ? 2 : 4);
     if (p.lanes == 16) forward_iter<16, 256>(p.iter, a, s);
     else if (p.lanes == 64) forward_iter<64, 256>(p.iter, a, s);
     else if (p.lanes == 256) forward_iter<256, 256>(p.iter, a, s);
@@ -344,7 +434,12 @@ struct Norm {
 
   template <int LANES, int ITER, int THREADS>
   static void backward_as(const vmcpde_norm_args& a, int64_t groups, A* partial, hipStream_t s) {
-    norm_backward_kernel<T, W, LANES, ITER, THREADS><<<(unsigned)groups, THREADS, 0, s>>>(
+    if (a.cols == (int64_t)LANES * ITER * V) backward_exactly<LANES, ITER, THREADS, true>(a, groups, partial, s);
+    else backward_exactly<LANES, ITER, THREADS, false>(a, groups, partial, s);
+  }
+  template <int LANES, int ITER, int THREADS, bool EXACT>
+  static void backward_exactly(const vmcpde_norm_args& a, int64_t groups, A* partial, hipStream_t s) {
+    norm_backward_kernel<T, W, LANES, ITER, THREADS, EXACT><<<(unsigned)groups, THREADS, 0, s>>>(
         static_cast<const T*>(a.dy), a.ldd, static_cast<const T*>(a.x), a.ldx, static_cast<const A*>(a.mean), static_cast<const A*>(a.rstd),
         static_cast<const W*>(a.weight), a.rows, a.cols, static_cast<T*>(a.dx), partial);
   }
@@ -354,15 +449,16 @@ struct Norm {
     else backward_as<LANES, 2, THREADS>(a, groups, partial, s);
   }
   static void backward(const vmcpde_norm_args& a, void* workspace, hipStream_t s) {
-    const Shape p = shape_of(a.cols, V, 2);
+    const Shape p = shape_of(a.cols, V, 2, sizeof(T) == 4 ? 4 : 2);
     const int64_t groups = backward_groups(p, a.rows);
     A* partial = a.dweight || a.dbias ? static_cast<A*>(workspace) : nullptr;
     if (p.lanes == 16) backward_iter<16, 256>(p.iter, a, groups, partial, s);
     else if (p.lanes == 64) backward_iter<64, 256>(p.iter, a, groups, partial, s);
     else if (p.lanes == 256) backward_iter<256, 256>(p.iter, a, groups, partial, s);
     else if (p.lanes == 1024 && p.iter <= 2) backward_iter<1024, 1024>(p.iter, a, groups, partial, s);
-    else if (p.lanes == 1024) backward_as<1024, 4, 1024>(a, groups, partial, s);
-    else {
+    else if (p.lanes == 1024) {
+      if constexpr (sizeof(T) == 4) backward_as<1024, 4, 1024>(a, groups, partial, s);
+    } else {
       if (a.dx && a.rows)
         norm_backward_wide_kernel<T, W><<<(unsigned)a.rows, 1024, 0, s>>>(static_cast<const T*>(a.dy), a.ldd, static_cast<const T*>(a.x), a.ldx,
                                                                           static_cast<const A*>(a.mean), static_cast<const A*>(a.rstd),
@@ -417,7 +513,7 @@ int vmcpde_layer_norm(const vmcpde_norm_args* a, void* stream) {
 
 int64_t vmcpde_layer_norm_backward_workspace_bytes(const vmcpde_norm_args* a) {
   if (check(a)) return -1;
-  const Shape p = shape_of(a->cols, 16 / dtype_size(a->dtype), 2);
+  const Shape p = shape_of(a->cols, 16 / dtype_size(a->dtype), 2, a->dtype == VMCPDE_F32 ? 4 : 2);
   return backward_groups(p, a->rows) * 2 * a->cols * (a->dtype == VMCPDE_F64 ? 8 : 4);
 }
 

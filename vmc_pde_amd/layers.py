@@ -148,8 +148,8 @@ def dense(x, kernel, bias=None, *, activation="none", scale=1.0, residual=None, 
     if residual is not None:
         _same_shape(residual, shape, "residual")
         residual, ldr = _rows(residual, n_out, "residual")
-    y = _empty(shape, dtype=dtype, device=device)
-    slope = _empty(shape, dtype=SLOPE[dtype], device=device) if want_slope and act else None
+    y = x.new_empty(shape)
+    slope = _empty(shape, dtype=SLOPE[dtype], device=index) if want_slope and act else None
     record = _pack_dense(DTYPE[dtype], act, kernel_t, 0, x.numel() // n_in, n_in, n_out, x.data_ptr(), ldx, kernel.data_ptr(), ldk,
                          0 if bias is None else bias.data_ptr(), 0 if residual is None else residual.data_ptr(), ldr, float(scale), y.data_ptr(), n_out,
                          0 if slope is None else slope.data_ptr(), 0, 0, 0, 0, 0)
@@ -180,9 +180,9 @@ def dense_backward(dy, x, kernel, slope=None, *, scale=1.0, want_x=True, want_ke
         _agrees(slope, "slope", SLOPE[dtype], index)
         _same_shape(slope, shape, "slope")
         slope = slope.contiguous()
-    dx = _empty(x_shape, dtype=dtype, device=device) if want_x else None
-    dkernel = _empty((n_in, n_out), dtype=dtype, device=device) if want_kernel else None
-    dbias = _empty(n_out, dtype=dtype, device=device) if want_bias else None
+    dx = x.new_empty(x_shape) if want_x else None
+    dkernel = x.new_empty((n_in, n_out)) if want_kernel else None
+    dbias = x.new_empty(n_out) if want_bias else None
     record = _pack_dense(DTYPE[dtype], 0, kernel_t, 0, x.numel() // n_in, n_in, n_out, x.data_ptr(), ldx, kernel.data_ptr(), ldk, 0, 0, 0, float(scale), 0, 0,
                          0 if slope is None else slope.data_ptr(), dy.data_ptr(), ldd, 0 if dx is None else dx.data_ptr(),
                          0 if dkernel is None else dkernel.data_ptr(), 0 if dbias is None else dbias.data_ptr())
@@ -233,10 +233,10 @@ def layer_norm(x, weight=None, bias=None, *, eps=1e-6, want_stats=False):
             return layer_norm(x, weight, bias, eps=eps, want_stats=want_stats)
     shape, device = x.shape, x.device
     x, ldx = _rows(x, cols, "x")
-    y = _empty(shape, dtype=dtype, device=device)
+    y = x.new_empty(shape)
     mean = rstd = None
     if want_stats:
-        mean, rstd = _empty(shape[:-1], dtype=WIDE[dtype], device=device), _empty(shape[:-1], dtype=WIDE[dtype], device=device)
+        mean, rstd = _empty((2, *shape[:-1]), dtype=WIDE[dtype], device=index).unbind(0)
     _call("vmcpde_layer_norm", _pack_norm(DTYPE[dtype], DTYPE[weights or dtype], x.numel() // cols, cols, x.data_ptr(), ldx, 0 if weight is None else weight.data_ptr(),
                                           0 if bias is None else bias.data_ptr(), float(eps), y.data_ptr(), cols, 0 if mean is None else mean.data_ptr(),
                                           0 if rstd is None else rstd.data_ptr(), 0, 0, 0, 0, 0), _stream(index))
@@ -270,9 +270,12 @@ def layer_norm_backward(dy, x, mean, rstd, weight=None, *, want_x=True, want_wei
     x, ldx = _rows(x, cols, "x")
     dy, ldd = _rows(dy, cols, "dy")
     mean, rstd = mean.contiguous(), rstd.contiguous()
-    dx = _empty(shape, dtype=dtype, device=device) if want_x else None
-    dweight = _empty(cols, dtype=weights, device=device) if want_weight else None
-    dbias = _empty(cols, dtype=weights, device=device) if want_bias else None
+    dx = x.new_empty(shape) if want_x else None
+    if want_weight and want_bias:
+        dweight, dbias = _empty((2, cols), dtype=weights, device=index).unbind(0)
+    else:
+        dweight = _empty(cols, dtype=weights, device=index) if want_weight else None
+        dbias = _empty(cols, dtype=weights, device=index) if want_bias else None
     record = _pack_norm(DTYPE[dtype], DTYPE[weights], x.numel() // cols, cols, x.data_ptr(), ldx, 0 if weight is None else weight.data_ptr(), 0, 0.0, 0, 0,
                         mean.data_ptr(), rstd.data_ptr(), dy.data_ptr(), ldd, 0 if dx is None else dx.data_ptr(), 0 if dweight is None else dweight.data_ptr(),
                         0 if dbias is None else dbias.data_ptr())
