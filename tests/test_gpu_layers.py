@@ -386,6 +386,38 @@ def test_global_norm_of_trees_and_layouts(layers):
             layers.clip_by_global_norm(tensors, 1.0)
 
 
+def test_both_readers_of_a_list_of_tensors(layers, monkeypatch):
+    """The native reader and the Python code that it spares the host from: the same table, the same results, the same refusals."""
+    from vmc_pde_amd import _native as nat
+    assert nat.tensor_reader() is not None
+    tensors = parts([7, 0, 300, 41, 1], DTYPES, 3)
+    out = [torch.empty_like(t) for t in tensors]
+    nested = [tensors[0], [tensors[1], (tensors[2],)], {"a": tensors[3], "b": tensors[4]}]
+    first = layers.clip_by_global_norm(tensors, 0.1, out=out)
+    kept = [o.clone() for o in out]
+    assert torch.equal(layers.global_norm(nested), first) and torch.equal(layers.clip_by_global_norm(tuple(tensors), 0.1, out=tuple(out)), first)
+    bad = [(tensors, out[:-1]), (tensors, out[::-1]), ([tensors[0]], [out[0][:-1]]), ([tensors[0]], [out[0].cpu()]), ([tensors[0].cpu()], None)]
+    parameter = torch.nn.Parameter(tensors[2].clone())
+    for native in (True, False):
+        if not native:
+            monkeypatch.setattr(nat, "_tensors", (None,))
+        again = layers.clip_by_global_norm(tensors, 0.1, out=out)
+        assert torch.equal(again, first) and all(torch.equal(a, b) for a, b in zip(out, kept))
+        for t, o in bad:
+            with pytest.raises(ValueError):
+                layers.clip_by_global_norm(t, 0.1, out=o)
+        with pytest.raises(TypeError):
+            layers.global_norm([tensors[0], tensors[0].int()])
+        with pytest.raises(ValueError, match="no_grad"):
+            layers.clip_by_global_norm([parameter], 0.1)
+        assert float(layers.global_norm([parameter])) > 0
+        with torch.no_grad():
+            layers.clip_by_global_norm([parameter], 0.1)
+        for empty in ([], [[]], {}):
+            with pytest.raises(ValueError, match="no tensors"):
+                layers.global_norm(empty)
+
+
 def test_global_norm_of_extreme_numbers(layers):
     def norm(*v, dtype=torch.float64):
         return float(layers.global_norm(torch.tensor(v, dtype=dtype, device="cuda")))

@@ -176,6 +176,22 @@ def lib():
     return _lib
 
 
+_tensors = None
+
+
+def tensor_reader():
+    """`vmcpde_read_tensors` of csrc/tensor_list.cpp, or None where that library is not built: it only saves the host's time."""
+    global _tensors
+    if _tensors is None:
+        path = LIB_PATH.parent / "libvmcpde_tensors.so"
+        _tensors = (None,)
+        if path.exists():
+            f = C.PyDLL(str(path)).vmcpde_read_tensors
+            f.restype, f.argtypes = _int, [C.py_object, C.py_object, _int, _vp, _i64, _vp]
+            _tensors = (f,)
+    return _tensors[0]
+
+
 def check(rc: int, what: str = ""):
     if rc != 0:
         msg = lib().vmcpde_last_error().decode(errors="replace")

@@ -911,8 +911,7 @@ struct Dense {
     else if (a.n_out <= 16) thin_backward<2, 1>(a, (unsigned)groups, partial);
     else thin_backward<2, 2>(a, (unsigned)groups, partial);
     if (partial)
-      add_columns_kernel<T, T><<<(unsigned)ceil_div(sums, 64), 1024, 0, stream>>>(partial, (int)groups, sums, a.n_in * a.n_out, a.n_out, static_cast<T*>(a.dkernel),
-                                                                                 static_cast<T*>(a.dbias));
+      add_columns<T, T>(partial, groups, sums, a.n_in * a.n_out, a.n_out, static_cast<T*>(a.dkernel), static_cast<T*>(a.dbias), stream);
   }
 
   void forward(const vmcpde_dense_args& a) {
@@ -951,7 +950,7 @@ struct Dense {
       if (launch) {
         scaled_copy<T>(dy, static_cast<const S*>(a.slope), a.scale, to, dz.ld, partial, groups, stream);
         if (a.dbias)
-          add_columns_kernel<A, T><<<(unsigned)ceil_div(a.n_out, 64), 1024, 0, stream>>>(partial, (int)groups, a.n_out, a.n_out, 0, static_cast<T*>(a.dbias), nullptr);
+          add_columns<A, T>(partial, groups, a.n_out, a.n_out, 0, static_cast<T*>(a.dbias), nullptr, stream);
       }
     }
     if (a.dx && a.rows) {

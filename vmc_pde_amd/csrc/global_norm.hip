@@ -272,19 +272,20 @@ int check_overlap(const vmcpde_tensor* t, int32_t count) {
   return 0;
 }
 
-// fills tables of at most TABLE non-empty tensors and hands each to `launch(table, groups before it)`
+// Fills tables of at most TABLE non-empty tensors and hands each to `launch(table, groups before it)`.
 template <typename F>
 int for_tables(const vmcpde_tensor* t, int32_t count, const Plan& p, F launch) {
   Table tab;
   tab.chunk = p.chunk;
   int64_t before = 0;
-  for (int32_t k = 0; k < count;) {
+  for (int32_t j = 0; j < count;) {
     tab.count = 0;
     int64_t groups = 0;
-    for (; k < count && tab.count < TABLE; ++k) {
-      if (t[k].n == 0) continue;
-      tab.e[tab.count++] = {t[k].in, t[k].out, t[k].n, t[k].dtype, (int32_t)groups};
-      groups += ceil_div(t[k].n, p.chunk);
+    for (; j < count && tab.count < TABLE; ++j) {
+      const vmcpde_tensor& e = t[j];
+      if (e.n == 0) continue;
+      tab.e[tab.count++] = {e.in, e.out, e.n, e.dtype, (int32_t)groups};
+      groups += ceil_div(e.n, p.chunk);
     }
     tab.groups = (int32_t)groups;
     if (tab.count) {

@@ -469,8 +469,7 @@ struct Norm {
             partial);
     }
     if (partial)
-      add_columns_kernel<A, W><<<(unsigned)ceil_div(2 * a.cols, 64), 1024, 0, s>>>(partial, (int)groups, 2 * a.cols, a.cols, a.cols, static_cast<W*>(a.dweight),
-                                                                                   static_cast<W*>(a.dbias));
+      add_columns<A, W>(partial, groups, 2 * a.cols, a.cols, a.cols, static_cast<W*>(a.dweight), static_cast<W*>(a.dbias), s);
   }
 };
 

@@ -74,28 +74,37 @@ __device__ __forceinline__ void store_vec(T* __restrict__ row, int64_t col, int6
 }
 
 // Last step of a sum over rows: columns col < cols0 of sum_g partial[g * pitch + col] go to out0, the cols1 behind them to out1 (a null one is skipped).
-// 64 columns x 16 parts of the groups a workgroup; a part's groups, then the parts, are added in their order.
-template <typename A, typename W>
+// 1024 / PARTS columns x PARTS parts of the groups a workgroup; a part's groups, then the parts, are added in their order.
+template <typename A, typename W, int PARTS>
 static __global__ __launch_bounds__(1024) void add_columns_kernel(const A* __restrict__ partial, int groups, int64_t pitch, int64_t cols0, int64_t cols1,
                                                                   W* __restrict__ out0, W* __restrict__ out1) {
-  __shared__ A sh[16][64];
-  const int part = threadIdx.x >> 6, c = threadIdx.x & 63;
-  const int64_t col = (int64_t)blockIdx.x * 64 + c;
+  constexpr int COLS = 1024 / PARTS;
+  __shared__ A sh[PARTS][COLS];
+  const int part = threadIdx.x / COLS, c = threadIdx.x % COLS;
+  const int64_t col = (int64_t)blockIdx.x * COLS + c;
   A v = 0;
   if (col < cols0 + cols1) {
 #pragma unroll 8
-    for (int g = part; g < groups; g += 16) v += partial[(int64_t)g * pitch + col];
+    for (int g = part; g < groups; g += PARTS) v += partial[(int64_t)g * pitch + col];
   }
   sh[part][c] = v;
   __syncthreads();
   if (part == 0 && col < cols0 + cols1) {
-    for (int p = 1; p < 16; ++p) v += sh[p][c];
+#pragma unroll 8
+    for (int p = 1; p < PARTS; ++p) v += sh[p][c];
     if (col < cols0) {
       if (out0) out0[col] = (W)v;
     } else if (out1) {
       out1[col - cols0] = (W)v;
     }
   }
+}
+// few columns: more lanes along the groups (42 columns of 1024 groups: one workgroup of 64 x 16 took 9 us)
+template <typename A, typename W>
+void add_columns(const A* partial, int64_t groups, int64_t pitch, int64_t cols0, int64_t cols1, W* out0, W* out1, hipStream_t s) {
+  const int64_t cols = cols0 + cols1;
+  if (cols <= 1024) add_columns_kernel<A, W, 64><<<(unsigned)ceil_div(cols, 16), 1024, 0, s>>>(partial, (int)groups, pitch, cols0, cols1, out0, out1);
+  else add_columns_kernel<A, W, 16><<<(unsigned)ceil_div(cols, 64), 1024, 0, s>>>(partial, (int)groups, pitch, cols0, cols1, out0, out1);
 }
 
 }  // namespace vmcpde

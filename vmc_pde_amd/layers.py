@@ -9,14 +9,14 @@ All run on the current HIP stream, allocate through torch, never synchronise wit
 and epilogues are held in fp32 for fp32 and 16-bit elements, in fp64 for fp64.  None uses atomics: the same call gives the same bits.
 
 Small calls are bound by the host: arguments travel as one packed record per call (`vmcpde_dense_args`, `vmcpde_norm_args` of include/vmcpde.h)
-and every tensor attribute is read once.
+every tensor attribute is read once, and lists of tensors are read by csrc/tensor_list.cpp.
 """
 from __future__ import annotations
 
 import ctypes as C
 import struct
+from array import array
 
-import numpy as np
 import torch
 
 from . import _native as nat
@@ -315,44 +315,54 @@ def _codes(leaves):
         raise TypeError(f"element type {unknown.args[0]}: fp64, fp32, fp16 and bf16 are supported") from None
 
 
-def _global_norm(tensors, max_norm, out):
-    leaves = _leaves(tensors, [])
-    if not leaves:
-        raise ValueError("no tensors")
+def _table(leaves, targets, clip):
+    """(rows of vmcpde_tensor, device index); refuses what cannot be reduced or written."""
     index, codes = leaves[0].get_device(), _codes(leaves)
     if index < 0:
         raise ValueError(_HOST)
     if any([t.get_device() != index for t in leaves]):
         raise ValueError(f"tensors on several devices: {sorted({str(t.device) for t in leaves})}")
-    if _device() != index:
-        with torch.cuda.device(index):
-            return _global_norm(tensors, max_norm, out)
     plain = all([t.is_contiguous() for t in leaves])
     if not plain:
         for t in leaves:
             if t.numel() and not t.is_contiguous() and not _fills_memory(t):
                 raise ValueError(f"a tensor of shape {tuple(t.shape)} and strides {t.stride()} does not fill its memory: pass a contiguous one")
-    places = [t.data_ptr() for t in leaves]
-    targets = leaves
-    if out is None:
-        to = places
-    else:
-        targets = _leaves(out, [])
+    places = to = [t.data_ptr() for t in leaves]
+    if targets is not None:
         if len(targets) != len(leaves):
             raise ValueError(f"{len(leaves)} tensors and {len(targets)} to write them to")
         if [t.shape for t in targets] != [t.shape for t in leaves] or _codes(targets) != codes or any([t.get_device() != index for t in targets]) \
                 or not (plain and all([t.is_contiguous() for t in targets])) and [t.stride() for t in targets] != [t.stride() for t in leaves]:
             raise ValueError("out: shapes, strides, element types and devices have to be those of the tensors")
         to = [t.data_ptr() for t in targets]
-    if max_norm is not None and _recording() and any([t.requires_grad for t in targets]):
+    if clip and _recording() and any([t.requires_grad for t in targets or leaves]):
         raise ValueError("clipping writes into tensors that automatic differentiation records: call it under torch.no_grad()")
+    return array("q", [v for row in zip(places, to, [t.numel() for t in leaves], codes) for v in row]), index
+
+
+def _global_norm(tensors, max_norm, out):
+    clip = max_norm is not None
+    leaves = tensors if type(tensors) is list else _leaves(tensors, [])
+    if not leaves:
+        raise ValueError("no tensors")
+    targets = out if out is None or type(out) is list else _leaves(out, [])
     count = len(leaves)
-    table = np.array((places, to, [t.numel() for t in leaves], codes), dtype=np.int64).T.copy()        # vmcpde_tensor: in, out, n, dtype
-    address, device = table.ctypes.data, leaves[0].device
-    norm = _empty((), dtype=torch.float64, device=device)
-    ws, nbytes = _workspace("vmcpde_global_norm_workspace_bytes", device, address, count)
-    _call("vmcpde_global_norm", address, count, 0 if max_norm is None else 1, 0.0 if max_norm is None else max_norm, norm.data_ptr(),
-          None if ws is None else ws.data_ptr(), nbytes, _stream(index))
+    read, table, place = nat.tensor_reader(), array("q", bytes(32 * count)), array("q", (0,))
+    if read is not None and read(leaves, targets, clip and _recording(), table.buffer_info()[0], count, place.buffer_info()[0]):
+        index = place[0]
+    else:
+        leaves = _leaves(leaves, [])
+        if not leaves:
+            raise ValueError("no tensors")
+        table, index = _table(leaves, None if targets is None else _leaves(targets, []), clip)
+        count = len(leaves)
+    if _device() != index:
+        with torch.cuda.device(index):
+            return _global_norm(tensors, max_norm, out)
+    address = table.buffer_info()[0]
+    norm = _empty((), dtype=torch.float64, device=index)
+    ws, nbytes = _workspace("vmcpde_global_norm_workspace_bytes", index, address, count)
+    _call("vmcpde_global_norm", address, count, clip, max_norm if clip else 0.0, norm.data_ptr(), None if ws is None else ws.data_ptr(), nbytes, _stream(index))
     return norm
 
 
