@@ -1,5 +1,6 @@
 // The dense layer  y = scale * act(x W + b) + r  and its gradients (dz = scale * slope * dy: dx = dz W^T, dW = x^T dz, db = sum_rows dz).
 #include <algorithm>
+#include <cmath>
 
 #include "layers.hpp"
 
@@ -742,36 +743,54 @@ __global__ __launch_bounds__(THIN_THREADS) void thin_backward_kernel(const T* __
 
 // ---- plans ---------------------------------------------------------------------------------------------------------------------------
 
-struct Tiles { int bm, bn, slices, k_slice; };
+struct Tiles { int bm, bn, slices, slice_steps; };
 
-// Tile and k slices of a product.  Sides of at most 32 rows or columns take 32, so that little is multiplied for nothing.  16-bit operands take
-// 256 x 256, which reads each operand half as often, where such tiles fill the card, else 128 x 128; fp32 and fp64 take 128 x 64, of which a CU holds
-// three.  Products of too few tiles take 64 x 64, and where those leave CUs idle too the k range is cut, and the slices' sums are joined by a second launch.
+// What a step of k costs a CU in microseconds, by type and square tile: alone (its fetches and barrier), and each of several workgroups that share the CU
+// (the matrix pipe).  Measured on products of 512 to 10 000 rows; `held`: workgroups a CU holds.
+struct Cost { int side, held; double alone, each; };
+constexpr Cost HALF_COSTS[] = {{64, 4, 0.5, 0.2}, {128, 2, 0.75, 0.48}, {256, 1, 1.6, 1.7}};
+constexpr Cost F32_COST = {64, 4, 0.65, 0.5}, F64_COST = {64, 4, 0.7, 0.55};
+
+// Tile and k slices of a product of `steps` steps of k.  Sides of at most 32 rows or columns take 32, so that little is multiplied for nothing: those read
+// one long operand once, and the k range is cut until two workgroups a CU do.  Everything else takes the tile and the number of slices of the least
+// estimated time: the steps of the fullest CU, and with slices a second launch that reads and joins their sums (3 us and their bytes at 4 TB/s).  The
+// estimate finds the best choice, or one within 15 % of it, for the 27 shapes that it was made from (three types, 0.1 to 140 GFLOP).
 template <typename T>
-Tiles tiles_of(int64_t m, int64_t n, int64_t k) {
-  constexpr int64_t step = step_of<T>();
-  constexpr bool half = sizeof(T) == 2;
-  Tiles t;
-  t.bm = m <= 32 ? 32 : 128;
-  t.bn = n <= 32 ? 32 : half || t.bm == 32 ? 128 : 64;
-  int64_t tiles = ceil_div(m, t.bm) * ceil_div(n, t.bn), fill = 512;
-  if (half && ceil_div(m, 256) * ceil_div(n, 256) >= 192) t.bm = t.bn = 256;
-  else if (t.bm == 128 && t.bn == 128 && tiles < 256) t.bm = t.bn = 64;
-  else if (t.bm == 128 && t.bn == 64 && tiles < 128) t.bm = 64;
-  else if (!half && t.bn == 64) fill = 768;
-  tiles = ceil_div(m, t.bm) * ceil_div(n, t.bn);
+Tiles tiles_of(int64_t m, int64_t n, int64_t steps) {
+  Tiles best = {m <= 32 ? 32 : 128, n <= 32 ? 32 : 128, 1, 0};
   int64_t slices = 1;
-  if (tiles > 0 && tiles < 256) slices = std::min<int64_t>(std::min<int64_t>(ceil_div(fill, tiles), ceil_div(k, 4 * step)), 256);
-  if (slices < 1) slices = 1;
-  t.k_slice = (int)round_up(ceil_div(k, slices), step);
-  if (t.k_slice < step) t.k_slice = (int)step;
-  t.slices = (int)std::max<int64_t>(1, ceil_div(k, t.k_slice));
-  return t;
+  if (best.bm == 32 || best.bn == 32) {
+    const int64_t tiles = ceil_div(m, best.bm) * ceil_div(n, best.bn);
+    if (tiles > 0 && tiles < 256) slices = std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(ceil_div(512, tiles), ceil_div(steps, 4)), 256));
+  } else {
+    double least = INFINITY;
+    auto consider = [&](const Cost& c) {
+      const int64_t tiles = ceil_div(m, c.side) * ceil_div(n, c.side);
+      for (const int s : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64, 96, 128, 192, 256}) {
+        if (s > 1 && (steps < 2 * s || tiles * s > 2048)) break;
+        const double on_one = (double)ceil_div(tiles * s, 256);
+        const double time = (double)ceil_div(steps, s) * std::max(c.alone * std::ceil(on_one / c.held), on_one * c.each) +
+                            (s > 1 ? 3 + (double)s * m * n * 2 * sizeof(typename Wide<T>::type) / 4e6 : 0);
+        if (time < least) {
+          least = time;
+          best.bm = best.bn = c.side;
+          slices = s;
+        }
+      }
+    };
+    if constexpr (sizeof(T) == 2)
+      for (const Cost& c : HALF_COSTS) consider(c);
+    else
+      consider(sizeof(T) == 4 ? F32_COST : F64_COST);
+  }
+  best.slice_steps = (int)std::max<int64_t>(1, ceil_div(steps, slices));
+  best.slices = (int)std::max<int64_t>(1, ceil_div(steps, best.slice_steps));
+  return best;
 }
 
 template <typename T>
 int64_t product_bytes(int64_t m, int64_t n, int64_t k) {
-  const Tiles t = tiles_of<T>(m, n, k);
+  const Tiles t = tiles_of<T>(m, n, ceil_div(k, step_of<T>()));
   return t.slices > 1 ? round_up((int64_t)t.slices * m * n * (int64_t)sizeof(typename Wide<T>::type), 256) : 0;
 }
 
@@ -779,21 +798,19 @@ template <typename T, int BM, int BN, int WM, int WN>
 void product_as(const Product& g, bool p_across, bool q_across, const Tiles& t, typename Wide<T>::type* part, const Epilogue<T>& e, hipStream_t s) {
   const int tiles_m = (int)ceil_div(g.m, BM), tiles_n = (int)ceil_div(g.n, BN);
   const dim3 grid((unsigned)(tiles_m * tiles_n), (unsigned)t.slices);
-  if (p_across) product_kernel<T, BM, BN, WM, WN, true, true><<<grid, 64 * WM * WN, 0, s>>>(g, tiles_m, tiles_n, t.k_slice, part, e);      // (P across: x^T dz, Q too)
-  else if (q_across) product_kernel<T, BM, BN, WM, WN, false, true><<<grid, 64 * WM * WN, 0, s>>>(g, tiles_m, tiles_n, t.k_slice, part, e);
-  else product_kernel<T, BM, BN, WM, WN, false, false><<<grid, 64 * WM * WN, 0, s>>>(g, tiles_m, tiles_n, t.k_slice, part, e);
+  if (p_across) product_kernel<T, BM, BN, WM, WN, true, true><<<grid, 64 * WM * WN, 0, s>>>(g, tiles_m, tiles_n, t.slice_steps * step_of<T>(), part, e);      // (P across: x^T dz, Q too)
+  else if (q_across) product_kernel<T, BM, BN, WM, WN, false, true><<<grid, 64 * WM * WN, 0, s>>>(g, tiles_m, tiles_n, t.slice_steps * step_of<T>(), part, e);
+  else product_kernel<T, BM, BN, WM, WN, false, false><<<grid, 64 * WM * WN, 0, s>>>(g, tiles_m, tiles_n, t.slice_steps * step_of<T>(), part, e);
 }
 
 template <typename T>
 void product(const Product& g, bool p_across, bool q_across, const Epilogue<T>& e, void* workspace, hipStream_t s) {
   typedef typename Wide<T>::type A;
-  const Tiles t = tiles_of<T>(g.m, g.n, g.k);
+  const Tiles t = tiles_of<T>(g.m, g.n, ceil_div(g.k, step_of<T>()));
   A* part = t.slices > 1 ? static_cast<A*>(workspace) : nullptr;
   if constexpr (sizeof(T) == 2) {
     if (t.bm == 256) product_as<T, 256, 256, 2, 4>(g, p_across, q_across, t, part, e, s);
     if (t.bm == 128 && t.bn == 128) product_as<T, 128, 128, 2, 2>(g, p_across, q_across, t, part, e, s);
-  } else {
-    if (t.bm == 128 && t.bn == 64) product_as<T, 128, 64, 2, 2>(g, p_across, q_across, t, part, e, s);
   }
   if (t.bm == 64) product_as<T, 64, 64, 2, 2>(g, p_across, q_across, t, part, e, s);
   else if (t.bm == 128 && t.bn == 32) product_as<T, 128, 32, 4, 1>(g, p_across, q_across, t, part, e, s);
