@@ -470,44 +470,63 @@ __global__ __launch_bounds__(256) void product_join_kernel(const typename Wide<T
   if (row < m) finish<T, 4>(e, row, col, z);
 }
 
-// ---- the gradient before the activation ----------------------------------------------------------------------------------------------
+// ---- what is made ready before the products --------------------------------------------------------------------------------------------
 
-// dz = scale * slope * dy (dz may be null; its row pitch may exceed n: zeros there), and sums of its columns over the rows that this
-// workgroup takes: partial[blockIdx.y][n] (may be null).  LANES lanes along the columns, 256 / LANES rows at a time.
-template <typename T, int LANES>
-__global__ __launch_bounds__(256) void dense_dz_kernel(const T* __restrict__ dy, int64_t ldd, const typename Slope<T>::type* __restrict__ slope,
-                                                       typename Wide<T>::type scale, int64_t rows, int64_t n, T* __restrict__ dz, int64_t ldz,
-                                                       typename Wide<T>::type* __restrict__ partial) {
+// Up to three copies in one launch: lines of n elements to lines of ld_to (zeros behind n), scaled by scale * slope: an operand into lines that the
+// products can fetch, or dz = scale * slope * dy; `to` may be null.  With `partial` also sums of dz's columns over the lines that a workgroup takes:
+// partial[group][n].  `lanes` (a power of two) lie along the columns, 256 / lanes lines are taken at a time.
+template <typename T>
+struct Job {
+  const T* from;
+  int64_t ld, lines, n;
+  const typename Slope<T>::type* slope;
+  typename Wide<T>::type scale;
+  T* to;
+  int64_t ld_to;
+  typename Wide<T>::type* partial;
+  int32_t lanes_log2, col_blocks, groups, first;       // first: the job's first workgroup in the launch
+};
+template <typename T>
+struct Jobs {
+  Job<T> job[3];
+  int32_t count, blocks;
+};
+
+template <typename T>
+__global__ __launch_bounds__(256) void prepare_kernel(Jobs<T> jobs) {
   typedef typename Wide<T>::type A;
-  constexpr int V = vec_of<T>(), ROWS = 256 / LANES;
-  __shared__ A sh[ROWS][LANES * V];
-  const int lane = threadIdx.x % LANES, part = threadIdx.x / LANES;
-  const int64_t col = ((int64_t)blockIdx.x * LANES + lane) * V;
+  constexpr int V = vec_of<T>();
+  __shared__ A sh[256 * V];
+  int which = 0;
+  while (which + 1 < jobs.count && (int)blockIdx.x >= jobs.job[which + 1].first) ++which;
+  const Job<T>& b = jobs.job[which];
+  const int block = blockIdx.x - b.first, group = block / b.col_blocks, lanes = 1 << b.lanes_log2, at_once = 256 >> b.lanes_log2;
+  const int lane = threadIdx.x & (lanes - 1), part = threadIdx.x >> b.lanes_log2;
+  const int64_t col0 = (int64_t)(block - group * b.col_blocks) * lanes * V, col = col0 + lane * V;
   A sum[V];
 #pragma unroll
   for (int k = 0; k < V; ++k) sum[k] = 0;
-  for (int64_t r = (int64_t)blockIdx.y * ROWS + part; r < rows; r += (int64_t)gridDim.y * ROWS) {
+  for (int64_t r = (int64_t)group * at_once + part; r < b.lines; r += (int64_t)b.groups * at_once) {
     A v[V], s[V];
-    load_vec<T, V>(dy + r * ldd, col, n, v);
-    if (slope) load_vec<typename Slope<T>::type, V>(slope + r * n, col, n, s);
+    load_vec<T, V>(b.from + r * b.ld, col, b.n, v);
+    if (b.slope) load_vec<typename Slope<T>::type, V>(b.slope + r * b.n, col, b.n, s);
 #pragma unroll
     for (int k = 0; k < V; ++k) {
-      v[k] *= scale;
-      if (slope) v[k] *= s[k];
-      if (col + k >= n) v[k] = 0;
+      v[k] *= b.scale;
+      if (b.slope) v[k] *= s[k];
+      if (col + k >= b.n) v[k] = 0;
       sum[k] += v[k];
     }
-    if (dz) store_vec<T, V>(dz + r * ldz, col, ldz, v);
+    if (b.to) store_vec<T, V>(b.to + r * b.ld_to, col, b.ld_to, v);
   }
-  if (!partial) return;
+  if (!b.partial) return;
 #pragma unroll
-  for (int k = 0; k < V; ++k) sh[part][lane * V + k] = sum[k];
+  for (int k = 0; k < V; ++k) sh[(part * lanes + lane) * V + k] = sum[k];
   __syncthreads();
-  for (int c = threadIdx.x; c < LANES * V; c += 256) {
+  for (int c = threadIdx.x; c < lanes * V; c += 256) {
     A v = 0;
-    for (int p = 0; p < ROWS; ++p) v += sh[p][c];
-    const int64_t to = (int64_t)blockIdx.x * LANES * V + c;
-    if (to < n) partial[blockIdx.y * n + to] = v;
+    for (int p = 0; p < at_once; ++p) v += sh[p * lanes * V + c];
+    if (col0 + c < b.n) b.partial[(int64_t)group * b.n + col0 + c] = v;
   }
 }
 
@@ -822,12 +841,6 @@ void product(const Product& g, bool p_across, bool q_across, const Epilogue<T>& 
   else product_join_kernel<T, 1><<<(unsigned)ceil_div(lanes, 256), 256, 0, s>>>(part, t.slices, g.m, g.n, e);
 }
 
-// workgroups along the rows of the dz kernel
-int64_t dz_groups(int64_t rows, int64_t cols_blocks, int rows_at_once) {
-  const int64_t want = std::max<int64_t>(1, 2048 / cols_blocks), have = std::max<int64_t>(1, ceil_div(rows, rows_at_once));
-  return std::min<int64_t>(std::min<int64_t>(want, have), 512);
-}
-
 // A matrix operand in memory: `lines` of `n` elements behind each other, `ld` apart.
 struct Lines {
   const void* p;
@@ -842,24 +855,6 @@ bool fetchable(const Lines& o, bool along_k) {
 }
 
 template <typename T>
-void scaled_copy(const Lines& from, const typename Slope<T>::type* slope, double scale, T* to, int64_t ld_to, typename Wide<T>::type* partial, int64_t groups, hipStream_t s) {
-  typedef typename Wide<T>::type A;
-  const int64_t width = to ? ld_to : from.n;
-  if (from.n <= 8 * vec_of<T>())
-    dense_dz_kernel<T, 8><<<dim3((unsigned)ceil_div(width, 8 * vec_of<T>()), (unsigned)groups), 256, 0, s>>>(static_cast<const T*>(from.p), from.ld, slope, (A)scale, from.lines,
-                                                                                                          from.n, to, ld_to, partial);
-  else
-    dense_dz_kernel<T, 32><<<dim3((unsigned)ceil_div(width, 32 * vec_of<T>()), (unsigned)groups), 256, 0, s>>>(static_cast<const T*>(from.p), from.ld, slope, (A)scale,
-                                                                                                            from.lines, from.n, to, ld_to, partial);
-}
-
-template <typename T>
-int64_t copy_groups(const Lines& o) {
-  const int lanes = o.n <= 8 * vec_of<T>() ? 8 : 32;
-  return dz_groups(o.lines, ceil_div(o.n, lanes * vec_of<T>()), 256 / lanes);
-}
-
-template <typename T>
 struct Dense {
   typedef typename Wide<T>::type A;
   typedef typename Slope<T>::type S;
@@ -869,7 +864,8 @@ struct Dense {
   hipStream_t stream;
   int64_t used = 0, most = 0;
   bool launch;
-  Dense(void* w, hipStream_t s, bool l) : workspace(static_cast<char*>(w)), stream(s), launch(l) {}
+  Jobs<T> jobs;
+  Dense(void* w, hipStream_t s, bool l) : workspace(static_cast<char*>(w)), stream(s), launch(l) { jobs.count = jobs.blocks = 0; }
 
   void* take(int64_t bytes) {
     void* p = workspace ? workspace + used : nullptr;
@@ -878,18 +874,41 @@ struct Dense {
     return p;
   }
 
-  // an operand that the products can fetch; `k_held` is what it holds along k where its lines lie along it
+  // A job of the launch before the products; its groups are also the rows of `partial`.
+  Job<T> job_of(const Lines& o) {
+    Job<T> b = {static_cast<const T*>(o.p), o.ld, o.lines, o.n, nullptr, 1, nullptr, o.n, nullptr, 5, 1, 1, 0};
+    while (b.lanes_log2 > 2 && (int64_t)vec_of<T>() << (b.lanes_log2 - 1) >= o.n) --b.lanes_log2;
+    return b;
+  }
+  void add(Job<T> b) {
+    Jobs<T>& all = jobs;
+    b.first = all.blocks;
+    all.job[all.count++] = b;
+    all.blocks += b.col_blocks * b.groups;
+  }
+  // workgroups: some 2048 along both axes, at most 512 along the lines
+  static void shape(Job<T>& b, int64_t width) {
+    b.col_blocks = (int)ceil_div(width, (int64_t)vec_of<T>() << b.lanes_log2);
+    b.groups = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(512, std::max(1, 2048 / b.col_blocks)), ceil_div(b.lines, 256 >> b.lanes_log2)));
+  }
+  void launch_jobs() {
+    if (launch && jobs.count) prepare_kernel<T><<<jobs.blocks, 256, 0, stream>>>(jobs);
+    jobs.count = jobs.blocks = 0;
+  }
+
+  // an operand that the products can fetch
   Lines ready(Lines o, bool along_k) {
     if (fetchable<T>(o, along_k)) return o;
     const int64_t ld = round_up(o.n, vec_of<T>());
-    T* to = static_cast<T*>(take(o.lines * ld * (int64_t)sizeof(T)));
-    if (launch && o.lines) scaled_copy<T>(o, nullptr, 1.0, to, ld, nullptr, copy_groups<T>(o), stream);
-    return {to, o.lines, along_k ? ld : o.n, ld};
+    Job<T> b = job_of(o);
+    b.to = static_cast<T*>(take(o.lines * ld * (int64_t)sizeof(T)));
+    b.ld_to = ld;
+    shape(b, ld);
+    if (o.lines) add(b);
+    return {b.to, o.lines, along_k ? ld : o.n, ld};
   }
 
   void multiply(Lines p, bool p_across, Lines q, bool q_across, int64_t m, int64_t n, int64_t k, const Epilogue<T>& e) {
-    p = ready(p, !p_across);
-    q = ready(q, !q_across);
     const int64_t kp = p_across ? p.lines : p.n, kq = q_across ? q.lines : q.n, k_all = std::max(k, std::max(kp, kq));
     const int64_t bytes = product_bytes<T>(m, n, k_all);
     void* rest = bytes ? take(bytes) : nullptr;
@@ -941,7 +960,9 @@ struct Dense {
         return;
       }
     }
-    multiply({a.x, a.rows, a.n_in, a.ldx}, false, kernel_lines(a), !a.kernel_t, a.rows, a.n_out, a.n_in, e);
+    const Lines x = ready({a.x, a.rows, a.n_in, a.ldx}, true), kernel = ready(kernel_lines(a), a.kernel_t);
+    launch_jobs();
+    multiply(x, false, kernel, !a.kernel_t, a.rows, a.n_out, a.n_in, e);
   }
 
   static Lines kernel_lines(const vmcpde_dense_args& a) {
@@ -955,30 +976,32 @@ struct Dense {
     const Lines dy = {a.dy, a.rows, a.n_out, a.ldd};
     Lines dz = dy;
     const bool own = (a.dx || a.dkernel) && (a.slope || a.scale != 1.0 || !fetchable<T>(dy, a.dx));
-    T* to = nullptr;
+    Job<T> b = job_of(dy);
     if (own) {
-      const int64_t ld = round_up(a.n_out, vec_of<T>());
-      to = static_cast<T*>(take(a.rows * ld * (int64_t)sizeof(T)));
-      dz = {to, a.rows, a.n_out, ld};
+      b.ld_to = round_up(a.n_out, vec_of<T>());
+      b.to = static_cast<T*>(take(a.rows * b.ld_to * (int64_t)sizeof(T)));
+      dz = {b.to, a.rows, a.n_out, b.ld_to};
     }
+    shape(b, own ? b.ld_to : a.n_out);
     if (own || a.dbias) {
-      const int64_t groups = copy_groups<T>(dy);
-      A* partial = a.dbias ? static_cast<A*>(take(groups * a.n_out * (int64_t)sizeof(A))) : nullptr;
-      if (launch) {
-        scaled_copy<T>(dy, static_cast<const S*>(a.slope), a.scale, to, dz.ld, partial, groups, stream);
-        if (a.dbias)
-          add_columns<A, T>(partial, groups, a.n_out, a.n_out, 0, static_cast<T*>(a.dbias), nullptr, stream);
-      }
+      b.slope = static_cast<const S*>(a.slope);
+      b.scale = (A)a.scale;
+      if (a.dbias) b.partial = static_cast<A*>(take(b.groups * a.n_out * (int64_t)sizeof(A)));
+      add(b);
     }
-    if (a.dx && a.rows) {
+    const bool want_x = a.dx && a.rows;
+    const Lines kernel = want_x ? ready(kernel_lines(a), !a.kernel_t) : Lines(), x = a.dkernel ? ready({a.x, a.rows, a.n_in, a.ldx}, false) : Lines();
+    launch_jobs();
+    if (launch && a.dbias) add_columns<A, T>(b.partial, b.groups, a.n_out, a.n_out, 0, static_cast<T*>(a.dbias), nullptr, stream);
+    if (want_x) {
       const Epilogue<T> e = {nullptr, nullptr, 0, static_cast<T*>(a.dx), a.n_in, nullptr, a.n_in, 1, VMCPDE_ACT_NONE};
       Lines z = dz;
       if (own) z.n = dz.ld;           // (zeros behind the line's end)
-      multiply(z, false, kernel_lines(a), a.kernel_t, a.rows, a.n_in, a.n_out, e);
+      multiply(z, false, kernel, a.kernel_t, a.rows, a.n_in, a.n_out, e);
     }
     if (a.dkernel) {
       const Epilogue<T> e = {nullptr, nullptr, 0, static_cast<T*>(a.dkernel), a.n_out, nullptr, a.n_out, 1, VMCPDE_ACT_NONE};
-      multiply({a.x, a.rows, a.n_in, a.ldx}, true, dz, true, a.n_in, a.n_out, a.rows, e);
+      multiply(x, true, dz, true, a.n_in, a.n_out, a.rows, e);
     }
   }
 };
