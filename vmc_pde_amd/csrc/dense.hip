@@ -312,7 +312,9 @@ __device__ __forceinline__ void tile_product(const Product& g, int row0, int col
   constexpr int THREADS = 64 * WM * WN, TM = BM / WM / 16, TN = BN / WN / 16, STEP = step_of<T>();
   typedef Tile<T, BM, PX, THREADS> P;
   typedef Tile<T, BN, QX, THREADS> Q;
-  __shared__ __attribute__((aligned(16))) char tiles[2 * (P::BYTES + Q::BYTES)];
+  // buffers: two; four where a step is shorter than a fetch (16-bit small tiles: 10000 x 1024 x 1024 of fp32 lost a tenth to the CU's fewer workgroups)
+  constexpr int STAGES = BM * BN >= 128 * 128 || (sizeof(T) > 2 && BM * BN >= 64 * 64) ? 2 : 4;
+  __shared__ __attribute__((aligned(16))) char tiles[STAGES * (P::BYTES + Q::BYTES)];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const int wr = (wave / WN) * TM * 16, wc = (wave % WN) * TN * 16;
   P p;
@@ -325,7 +327,7 @@ __device__ __forceinline__ void tile_product(const Product& g, int row0, int col
 #pragma unroll
     for (int b = 0; b < TN; ++b) acc[a][b] = {0, 0, 0, 0};
   // A step's k is multiplied in two halves.  While the first half is multiplied the second's fragments are read; then the next step's tiles have arrived
-  // and everyone has read this step's: the buffer is free for the step after next, and while the second half is multiplied the next step's first
+  // and everyone has read this step's: the buffer is free for a later step's, and while the second half is multiplied the next step's first
   // fragments are read.  One barrier a step, and the matrix pipe has work on both sides of it.
   Frag p0[TM], q0[TN], p1[TM], q1[TN];
   auto read = [&](const lds_char* from, int s, Frag (&fp)[TM], Frag (&fq)[TN]) {
@@ -360,24 +362,23 @@ __device__ __forceinline__ void tile_product(const Product& g, int row0, int col
     q.fetch(place + buffer + P::BYTES, k_left);
   };
   if (k_begin < k_end) {
+    constexpr int FETCHES = P::LOADS + Q::LOADS;
     const int steps = (k_end - k_begin + STEP - 1) / STEP;
     int k_left = k_end - k_begin, now = 0;
-    fetch(0, k_left);
-    if (steps > 1) {
-      fetch(BUFFER, k_left - STEP);
-      asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(P::LOADS + Q::LOADS) : "memory");
-    } else {
-      asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
-    }
+    for (int s = 0; s < STAGES && s < steps; ++s) fetch(s * BUFFER, k_left - s * STEP);
+    if (steps >= STAGES) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((STAGES - 1) * FETCHES) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
     read(lds, 0, p0, q0);
     for (int left = steps - 1; left > 0; --left) {
       read(lds + now, 1, p1, q1);
       multiply(p0, q0);
       interleave();
-      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-      if (left > 1) fetch(now, k_left - 2 * STEP);
+      // the next step's tiles (behind them at most STAGES - 2 more have been asked for), and everyone's reads of this step's
+      if (left >= STAGES - 1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((STAGES - 2) * FETCHES) : "memory");
+      else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      if (left >= STAGES) fetch(now, k_left - STAGES * STEP);
       k_left -= STEP;
-      now ^= BUFFER;
+      now = now + BUFFER == STAGES * BUFFER ? 0 : now + BUFFER;
       read(lds + now, 0, p0, q0);
       multiply(p1, q1);
       interleave();
@@ -389,7 +390,7 @@ __device__ __forceinline__ void tile_product(const Product& g, int row0, int col
   // Sixteen rows at a time through a piece of LDS of the wave's own, so that a lane ends with N columns of a row and a row's lanes write whole lines.
   // The loop stays rolled (the epilogue is long); the registers are picked by number inside it.
   constexpr int N = sizeof(T) == 8 ? 2 : sizeof(T) == 4 || TN == 1 ? 4 : 8, COLS = TN * 16, PITCH = COLS + 4;
-  static_assert(WM * WN * 16 * PITCH * (int)sizeof(A) <= 2 * (P::BYTES + Q::BYTES), "the rows fit the tiles' LDS");
+  static_assert(WM * WN * 16 * PITCH * (int)sizeof(A) <= STAGES * (P::BYTES + Q::BYTES), "the rows fit the tiles' LDS");
   __syncthreads();
   A* rows = reinterpret_cast<A*>(tiles) + wave * 16 * PITCH;
   const int i = lane & 15, group = lane >> 4;
