@@ -10,14 +10,13 @@ namespace {
 
 // ---- the epilogue ------------------------------------------------------------------------------------------------------------------
 
-// tanh(z) and 1 - tanh(z)^2, to a few units in the last place (of the smallest numbers too): with e^(-2|z|) - 1 = m, tanh|z| = -m / (2 + m) and the slope
-// is 4 (1 + m) / (2 + m)^2.  m from a range reduction by ln 2 and the Taylor series of e^r - 1 on |r| <= ln 2 / 2 (degree 13: remainder 4e-18 r, fp32
-// degree 7: 1e-9 r).  A quarter of the library function's instructions, and no branches.
-__device__ __forceinline__ void tanh_slope(double z, double& a, double& slope) {
-  const double x = fabs(z) > 25.0 ? 25.0 : fabs(z), y = -2.0 * x, n = rint(y * 1.4426950408889634074);      // (NaN stays)
-  double r = fma(n, -6.93147180369123816490e-01, y);
+// e^-x - 1 = 2^n p + 2^n - 1 for x >= 0: range reduction by ln 2 and the Taylor series of e^r - 1 on |r| <= ln 2 / 2 (degree 13: remainder 4e-18 r, fp32
+// degree 7: 1e-9 r), which leaves the small results their last places.  A quarter of the instructions of the library's functions, and no branches.
+__device__ __forceinline__ double exp_minus_one(double x, double& two_n, double& p) {
+  const double n = rint(x * -1.4426950408889634074);
+  double r = fma(n, -6.93147180369123816490e-01, -x);
   r = fma(n, -1.90821492927058770002e-10, r);
-  double p = 1.0 / 6227020800.0;
+  p = 1.0 / 6227020800.0;
   p = fma(p, r, 1.0 / 479001600.0);
   p = fma(p, r, 1.0 / 39916800.0);
   p = fma(p, r, 1.0 / 3628800.0);
@@ -30,40 +29,45 @@ __device__ __forceinline__ void tanh_slope(double z, double& a, double& slope) {
   p = fma(p, r, 1.0 / 6.0);
   p = fma(p, r, 0.5);
   p = fma(p * r, r, r);
-  const double two_n = ldexp(1.0, (int)n), m = fma(two_n, p, two_n - 1.0), den = 2.0 + m;
-  double q = __builtin_amdgcn_rcp(den);
-  q = fma(fma(-den, q, 1.0), q, q);
-  q = fma(fma(-den, q, 1.0), q, q);
-  double h = -m * q;
-  h = fma(fma(-den, h, -m), q, h);
-  a = copysign(h, z);
-  slope = 4.0 * fma(two_n, p, two_n) * q * q;
+  two_n = ldexp(1.0, (int)n);
+  return fma(two_n, p, two_n - 1.0);
 }
-__device__ __forceinline__ void tanh_slope(float z, float& a, float& slope) {
-  const float x = fabsf(z) > 15.0f ? 15.0f : fabsf(z), y = -2.0f * x, n = rintf(y * 1.44269504f);
-  float r = fmaf(n, -0.693359375f, y);
+__device__ __forceinline__ float exp_minus_one(float x, float& two_n, float& p) {
+  const float n = rintf(x * -1.44269504f);
+  float r = fmaf(n, -0.693359375f, -x);
   r = fmaf(n, 2.12194440e-4f, r);
-  float p = 1.0f / 5040.0f;
+  p = 1.0f / 5040.0f;
   p = fmaf(p, r, 1.0f / 720.0f);
   p = fmaf(p, r, 1.0f / 120.0f);
   p = fmaf(p, r, 1.0f / 24.0f);
   p = fmaf(p, r, 1.0f / 6.0f);
   p = fmaf(p, r, 0.5f);
   p = fmaf(p * r, r, r);
-  const float two_n = ldexpf(1.0f, (int)n), m = fmaf(two_n, p, two_n - 1.0f), den = 2.0f + m;
-  float q = __builtin_amdgcn_rcpf(den);
-  q = fmaf(fmaf(-den, q, 1.0f), q, q);
-  float h = -m * q;
-  h = fmaf(fmaf(-den, h, -m), q, h);
-  a = copysignf(h, z);
-  slope = 4.0f * fmaf(two_n, p, two_n) * q * q;
+  two_n = ldexpf(1.0f, (int)n);
+  return fmaf(two_n, p, two_n - 1.0f);
+}
+// 1 / v for 1 <= v <= 2, within a unit in the last place
+__device__ __forceinline__ double reciprocal(double v) {
+  double q = __builtin_amdgcn_rcp(v);
+  q = fma(fma(-v, q, 1.0), q, q);
+  return fma(fma(-v, q, 1.0), q, q);
+}
+__device__ __forceinline__ float reciprocal(float v) {
+  const float q = __builtin_amdgcn_rcpf(v);
+  return fmaf(fmaf(-v, q, 1.0f), q, q);
 }
 
 // act(z) and act'(z), to a few units of the arithmetic type's last place
 template <typename A>
 __device__ __forceinline__ void activate_exact(int act, A z, A& a, A& slope) {
-  if (act == VMCPDE_ACT_TANH) {
-    tanh_slope(z, a, slope);
+  const A x = fabs(z);
+  if (act == VMCPDE_ACT_TANH) {             // with m = e^-2|z| - 1: tanh |z| = -m / (2 + m), the slope 4 (1 + m) / (2 + m)^2
+    A two_n, p;
+    const A m = exp_minus_one(x > 25 ? (A)50 : 2 * x, two_n, p), den = 2 + m, q = reciprocal(den);      // (NaN stays)
+    A h = -m * q;
+    h = fma(fma(-den, h, -m), q, h);
+    a = copysign(h, z);
+    slope = 4 * fma(two_n, p, two_n) * q * q;
   } else if (act == VMCPDE_ACT_GELU) {
     A cdf, density;
     if constexpr (sizeof(A) == 8) {
@@ -73,14 +77,14 @@ __device__ __forceinline__ void activate_exact(int act, A z, A& a, A& slope) {
       cdf = 0.5f * erfcf(-z * 0.70710678f);
       density = 0.39894228f * expf(-0.5f * z * z);
     }
-    a = z * cdf;
+    a = z == -(A)INFINITY ? 0 : z * cdf;
     slope = density != 0 ? cdf + z * density : cdf;      // (z = +-inf: no inf * 0)
-    if (z == -(A)INFINITY) a = 0;
-  } else {
-    const A e = sizeof(A) == 8 ? (A)exp(-(double)z) : (A)expf(-(float)z);
-    const A gate = 1 / (1 + e);
+  } else {                                  // with e = e^-|z|: the gate is 1 / (1 + e), or e / (1 + e) for z < 0
+    A two_n, p;
+    const A far = sizeof(A) == 8 ? 800 : 120;
+    const A q = reciprocal(2 + exp_minus_one(x > far ? far : x, two_n, p)), e = fma(two_n, p, two_n), gate = z < 0 ? e * q : q, rest = z < 0 ? q : e * q;
     a = z == -(A)INFINITY ? 0 : z * gate;
-    slope = gate != 0 && gate != 1 ? gate * (1 + z * (1 - gate)) : gate;
+    slope = gate != 0 && rest != 0 ? gate * (1 + z * rest) : gate;
   }
 }
 

@@ -212,7 +212,7 @@ __global__ __launch_bounds__(THREADS) void norm_backward_kernel(const T* __restr
   typedef typename Wide<T>::type A;
   constexpr int V = vec_of<T>(), GROUPS = THREADS / LANES, WAVES = THREADS / 64;
   constexpr int SHARED = LANES <= 64 ? WAVES * LANES * ITER * V : 4 * WAVES;   // column sums of every wave, or the slots of the row sums
-  constexpr bool KEEP = LANES < 1024 || ITER * V <= 8;           // (1024 lanes have 128 registers each)
+  constexpr bool KEEP = LANES < 1024 || ITER * V <= 8, AHEAD = LANES < 1024 || ITER * (int)sizeof(T) <= 8;      // (1024 lanes have 128 registers each)
   __shared__ A sh[SHARED];
   const int lane = threadIdx.x % LANES;
   const A inv = (A)1 / (A)cols;
@@ -236,9 +236,10 @@ __global__ __launch_bounds__(THREADS) void norm_backward_kernel(const T* __restr
     }
   };
   int64_t first = (int64_t)blockIdx.x * GROUPS;
-  if (first < rows) fetch(first + threadIdx.x / LANES);
+  if (AHEAD && first < rows) fetch(first + threadIdx.x / LANES);
   for (int turn = 0; first < rows; turn ^= 1) {
     const int64_t row = first + threadIdx.x / LANES;
+    if (!AHEAD) fetch(row);
     const bool live = GROUPS == 1 || row < rows;                 // lanes of no row add zeros
     first += (int64_t)gridDim.x * GROUPS;
     const A mean = next_mean, rstd = next_rstd;
@@ -250,7 +251,7 @@ __global__ __launch_bounds__(THREADS) void norm_backward_kernel(const T* __restr
         h[i][k] = live ? ((A)next_x[i].v[k] - mean) * rstd : (A)0;
         g[i][k] = live ? (A)next_d[i].v[k] : (A)0;
       }
-    if (first < rows) fetch(first + threadIdx.x / LANES);
+    if (AHEAD && first < rows) fetch(first + threadIdx.x / LANES);
 #pragma unroll
     for (int i = 0; i < ITER; ++i) {
       A wi[V];
