@@ -393,7 +393,7 @@ __device__ __forceinline__ void tile_product(const Product& g, int row0, int col
   }
   // Sixteen rows at a time through a piece of LDS of the wave's own, so that a lane ends with N columns of a row and a row's lanes write whole lines.
   // The loop stays rolled (the epilogue is long); the registers are picked by number inside it.
-  constexpr int N = sizeof(T) == 8 ? 2 : sizeof(T) == 4 || TN == 1 ? 4 : 8, COLS = TN * 16, PITCH = COLS + 4;
+  constexpr int N = TN == 1 ? 4 : 8, COLS = TN * 16, PITCH = COLS + 4;
   static_assert(WM * WN * 16 * PITCH * (int)sizeof(A) <= STAGES * (P::BYTES + Q::BYTES), "the rows fit the tiles' LDS");
   __syncthreads();
   A* rows = reinterpret_cast<A*>(tiles) + wave * 16 * PITCH;
