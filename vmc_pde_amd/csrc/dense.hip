@@ -478,8 +478,8 @@ __global__ __launch_bounds__(256) void product_join_kernel(const typename Wide<T
 // ---- what is made ready before the products --------------------------------------------------------------------------------------------
 
 // Up to three copies in one launch: lines of n elements to lines of ld_to (zeros behind n), scaled by scale * slope: an operand into lines that the
-// products can fetch, or dz = scale * slope * dy; `to` may be null.  With `partial` also sums of dz's columns over the lines that a workgroup takes:
-// partial[group][n].  `lanes` (a power of two) lie along the columns, 256 / lanes lines are taken at a time.
+// products can fetch, or dz = scale * slope * dy; `to` may be null.  With `sums` also the sums of dz's columns, or where several groups of workgroups share
+// the lines each one's part of them: partial[group][n].  `lanes` (a power of two) lie along the columns, 256 / lanes lines are taken at a time.
 template <typename T>
 struct Job {
   const T* from;
@@ -489,6 +489,7 @@ struct Job {
   T* to;
   int64_t ld_to;
   typename Wide<T>::type* partial;
+  T* sums;             // with one group: the sums themselves
   int32_t lanes_log2, col_blocks, groups, first;       // first: the job's first workgroup in the launch
 };
 template <typename T>
@@ -524,14 +525,17 @@ __global__ __launch_bounds__(256) void prepare_kernel(Jobs<T> jobs) {
     }
     if (b.to) store_vec<T, V>(b.to + r * b.ld_to, col, b.ld_to, v);
   }
-  if (!b.partial) return;
+  if (!b.sums) return;
 #pragma unroll
   for (int k = 0; k < V; ++k) sh[(part * lanes + lane) * V + k] = sum[k];
   __syncthreads();
   for (int c = threadIdx.x; c < lanes * V; c += 256) {
     A v = 0;
     for (int p = 0; p < at_once; ++p) v += sh[p * lanes * V + c];
-    if (col0 + c < b.n) b.partial[(int64_t)group * b.n + col0 + c] = v;
+    if (col0 + c < b.n) {
+      if (b.groups == 1) b.sums[col0 + c] = (T)v;
+      else b.partial[(int64_t)group * b.n + col0 + c] = v;
+    }
   }
 }
 
@@ -626,11 +630,13 @@ __global__ __launch_bounds__(256) void thin_forward_kernel(const T* __restrict__
   }
 }
 
-// dx (may be null) and this workgroup's sums partial[blockIdx.x][n_in * n_out + n_out] of x^T dz and dz (null: not wanted).
+// dx (may be null) and this workgroup's sums partial[blockIdx.x][n_in * n_out + n_out] of x^T dz and dz (null: not wanted); a single workgroup writes them
+// to dkernel and dbias (either may be null) itself.
 template <typename T, int KT, int NT>
 __global__ __launch_bounds__(THIN_THREADS) void thin_backward_kernel(const T* __restrict__ dy, int64_t ldd, const T* __restrict__ slope, T scale,
                                                                      const T* __restrict__ x, int64_t ldx, const T* __restrict__ w, int64_t sk, int64_t sn, int64_t rows,
-                                                                     int n_in, int n_out, T* __restrict__ dx, T* __restrict__ partial) {
+                                                                     int n_in, int n_out, T* __restrict__ dx, T* __restrict__ partial, T* __restrict__ dkernel,
+                                                                     T* __restrict__ dbias) {
   typedef typename Matrix<T>::Acc Acc;
   constexpr int NS = NT * 4, WAVES = THIN_THREADS / 64, SUMS = KT * 16 * NT * 16 + NT * 16;
   __shared__ T sh[WAVES * 2 * THIN_TILE], wt[KT * 16 * THIN_PITCH];
@@ -760,7 +766,9 @@ __global__ __launch_bounds__(THIN_THREADS) void thin_backward_kernel(const T* __
     if (n < n_out && (is_bias || k < n_in)) {
       T v = sh[u];
       for (int s = 1; s < WAVES / 2; ++s) v += sh[s * SUMS + u];
-      to[(is_bias ? n_in : k) * n_out + n] = v;
+      if (gridDim.x > 1) to[(is_bias ? n_in : k) * n_out + n] = v;
+      else if (is_bias && dbias) dbias[n] = v;
+      else if (!is_bias && dkernel) dkernel[k * n_out + n] = v;
     }
   }
 }
@@ -777,7 +785,7 @@ constexpr Cost F32_COST = {64, 4, 0.65, 0.5}, F64_COST = {64, 4, 0.7, 0.55};
 
 // Tile and k slices of a product of `steps` steps of k.  Sides of at most 32 rows or columns take 32, so that little is multiplied for nothing: those read
 // one long operand once, and the k range is cut until two workgroups a CU do.  Everything else takes the tile and the number of slices of the least
-// estimated time: the steps of the fullest CU, and with slices a second launch that reads and joins their sums (3 us and their bytes at 4 TB/s).  The
+// estimated time: the steps of the fullest CU, and with slices a second launch that reads and joins their sums (5 us, of which the host takes most, and their bytes at 4 TB/s).  The
 // estimate finds the best choice, or one within 15 % of it, for the 27 shapes that it was made from (three types, 0.1 to 140 GFLOP).
 template <typename T>
 Tiles tiles_of(int64_t m, int64_t n, int64_t steps) {
@@ -794,7 +802,7 @@ Tiles tiles_of(int64_t m, int64_t n, int64_t steps) {
         if (s > 1 && (steps < 2 * s || tiles * s > 2048)) break;
         const double on_one = (double)ceil_div(tiles * s, 256);
         const double time = (double)ceil_div(steps, s) * std::max(c.alone * std::ceil(on_one / c.held), on_one * c.each) +
-                            (s > 1 ? 3 + (double)s * m * n * 2 * sizeof(typename Wide<T>::type) / 4e6 : 0);
+                            (s > 1 ? 5 + (double)s * m * n * 2 * sizeof(typename Wide<T>::type) / 4e6 : 0);
         if (time < least) {
           least = time;
           best.bm = best.bn = c.side;
@@ -881,7 +889,7 @@ struct Dense {
 
   // A job of the launch before the products; its groups are also the rows of `partial`.
   Job<T> job_of(const Lines& o) {
-    Job<T> b = {static_cast<const T*>(o.p), o.ld, o.lines, o.n, nullptr, 1, nullptr, o.n, nullptr, 5, 1, 1, 0};
+    Job<T> b = {static_cast<const T*>(o.p), o.ld, o.lines, o.n, nullptr, 1, nullptr, o.n, nullptr, nullptr, 5, 1, 1, 0};
     while (b.lanes_log2 > 2 && (int64_t)vec_of<T>() << (b.lanes_log2 - 1) >= o.n) --b.lanes_log2;
     return b;
   }
@@ -894,7 +902,8 @@ struct Dense {
   // workgroups: some 2048 along both axes, at most 512 along the lines
   static void shape(Job<T>& b, int64_t width) {
     b.col_blocks = (int)ceil_div(width, (int64_t)vec_of<T>() << b.lanes_log2);
-    b.groups = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(512, std::max(1, 2048 / b.col_blocks)), ceil_div(b.lines, 256 >> b.lanes_log2)));
+    const int64_t rounds = ceil_div(b.lines, 256 >> b.lanes_log2);
+    b.groups = rounds <= 4 ? 1 : (int)std::min<int64_t>(std::min<int64_t>(512, std::max(1, 2048 / b.col_blocks)), rounds);
   }
   void launch_jobs() {
     if (launch && jobs.count) prepare_kernel<T><<<jobs.blocks, 256, 0, stream>>>(jobs);
@@ -940,18 +949,19 @@ struct Dense {
   void thin_backward(const vmcpde_dense_args& a, unsigned groups, T* partial) {
     thin_backward_kernel<T, KT, NT><<<groups, THIN_THREADS, 0, stream>>>(
         static_cast<const T*>(a.dy), a.ldd, static_cast<const T*>(a.slope), (T)a.scale, a.dkernel ? static_cast<const T*>(a.x) : nullptr, a.ldx,
-        static_cast<const T*>(a.kernel), a.kernel_t ? 1 : a.ldk, a.kernel_t ? a.ldk : 1, a.rows, (int)a.n_in, (int)a.n_out, static_cast<T*>(a.dx), partial);
+        static_cast<const T*>(a.kernel), a.kernel_t ? 1 : a.ldk, a.kernel_t ? a.ldk : 1, a.rows, (int)a.n_in, (int)a.n_out, static_cast<T*>(a.dx), partial,
+        static_cast<T*>(a.dkernel), static_cast<T*>(a.dbias));
   }
 
   void thin_backward(const vmcpde_dense_args& a) {
-    const int64_t groups = std::max<int64_t>(1, std::min<int64_t>(ceil_div(a.rows, 16 * (THIN_THREADS / 64)), THIN_GROUPS)), sums = (a.n_in + 1) * a.n_out;
+    const int64_t rounds = ceil_div(a.rows, 16 * (THIN_THREADS / 64)), groups = rounds <= 4 ? 1 : std::min<int64_t>(rounds, THIN_GROUPS), sums = (a.n_in + 1) * a.n_out;
     T* partial = a.dkernel || a.dbias ? static_cast<T*>(take(groups * sums * (int64_t)sizeof(T))) : nullptr;
     if (!launch || (!partial && !(a.dx && a.rows))) return;
     if (a.n_in <= 16 && a.n_out <= 16) thin_backward<1, 1>(a, (unsigned)groups, partial);
     else if (a.n_in <= 16) thin_backward<1, 2>(a, (unsigned)groups, partial);
     else if (a.n_out <= 16) thin_backward<2, 1>(a, (unsigned)groups, partial);
     else thin_backward<2, 2>(a, (unsigned)groups, partial);
-    if (partial)
+    if (partial && groups > 1)
       add_columns<T, T>(partial, groups, sums, a.n_in * a.n_out, a.n_out, static_cast<T*>(a.dkernel), static_cast<T*>(a.dbias), stream);
   }
 
@@ -991,13 +1001,14 @@ struct Dense {
     if (own || a.dbias) {
       b.slope = static_cast<const S*>(a.slope);
       b.scale = (A)a.scale;
-      if (a.dbias) b.partial = static_cast<A*>(take(b.groups * a.n_out * (int64_t)sizeof(A)));
+      b.sums = static_cast<T*>(a.dbias);
+      if (a.dbias && b.groups > 1) b.partial = static_cast<A*>(take(b.groups * a.n_out * (int64_t)sizeof(A)));
       add(b);
     }
     const bool want_x = a.dx && a.rows;
     const Lines kernel = want_x ? ready(kernel_lines(a), !a.kernel_t) : Lines(), x = a.dkernel ? ready({a.x, a.rows, a.n_in, a.ldx}, false) : Lines();
     launch_jobs();
-    if (launch && a.dbias) add_columns<A, T>(b.partial, b.groups, a.n_out, a.n_out, 0, static_cast<T*>(a.dbias), nullptr, stream);
+    if (launch && b.partial) add_columns<A, T>(b.partial, b.groups, a.n_out, a.n_out, 0, static_cast<T*>(a.dbias), nullptr, stream);
     if (want_x) {
       const Epilogue<T> e = {nullptr, nullptr, 0, static_cast<T*>(a.dx), a.n_in, nullptr, a.n_in, 1, VMCPDE_ACT_NONE};
       Lines z = dz;

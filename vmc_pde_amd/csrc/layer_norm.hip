@@ -203,12 +203,14 @@ __global__ __launch_bounds__(1024) void norm_forward_wide_kernel(const T* __rest
   }
 }
 
-// dx (may be null) and, with `partial`, this workgroup's column sums: partial[group][2][cols] = { sum dy h, sum dy }
+// dx (may be null) and, with `partial`, this workgroup's column sums: partial[group][2][cols] = { sum dy h, sum dy }; a single workgroup writes them to
+// dweight and dbias (either may be null) itself.
 template <typename T, typename W, int LANES, int ITER, int THREADS, bool EXACT>
 __global__ __launch_bounds__(THREADS) void norm_backward_kernel(const T* __restrict__ dy, int64_t ldd, const T* __restrict__ x, int64_t ldx,
                                                                 const typename Wide<T>::type* __restrict__ mean_in,
                                                                 const typename Wide<T>::type* __restrict__ rstd_in, const W* __restrict__ weight,
-                                                                int64_t rows, int64_t cols, T* __restrict__ dx, typename Wide<T>::type* __restrict__ partial) {
+                                                                int64_t rows, int64_t cols, T* __restrict__ dx, typename Wide<T>::type* __restrict__ partial,
+                                                                W* __restrict__ dweight, W* __restrict__ dbias) {
   typedef typename Wide<T>::type A;
   constexpr int V = vec_of<T>(), GROUPS = THREADS / LANES, WAVES = THREADS / 64;
   constexpr int SHARED = LANES <= 64 ? WAVES * LANES * ITER * V : 4 * WAVES;   // column sums of every wave, or the slots of the row sums
@@ -283,13 +285,19 @@ __global__ __launch_bounds__(THREADS) void norm_backward_kernel(const T* __restr
     }
   }
   if (!partial) return;
-  A* out = partial + (int64_t)blockIdx.x * 2 * cols;
+  const bool alone = gridDim.x == 1;
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
+    A* out = partial + ((int64_t)blockIdx.x * 2 + which) * cols;
+    W* last = which ? dbias : dweight;
+    if (alone && !last) continue;
     if constexpr (LANES > 64) {
 #pragma unroll
       for (int i = 0; i < ITER; ++i)
-        if (EXACT || at.skip[i] < V) put<A, V>(out + which * cols + at.base[i], which ? db[i] : dw[i]);
+        if (EXACT || at.skip[i] < V) {
+          if (alone) put<W, V>(last + at.base[i], which ? db[i] : dw[i]);
+          else put<A, V>(out + at.base[i], which ? db[i] : dw[i]);
+        }
     } else {
       const int wave = threadIdx.x >> 6;
       __syncthreads();
@@ -308,8 +316,11 @@ __global__ __launch_bounds__(THREADS) void norm_backward_kernel(const T* __restr
       for (int c = threadIdx.x; c < ITER * LANES * V; c += THREADS) {
         A v = 0;
         for (int w = 0; w < WAVES; ++w) v += sh[w * ITER * LANES * V + c];
-        const int col = c / V * V;
-        if (col < cols) out[which * cols + min(col, (int)cols - V) + c % V] = v;
+        const int nominal = c / V * V, col = min(nominal, (int)cols - V) + c % V;
+        if (nominal < cols) {
+          if (alone) last[col] = (W)v;
+          else out[col] = v;
+        }
       }
     }
   }
@@ -392,12 +403,13 @@ Shape shape_of(int64_t cols, int vec, int most, int most_1024) {
   return {0, 0, 1024};
 }
 
-// workgroups of the backward pass: enough to fill the card, few enough that their column sums stay small beside the rows
+// workgroups of the backward pass: enough to fill the card, few enough that their column sums stay small beside the rows; one for up to four rows each of
+// its groups of lanes, which then needs no second launch
 int64_t backward_groups(const Shape& s, int64_t rows) {
   const int64_t per = s.lanes ? s.threads / s.lanes : 4;
   const int64_t most = s.threads == 1024 ? 256 : 1024;
   const int64_t n = ceil_div(rows, per);
-  return n < 1 ? 1 : n < most ? n : most;
+  return n <= 4 ? 1 : n < most ? n : most;
 }
 
 template <typename T, typename W>
@@ -442,7 +454,7 @@ struct Norm {
   static void backward_exactly(const vmcpde_norm_args& a, int64_t groups, A* partial, hipStream_t s) {
     norm_backward_kernel<T, W, LANES, ITER, THREADS, EXACT><<<(unsigned)groups, THREADS, 0, s>>>(
         static_cast<const T*>(a.dy), a.ldd, static_cast<const T*>(a.x), a.ldx, static_cast<const A*>(a.mean), static_cast<const A*>(a.rstd),
-        static_cast<const W*>(a.weight), a.rows, a.cols, static_cast<T*>(a.dx), partial);
+        static_cast<const W*>(a.weight), a.rows, a.cols, static_cast<T*>(a.dx), partial, static_cast<W*>(a.dweight), static_cast<W*>(a.dbias));
   }
   template <int LANES, int THREADS>
   static void backward_iter(int iter, const vmcpde_norm_args& a, int64_t groups, A* partial, hipStream_t s) {
@@ -469,7 +481,7 @@ struct Norm {
             static_cast<const T*>(a.dy), a.ldd, static_cast<const T*>(a.x), a.ldx, static_cast<const A*>(a.mean), static_cast<const A*>(a.rstd), a.rows, a.cols,
             partial);
     }
-    if (partial)
+    if (partial && (groups > 1 || !p.lanes))
       add_columns<A, W>(partial, groups, 2 * a.cols, a.cols, a.cols, static_cast<W*>(a.dweight), static_cast<W*>(a.dbias), s);
   }
 };
