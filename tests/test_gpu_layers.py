@@ -25,7 +25,7 @@ def normal(shape, dtype, seed, scale=1.0):
 # ---- dense -------------------------------------------------------------------------------------------------------------------------------
 
 SIZES = [(0, 5, 7), (1, 1, 1), (1, 8, 16), (3, 5, 7), (17, 33, 65), (33, 64, 8), (128, 128, 128), (130, 129, 131), (257, 64, 40), (1, 2048, 264), (5, 1000, 513),
-         (64, 520, 24), (1000, 21, 21), (2049, 40, 9), (300, 520, 264), (512, 256, 512), (40, 16, 1300), (3500, 72, 4100), (40, 3601, 3700), (70, 32, 32), (70, 33, 32), (333, 8, 17), (333, 16, 16), (17, 17, 1), (9000, 24, 30), (200, 1, 21)]
+         (64, 520, 24), (1000, 21, 21), (2049, 40, 9), (300, 520, 264), (512, 256, 512), (40, 16, 1300), (3500, 72, 4100), (40, 3601, 3700), (70, 32, 32), (70, 33, 32), (333, 8, 17), (333, 16, 16), (17, 17, 1), (9000, 24, 30), (200, 1, 21), (700, 43, 43), (520, 48, 30), (1000, 12, 48), (90, 40, 7), (64, 49, 48)]
 ACTS = ["none", "tanh", "gelu", "silu"]
 
 

@@ -541,24 +541,27 @@ __global__ __launch_bounds__(256) void prepare_kernel(Jobs<T> jobs) {
 
 // ---- thin layers ---------------------------------------------------------------------------------------------------------------------
 
-// At most 32 inputs and outputs in fp32 or fp64 (the flow's own conditioners): bound by reading and writing the rows once.  The kernel's fragments
+// At most 48 inputs and outputs in fp32 or fp64 (the flow's own conditioners): bound by reading and writing the rows once.  The kernel's fragments
 // stay in registers, a wave takes sixteen rows at a time, and no operand is copied.  Between memory and the matrix instruction's lane layout a tile
 // passes through a piece of LDS of the wave's own: its elements are fetched and written in the order of the rows (whole lines at any pitch), and the
 // epilogue runs over them in that order too, so that no lane evaluates an activation for a column that is not there.
-constexpr int THIN = 32, THIN_THREADS = 512, THIN_GROUPS = 256, THIN_PITCH = 36, THIN_TILE = 16 * THIN_PITCH;
+constexpr int THIN = 48, THIN_THREADS = 512, THIN_GROUPS = 256;
+// pitch of a tile's rows in LDS: sixteen rows four or eight banks apart
+constexpr int thin_pitch(int wide) { return wide <= 32 ? 36 : 52; }
 
 __device__ __forceinline__ float4v mfma4(float a, float b, float4v c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ double4v mfma4(double a, double b, double4v c) { return __builtin_amdgcn_mfma_f64_16x16x4f64(a, b, c, 0, 0, 0); }
 // row of a 16 x 16 result that register r of a lane of group g holds
 template <typename T> __device__ __forceinline__ int result_row(int g, int r) { return sizeof(T) == 8 ? g + 4 * r : g * 4 + r; }
 
-// Element u < 16 n of sixteen rows of n <= 32 (the product is off by far less than the half that keeps it from a whole number)
+// Element u < 16 n of sixteen rows of n <= 48 (the product is off by far less than the half that keeps it from a whole number)
+template <int PITCH>
 struct InOrder {
   int n;
   float inv;
   __device__ __forceinline__ explicit InOrder(int n_) : n(n_), inv(1.0f / (float)n_) {}
   __device__ __forceinline__ int row(int u) const { return (int)(((float)u + 0.5f) * inv); }
-  __device__ __forceinline__ int place(int u, int r) const { return r * THIN_PITCH + u - r * n; }
+  __device__ __forceinline__ int place(int u, int r) const { return r * PITCH + u - r * n; }
 };
 
 // The kernel's element (k, n) is at w[k * sk + n * sn].  KS: steps of four inputs, NT: tiles of sixteen outputs.
@@ -566,14 +569,15 @@ template <typename T, int KS, int NT>
 __global__ __launch_bounds__(256) void thin_forward_kernel(const T* __restrict__ x, int64_t ldx, const T* __restrict__ w, int64_t sk, int64_t sn, int64_t rows, int n_in,
                                                            Epilogue<T> e) {
   typedef typename Matrix<T>::Acc Acc;
-  __shared__ T sh[4][2][THIN_TILE];
+  constexpr int PITCH = thin_pitch(KS * 4 > NT * 16 ? KS * 4 : NT * 16), TILE = 16 * PITCH;
+  __shared__ T sh[4][2][TILE];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4, n_out = (int)e.n;
   const int64_t tiles = (rows + 15) / 16, stride = (int64_t)gridDim.x * 4;
   int64_t tile = (int64_t)blockIdx.x * 4 + wave;
   if (tile >= tiles) return;
   T* tx = sh[wave][0];
   T* tz = sh[wave][1];
-  const InOrder in(n_in), out(n_out);
+  const InOrder<PITCH> in(n_in), out(n_out);
   T wf[KS][NT], bias[NT], xv[KS];
 #pragma unroll
   for (int b = 0; b < NT; ++b) {
@@ -581,7 +585,7 @@ __global__ __launch_bounds__(256) void thin_forward_kernel(const T* __restrict__
 #pragma unroll
     for (int s = 0; s < KS; ++s) wf[s][b] = 4 * s + g < n_in && b * 16 + i < n_out ? w[(4 * s + g) * sk + (b * 16 + i) * sn] : (T)0;
   }
-  for (int u = lane; u < THIN_TILE; u += 64) tx[u] = 0;          // (behind the inputs it stays zero)
+  for (int u = lane; u < TILE; u += 64) tx[u] = 0;          // (behind the inputs it stays zero)
   auto load = [&](int64_t at) {                                  // (no branches: a lane without an element reads the tile's first one, so that all loads fly at once)
     const T* p = x + at * 16 * ldx;
     const int live = (int)min((int64_t)16, rows - at * 16);
@@ -606,14 +610,14 @@ __global__ __launch_bounds__(256) void thin_forward_kernel(const T* __restrict__
     for (int b = 0; b < NT; ++b) acc[b] = {bias[b], bias[b], bias[b], bias[b]};
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
-      const T xf = tx[i * THIN_PITCH + 4 * s + g];
+      const T xf = tx[i * PITCH + 4 * s + g];
 #pragma unroll
       for (int b = 0; b < NT; ++b) acc[b] = mfma4(xf, wf[s][b], acc[b]);
     }
 #pragma unroll
     for (int b = 0; b < NT; ++b)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) tz[result_row<T>(g, r) * THIN_PITCH + b * 16 + i] = acc[b][r];
+      for (int r = 0; r < 4; ++r) tz[result_row<T>(g, r) * PITCH + b * 16 + i] = acc[b][r];
     __builtin_amdgcn_wave_barrier();
     const int live = (int)min((int64_t)16, rows - tile * 16) * n_out;
 #pragma unroll 1
@@ -638,19 +642,19 @@ __global__ __launch_bounds__(THIN_THREADS) void thin_backward_kernel(const T* __
                                                                      int n_in, int n_out, T* __restrict__ dx, T* __restrict__ partial, T* __restrict__ dkernel,
                                                                      T* __restrict__ dbias) {
   typedef typename Matrix<T>::Acc Acc;
-  constexpr int NS = NT * 4, WAVES = THIN_THREADS / 64, SUMS = KT * 16 * NT * 16 + NT * 16;
-  __shared__ T sh[WAVES * 2 * THIN_TILE], wt[KT * 16 * THIN_PITCH];
-  static_assert(WAVES / 2 * SUMS <= WAVES * 2 * THIN_TILE, "the sums fit the tiles' LDS");
+  constexpr int PITCH = thin_pitch(16 * (KT > NT ? KT : NT)), TILE = 16 * PITCH, NS = NT * 4, WAVES = THIN_THREADS / 64, SUMS = KT * 16 * NT * 16 + NT * 16;
+  __shared__ T sh[WAVES * 2 * TILE], wt[KT * 16 * PITCH];
+  static_assert(WAVES / 2 * SUMS <= WAVES * 2 * TILE, "the sums fit the tiles' LDS");
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
   const int64_t tiles = (rows + 15) / 16, stride = (int64_t)gridDim.x * WAVES;
-  T* tx = sh + wave * 2 * THIN_TILE;
-  T* tz = tx + THIN_TILE;
-  const InOrder in(n_in), out(n_out);
+  T* tx = sh + wave * 2 * TILE;
+  T* tz = tx + TILE;
+  const InOrder<PITCH> in(n_in), out(n_out);
   for (int u = threadIdx.x; u < KT * 16 * NT * 16; u += THIN_THREADS) {
     const int k = u / (NT * 16), n = u % (NT * 16);
-    wt[k * THIN_PITCH + n] = dx && k < n_in && n < n_out ? w[k * sk + n * sn] : (T)0;
+    wt[k * PITCH + n] = dx && k < n_in && n < n_out ? w[k * sk + n * sn] : (T)0;
   }
-  for (int u = lane; u < 2 * THIN_TILE; u += 64) tx[u] = 0;      // (behind dz's columns it stays zero: they are summed over)
+  for (int u = lane; u < 2 * TILE; u += 64) tx[u] = 0;      // (behind dz's columns it stays zero: they are summed over)
   __syncthreads();
   Acc sum[KT][NT];
   T bias[NT];
@@ -702,10 +706,10 @@ __global__ __launch_bounds__(THIN_THREADS) void thin_backward_kernel(const T* __
       for (int s = 0; s < 4; ++s) {
         T xc[KT];
 #pragma unroll
-        for (int a = 0; a < KT; ++a) xc[a] = tx[(4 * s + g) * THIN_PITCH + a * 16 + i];
+        for (int a = 0; a < KT; ++a) xc[a] = tx[(4 * s + g) * PITCH + a * 16 + i];
 #pragma unroll
         for (int b = 0; b < NT; ++b) {
-          const T zc = tz[(4 * s + g) * THIN_PITCH + b * 16 + i];
+          const T zc = tz[(4 * s + g) * PITCH + b * 16 + i];
           bias[b] += zc;
 #pragma unroll
           for (int a = 0; a < KT; ++a) sum[a][b] = mfma4(xc[a], zc, sum[a][b]);
@@ -718,15 +722,15 @@ __global__ __launch_bounds__(THIN_THREADS) void thin_backward_kernel(const T* __
       for (int a = 0; a < KT; ++a) acc[a] = {0, 0, 0, 0};
 #pragma unroll
       for (int s = 0; s < NS; ++s) {
-        const T zr = tz[i * THIN_PITCH + 4 * s + g];
+        const T zr = tz[i * PITCH + 4 * s + g];
 #pragma unroll
-        for (int a = 0; a < KT; ++a) acc[a] = mfma4(zr, wt[(a * 16 + i) * THIN_PITCH + 4 * s + g], acc[a]);
+        for (int a = 0; a < KT; ++a) acc[a] = mfma4(zr, wt[(a * 16 + i) * PITCH + 4 * s + g], acc[a]);
       }
       __builtin_amdgcn_wave_barrier();
 #pragma unroll
       for (int a = 0; a < KT; ++a)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) tx[result_row<T>(g, r) * THIN_PITCH + a * 16 + i] = acc[a][r];
+        for (int r = 0; r < 4; ++r) tx[result_row<T>(g, r) * PITCH + a * 16 + i] = acc[a][r];
       __builtin_amdgcn_wave_barrier();
       T* dxt = dx + tile * 16 * n_in;
 #pragma unroll 4
@@ -942,7 +946,8 @@ struct Dense {
     if (a.n_in <= 8) thin_forward_kernel<T, 2, NT><<<groups, 256, 0, stream>>>(x, a.ldx, w, sk, sn, a.rows, (int)a.n_in, e);
     else if (a.n_in <= 16) thin_forward_kernel<T, 4, NT><<<groups, 256, 0, stream>>>(x, a.ldx, w, sk, sn, a.rows, (int)a.n_in, e);
     else if (a.n_in <= 24) thin_forward_kernel<T, 6, NT><<<groups, 256, 0, stream>>>(x, a.ldx, w, sk, sn, a.rows, (int)a.n_in, e);
-    else thin_forward_kernel<T, 8, NT><<<groups, 256, 0, stream>>>(x, a.ldx, w, sk, sn, a.rows, (int)a.n_in, e);
+    else if (a.n_in <= 32) thin_forward_kernel<T, 8, NT><<<groups, 256, 0, stream>>>(x, a.ldx, w, sk, sn, a.rows, (int)a.n_in, e);
+    else thin_forward_kernel<T, 12, NT><<<groups, 256, 0, stream>>>(x, a.ldx, w, sk, sn, a.rows, (int)a.n_in, e);
   }
 
   template <int KT, int NT>
@@ -953,14 +958,20 @@ struct Dense {
         static_cast<T*>(a.dkernel), static_cast<T*>(a.dbias));
   }
 
+  template <int KT>
+  void thin_backward_outputs(const vmcpde_dense_args& a, unsigned groups, T* partial) {
+    if (a.n_out <= 16) thin_backward<KT, 1>(a, groups, partial);
+    else if (a.n_out <= 32) thin_backward<KT, 2>(a, groups, partial);
+    else thin_backward<KT, 3>(a, groups, partial);
+  }
+
   void thin_backward(const vmcpde_dense_args& a) {
     const int64_t rounds = ceil_div(a.rows, 16 * (THIN_THREADS / 64)), groups = rounds <= 4 ? 1 : std::min<int64_t>(rounds, THIN_GROUPS), sums = (a.n_in + 1) * a.n_out;
     T* partial = a.dkernel || a.dbias ? static_cast<T*>(take(groups * sums * (int64_t)sizeof(T))) : nullptr;
     if (!launch || (!partial && !(a.dx && a.rows))) return;
-    if (a.n_in <= 16 && a.n_out <= 16) thin_backward<1, 1>(a, (unsigned)groups, partial);
-    else if (a.n_in <= 16) thin_backward<1, 2>(a, (unsigned)groups, partial);
-    else if (a.n_out <= 16) thin_backward<2, 1>(a, (unsigned)groups, partial);
-    else thin_backward<2, 2>(a, (unsigned)groups, partial);
+    if (a.n_in <= 16) thin_backward_outputs<1>(a, (unsigned)groups, partial);
+    else if (a.n_in <= 32) thin_backward_outputs<2>(a, (unsigned)groups, partial);
+    else thin_backward_outputs<3>(a, (unsigned)groups, partial);
     if (partial && groups > 1)
       add_columns<T, T>(partial, groups, sums, a.n_in * a.n_out, a.n_out, static_cast<T*>(a.dkernel), static_cast<T*>(a.dbias), stream);
   }
@@ -971,7 +982,7 @@ struct Dense {
                            (A)a.scale, a.activation};
     if constexpr (sizeof(T) > 2) {
       if (thin(a)) {
-        if (launch) a.n_out <= 16 ? thin_forward<1>(a, e) : thin_forward<2>(a, e);
+        if (launch) a.n_out <= 16 ? thin_forward<1>(a, e) : a.n_out <= 32 ? thin_forward<2>(a, e) : thin_forward<3>(a, e);
         return;
       }
     }
