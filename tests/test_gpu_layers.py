@@ -113,11 +113,11 @@ def test_dense_writes_its_rows_only(layers, dtype, across):
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
 def test_dense_keeps_what_is_not_finite_in_its_row(layers, dtype):
     """Infinities and NaN reach their own row of y and dx, and nothing else; what lies behind a view's columns reaches nothing."""
-    whole = torch.full((40, 64), float("nan"), dtype=dtype, device="cuda")
-    whole[:, :48] = normal((40, 48), dtype, 1)
-    kernel = torch.full((48, 80), float("nan"), dtype=dtype, device="cuda")
-    kernel[:, :52] = normal((48, 52), dtype, 2, 0.2)
-    for width in (48, 45):
+    whole = torch.full((40, 320), float("nan"), dtype=dtype, device="cuda")
+    kernel = torch.full((304, 80), float("nan"), dtype=dtype, device="cuda")
+    for width in (304, 301, 130, 48, 45, 7):
+        whole[:, :width], kernel[:width, :52] = normal((40, width), dtype, 1), normal((width, 52), dtype, 2, 0.2)
+        whole[:, width:], kernel[width:] = float("nan"), float("nan")
         x, k = whole[:, :width].clone(), kernel[:width, :52]
         clean = layers.dense(whole[:, :width], k, activation="silu")
         assert bool(torch.isfinite(clean).all())

@@ -165,7 +165,6 @@ struct Product {
   const void* q;
   int64_t ldp, ldq;
   int32_t m, n, k;
-  int32_t kp, kq;          // what P and Q hold along k (k may be rounded up to whole chunks; what lies behind is zero)
 };
 
 typedef short short8 __attribute__((ext_vector_type(8)));
@@ -218,7 +217,7 @@ template <> struct Matrix<double> {
 // One operand's tile, R rows x one step of k, 16-byte chunks straight from memory into LDS.  Along k: [row][8 chunks], chunk c of row r at
 // place c ^ (r & 7).  Across: [k][chunks of R rows], chunk c of line k at place c ^ swizzle(k); there a lane gathers its k line by line, by the
 // transposing LDS read for the 16-bit types.  The places are permuted on the memory side (a lane fetches the chunk that belongs where it
-// writes), so that the fragment reads of a wave fall on different banks.
+// writes), so that the fragment reads of a wave fall on different banks.  Memory addresses are multiples of four bytes.
 template <typename T, int R, bool ACROSS, int THREADS>
 struct Tile {
   typedef typename Matrix<T>::Frag Frag;
@@ -288,6 +287,15 @@ struct Tile {
     left -= step;
   }
 
+  // A chunk that a row along k ends in also brought what lies behind the row: zeros there.  `k` of the step's k are inside.
+  static __device__ __forceinline__ void trim(char* tile, int k) {
+    if constexpr (!ACROSS)
+      for (int r = threadIdx.x; r < R; r += THREADS) {
+        T* chunk = reinterpret_cast<T*>(tile + r * LINE + (((k / E) ^ (r & 7)) << 4));
+        for (int e = k % E; e < E; ++e) chunk[e] = (T)0;
+      }
+  }
+
   // rows row_w + 16 t .. + 16, half s of the step's k
   __device__ __forceinline__ Frag fragment(const lds_char* tile, int t, int s) const {
     if constexpr (!ACROSS) {
@@ -323,8 +331,8 @@ __device__ __forceinline__ void tile_product(const Product& g, int row0, int col
   const int wr = (wave / WN) * TM * 16, wc = (wave % WN) * TN * 16;
   P p;
   Q q;
-  p.init(g.p, g.ldp, g.m, min(k_end, g.kp), row0, k_begin, wr);
-  q.init(g.q, g.ldq, g.n, min(k_end, g.kq), col0, k_begin, wc);
+  p.init(g.p, g.ldp, g.m, k_end, row0, k_begin, wr);
+  q.init(g.q, g.ldq, g.n, k_end, col0, k_begin, wc);
   Acc acc[TM][TN];
 #pragma unroll
   for (int a = 0; a < TM; ++a)
@@ -369,9 +377,17 @@ __device__ __forceinline__ void tile_product(const Product& g, int row0, int col
     constexpr int FETCHES = P::LOADS + Q::LOADS;
     const int steps = (k_end - k_begin + STEP - 1) / STEP;
     int k_left = k_end - k_begin, now = 0;
+    const int last = k_left - (steps - 1) * STEP;        // of the last step
+    auto trim = [&](int buffer) {
+      P::trim(tiles + buffer, last);
+      Q::trim(tiles + buffer + P::BYTES, last);
+      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    };
+    const bool ragged = (!PX || !QX) && last % P::E != 0;
     for (int s = 0; s < STAGES && s < steps; ++s) fetch(s * BUFFER, k_left - s * STEP);
     if (steps >= STAGES) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((STAGES - 1) * FETCHES) : "memory");
     else asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+    if (ragged && steps == 1) trim(0);
     read(lds, 0, p0, q0);
     for (int left = steps - 1; left > 0; --left) {
       read(lds + now, 1, p1, q1);
@@ -383,6 +399,7 @@ __device__ __forceinline__ void tile_product(const Product& g, int row0, int col
       if (left >= STAGES) fetch(now, k_left - STAGES * STEP);
       k_left -= STEP;
       now = now + BUFFER == STAGES * BUFFER ? 0 : now + BUFFER;
+      if (ragged && left == 1) trim(now);
       read(lds + now, 0, p0, q0);
       multiply(p1, q1);
       interleave();
@@ -864,11 +881,11 @@ struct Lines {
   int64_t lines, n, ld;
 };
 
-// Whether the products can fetch it: 16-byte chunks at 16-byte addresses, and whole chunks where its lines lie along k.  What they cannot is
-// copied into lines of whole chunks first, zeros behind each line's end.
+// Whether the products can fetch it: lines at multiples of four bytes (every fp32 and fp64 operand, 16-bit ones of an even pitch).  What they cannot is
+// copied into lines of whole 16-byte chunks first.
 template <typename T>
-bool fetchable(const Lines& o, bool along_k) {
-  return aligned16(o.p) && o.ld % vec_of<T>() == 0 && (!along_k || o.n % vec_of<T>() == 0);
+bool fetchable(const Lines& o) {
+  return reinterpret_cast<uintptr_t>(o.p) % 4 == 0 && o.ld * (int64_t)sizeof(T) % 4 == 0;
 }
 
 template <typename T>
@@ -915,22 +932,21 @@ struct Dense {
   }
 
   // an operand that the products can fetch
-  Lines ready(Lines o, bool along_k) {
-    if (fetchable<T>(o, along_k)) return o;
+  Lines ready(Lines o) {
+    if (fetchable<T>(o)) return o;
     const int64_t ld = round_up(o.n, vec_of<T>());
     Job<T> b = job_of(o);
     b.to = static_cast<T*>(take(o.lines * ld * (int64_t)sizeof(T)));
     b.ld_to = ld;
     shape(b, ld);
     if (o.lines) add(b);
-    return {b.to, o.lines, along_k ? ld : o.n, ld};
+    return {b.to, o.lines, o.n, ld};
   }
 
-  void multiply(Lines p, bool p_across, Lines q, bool q_across, int64_t m, int64_t n, int64_t k, const Epilogue<T>& e) {
-    const int64_t kp = p_across ? p.lines : p.n, kq = q_across ? q.lines : q.n, k_all = std::max(k, std::max(kp, kq));
-    const int64_t bytes = product_bytes<T>(m, n, k_all);
+  void multiply(const Lines& p, bool p_across, const Lines& q, bool q_across, int64_t m, int64_t n, int64_t k, const Epilogue<T>& e) {
+    const int64_t bytes = product_bytes<T>(m, n, k);
     void* rest = bytes ? take(bytes) : nullptr;
-    if (launch) product<T>({p.p, q.p, p.ld, q.ld, (int32_t)m, (int32_t)n, (int32_t)k_all, (int32_t)kp, (int32_t)kq}, p_across, q_across, e, rest, stream);
+    if (launch) product<T>({p.p, q.p, p.ld, q.ld, (int32_t)m, (int32_t)n, (int32_t)k}, p_across, q_across, e, rest, stream);
     used -= round_up(bytes, 256);
   }
 
@@ -986,7 +1002,7 @@ struct Dense {
         return;
       }
     }
-    const Lines x = ready({a.x, a.rows, a.n_in, a.ldx}, true), kernel = ready(kernel_lines(a), a.kernel_t);
+    const Lines x = ready({a.x, a.rows, a.n_in, a.ldx}), kernel = ready(kernel_lines(a));
     launch_jobs();
     multiply(x, false, kernel, !a.kernel_t, a.rows, a.n_out, a.n_in, e);
   }
@@ -1001,7 +1017,7 @@ struct Dense {
     }
     const Lines dy = {a.dy, a.rows, a.n_out, a.ldd};
     Lines dz = dy;
-    const bool own = (a.dx || a.dkernel) && (a.slope || a.scale != 1.0 || !fetchable<T>(dy, a.dx));
+    const bool own = (a.dx || a.dkernel) && (a.slope || a.scale != 1.0 || !fetchable<T>(dy));
     Job<T> b = job_of(dy);
     if (own) {
       b.ld_to = round_up(a.n_out, vec_of<T>());
@@ -1017,14 +1033,12 @@ struct Dense {
       add(b);
     }
     const bool want_x = a.dx && a.rows;
-    const Lines kernel = want_x ? ready(kernel_lines(a), !a.kernel_t) : Lines(), x = a.dkernel ? ready({a.x, a.rows, a.n_in, a.ldx}, false) : Lines();
+    const Lines kernel = want_x ? ready(kernel_lines(a)) : Lines(), x = a.dkernel ? ready({a.x, a.rows, a.n_in, a.ldx}) : Lines();
     launch_jobs();
     if (launch && b.partial) add_columns<A, T>(b.partial, b.groups, a.n_out, a.n_out, 0, static_cast<T*>(a.dbias), nullptr, stream);
     if (want_x) {
       const Epilogue<T> e = {nullptr, nullptr, 0, static_cast<T*>(a.dx), a.n_in, nullptr, a.n_in, 1, VMCPDE_ACT_NONE};
-      Lines z = dz;
-      if (own) z.n = dz.ld;           // (zeros behind the line's end)
-      multiply(z, false, kernel, a.kernel_t, a.rows, a.n_in, a.n_out, e);
+      multiply(dz, false, kernel, a.kernel_t, a.rows, a.n_in, a.n_out, e);
     }
     if (a.dkernel) {
       const Epilogue<T> e = {nullptr, nullptr, 0, static_cast<T*>(a.dkernel), a.n_out, nullptr, a.n_out, 1, VMCPDE_ACT_NONE};
