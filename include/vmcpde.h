@@ -11,7 +11,8 @@
  *     all buffers including the explicit workspaces; nothing here allocates per call, nothing synchronises the
  *     host, every launch goes to the hipStream_t passed as `stream` (void* so that no HIP header is needed).
  *   - return value 0 = success, <0 = error; vmcpde_last_error() gives a thread-local message.
- *   - all arithmetic is IEEE fp64 (reference: global_defs.py:8 tReal = float64, main.py:2 jax_enable_x64).
+ *   - all arithmetic is IEEE fp64 (reference: global_defs.py:8 tReal = float64, main.py:2 jax_enable_x64); the layer operators at the
+ *     end take fp32, fp16 and bf16 elements as well.
  *   - sample arrays are row-major [N][d]; the per-sample parameter Jacobian is stored PARAMETER-MAJOR:
  *     JT[p * ldj + n] = d logp(x_n) / d theta_p  (the reference's (1,N,P) array is a strided view of it).
  */
@@ -423,7 +424,8 @@ int vmcpde_sytrd_medium(const double* T, int64_t ldt, int32_t n, double* D, doub
 /* What a fit of a wide conditioner is made of, beside the flow kernels (whose networks live in LDS): net.py:53-61 is a chain of dense
  * layers, var_state.py:45-53 hands out the gradient of a likelihood fit.  Element types of these entry points; every other one is fp64.
  * Sums, statistics and epilogues are held in fp32 for fp32 and 16-bit elements, in fp64 for fp64.  Row pitches count elements; a row's
- * elements lie behind each other.  Nothing needs to be aligned beyond its elements. */
+ * elements lie behind each other.  Nothing needs to be aligned beyond its elements.  No output may overlap an input or another output,
+ * except where clipping is said to run in place. */
 enum { VMCPDE_F64 = 0, VMCPDE_F32 = 1, VMCPDE_F16 = 2, VMCPDE_BF16 = 3 };
 enum { VMCPDE_ACT_NONE = 0, VMCPDE_ACT_TANH = 1, VMCPDE_ACT_GELU = 2 /* z Phi(z), the exact form */, VMCPDE_ACT_SILU = 3 };
 
@@ -431,8 +433,9 @@ enum { VMCPDE_ACT_NONE = 0, VMCPDE_ACT_TANH = 1, VMCPDE_ACT_GELU = 2 /* z Phi(z)
  * stored [n_out][n_in] with kernel_t != 0.  b, r, slope may be NULL.  slope [rows][n_out] receives act'(x W + b) for the backward pass:
  * fp16 for bf16, fp32 for fp16, else the element type.
  * Backward, with dz = scale * slope * dy (slope NULL: 1):  dx = dz W^T [rows][n_in], dkernel = x^T dz [n_in][n_out] (this order whatever
- * kernel_t), dbias = sum of dz over the rows; each may be NULL = not wanted, x may be NULL without dkernel, kernel without dx.  The residual's gradient is dy.  dz is rounded
- * to the element type, in which the matrix pipe takes it; sums are fp32 / fp64.  No atomics: the same call gives the same bits. */
+ * kernel_t), dbias = sum of dz over the rows; each may be NULL = not wanted, x may be NULL without dkernel, kernel without dx.  The
+ * residual's gradient is dy.  dz is rounded to the element type, in which the matrix pipe takes it; sums are fp32 / fp64.  No atomics:
+ * the same call gives the same bits.  Rows below 2^30, widths and pitches below 2^22 (2^21 in fp64). */
 typedef struct {
   int32_t dtype, activation, kernel_t, reserved;
   int64_t rows, n_in, n_out;
@@ -452,7 +455,8 @@ int vmcpde_dense_backward(const vmcpde_dense_args* args, void* workspace, int64_
 
 /* Layer norm of the rows of x [rows][cols]: y = (x - mean) * rstd * weight + bias, rstd = 1 / sqrt(variance + eps) (variance over cols, not
  * cols - 1).  weight, bias may be NULL; they have the element type, or fp32 beside 16-bit elements.  mean, rstd [rows] (fp32, fp64 for fp64)
- * are written by the forward pass where given and read by the backward pass:  dx, dweight, dbias, each may be NULL = not wanted. */
+ * are written by the forward pass where given and read by the backward pass:  dx, dweight, dbias, each may be NULL = not wanted.
+ * Rows below 2^31 (2^22 of rows longer than 16384, in fp64 4096, elements), columns below 2^27. */
 typedef struct {
   int32_t dtype, weight_dtype;
   int64_t rows, cols;

@@ -310,6 +310,23 @@ def test_layer_norm_beyond_32_bits(layers):
     assert torch.equal(dx[0].expand(5, 8192), dx[-8:-3])
 
 
+@pytest.mark.parametrize("dtype, weights, size", [(torch.bfloat16, torch.float32, (4500000, 3)), (torch.float64, torch.float64, (3001, 1)), (torch.float32, torch.float32, (70001, 3)),
+                                                  (torch.float16, torch.float16, (257, 7)), (torch.bfloat16, torch.bfloat16, (1025, 4))],
+                         ids=lambda v: "x".join(map(str, v)) if isinstance(v, tuple) else None)
+def test_layer_norm_of_rows_shorter_than_a_vector(layers, dtype, weights, size):
+    rows, cols = size
+    x, dy = normal((rows, cols + 2), dtype, 1)[:, 1:1 + cols], normal((rows, cols + 1), dtype, 2)[:, :cols]
+    weight, bias = normal((cols,), weights, 3), normal((cols,), weights, 4)
+    y, mean, rstd = layers.layer_norm(x, weight, bias, eps=1e-3, want_stats=True)
+    grads = layers.layer_norm_backward(dy, x, mean, rstd, weight)
+    want = plain.layer_norm(x, weight, bias, 1e-3, dy, dtype, weights)
+    for name, got in (("y", y), ("mean", mean), ("rstd", rstd), ("dx", grads[0]), ("dweight", grads[1]), ("dbias", grads[2])):
+        plain.agrees(got, want[name], name)
+    for k in range(3):
+        only = layers.layer_norm_backward(dy, x, mean, rstd, weight, want_x=k == 0, want_weight=k == 1, want_bias=k == 2)
+        assert torch.equal(only[k], grads[k])
+
+
 def test_layer_norm_refuses_shapes(layers):
     x = torch.zeros(3, 4, device="cuda")
     stats = torch.zeros(3, device="cuda")
@@ -384,6 +401,11 @@ def test_global_norm_of_trees_and_layouts(layers):
     for tensors in ([a, a], [a.view(-1)[:20], a.view(-1)[19:]]):
         with pytest.raises(nat.VmcpdeError, match="overlaps"):
             layers.clip_by_global_norm(tensors, 1.0)
+
+
+def test_clipping_nothing(layers):
+    for tensors in ([torch.empty(0, device="cuda")], [torch.empty((3, 0), device="cuda", dtype=torch.bfloat16)] * 200):
+        assert float(layers.global_norm(tensors)) == 0 and float(layers.clip_by_global_norm(tensors, 0.0)) == 0
 
 
 def test_both_readers_of_a_list_of_tensors(layers, monkeypatch):

@@ -66,7 +66,8 @@ def test_dense_without_rows_launches_nothing(nat):
 
 
 @pytest.mark.parametrize("changed", [dict(dtype=7), dict(weight_dtype=F64), dict(dtype=F32, weight_dtype=BF16), dict(dtype=F64, weight_dtype=F32), dict(weight_dtype=F16),
-                                     dict(rows=-1), dict(rows=1 << 31), dict(cols=0), dict(x=None), dict(ldx=4)])
+                                     dict(rows=-1), dict(rows=1 << 31), dict(cols=0), dict(x=None), dict(ldx=4), dict(cols=1 << 27, ldx=1 << 27),
+                                     dict(rows=1 << 22, cols=16385, ldx=16385), dict(rows=1 << 22, dtype=F64, weight_dtype=F64, cols=4097, ldx=4097)])
 def test_layer_norm_refuses(nat, changed):
     L, a = nat.lib(), norm_args(nat, **changed)
     assert L.vmcpde_layer_norm(a, None) == -1 and b"layer norm" in L.vmcpde_last_error()
