@@ -424,7 +424,7 @@ int vmcpde_sytrd_medium(const double* T, int64_t ldt, int32_t n, double* D, doub
 /* What a fit of a wide conditioner is made of, beside the flow kernels (whose networks live in LDS): net.py:53-61 is a chain of dense
  * layers, var_state.py:45-53 hands out the gradient of a likelihood fit.  Element types of these entry points; every other one is fp64.
  * Sums, statistics and epilogues are held in fp32 for fp32 and 16-bit elements, in fp64 for fp64.  Row pitches count elements; a row's
- * elements lie behind each other.  Nothing needs to be aligned beyond its elements.  No output may overlap an input or another output,
+ * elements lie behind each other.  Nothing needs to be aligned beyond its elements, but workspaces to 16 bytes.  No output may overlap an input or another output,
  * except where clipping is said to run in place. */
 enum { VMCPDE_F64 = 0, VMCPDE_F32 = 1, VMCPDE_F16 = 2, VMCPDE_BF16 = 3 };
 enum { VMCPDE_ACT_NONE = 0, VMCPDE_ACT_TANH = 1, VMCPDE_ACT_GELU = 2 /* z Phi(z), the exact form */, VMCPDE_ACT_SILU = 3 };

@@ -94,11 +94,33 @@ def test_dense_takes_views(layers, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("rows", [1, 2, 3, 4, 7, 8])
+def test_dense_of_few_rows(layers, dtype, rows):
+    """A token or a handful of them, either layout, odd widths and pitches, with and without slices of k: the forward pass and dx."""
+    for number, (n_in, n_out) in enumerate([(1, 8), (7, 9), (63, 65), (64, 200), (129, 71), (515, 1003), (5000, 40), (9001, 50), (2100, 17)]):
+        act, scale = ACTS[(number + rows) % 4], (1.0, 10.0, -0.5)[number % 3]
+        x, dy = normal((rows, n_in + 1), dtype, 10 * number)[:, 1:], normal((rows, n_out + 3), dtype, 10 * number + 4)[:, 2:2 + n_out]
+        bias, residual = normal((n_out,), dtype, 10 * number + 2, 0.3), normal((rows, n_out), dtype, 10 * number + 3) if number % 2 else None
+        for kernel in (normal((n_in, n_out + number % 3), dtype, 10 * number + 1, n_in ** -0.5)[:, number % 3:],
+                       normal((n_out, n_in + number % 2), dtype, 10 * number + 5, n_in ** -0.5)[:, number % 2:].t()):
+            y, slope = layers.dense(x, kernel, bias, activation=act, scale=scale, residual=residual, want_slope=True)
+            dx, _, _ = layers.dense_backward(dy, x, kernel, slope, scale=scale, want_kernel=False, want_bias=False)
+            want = plain.dense(x, kernel, bias, residual, act, scale, dy, dtype)
+            for name, got in (("y", y), ("slope", slope), ("dx", dx)):
+                if got is not None:
+                    plain.agrees(got, want[name], name)
+            if rows * n_in >= 64:
+                plain.near(dx, want["dx"], 3 if dtype in (torch.float16, torch.bfloat16) else 40, dtype, "dx")
+            assert torch.equal(layers.dense(x.contiguous(), kernel.clone(), bias, activation=act, scale=scale, residual=residual), y)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
 @pytest.mark.parametrize("across", [0, 1])
-def test_dense_writes_its_rows_only(layers, dtype, across):
+@pytest.mark.parametrize("rows", [3, 37])
+def test_dense_writes_its_rows_only(layers, dtype, across, rows):
     """A target with a row pitch: what lies between and behind the rows stays as it was."""
     from vmc_pde_amd import _native as nat
-    rows, n_in, n_out, pitch = 37, 72, 43, 56
+    n_in, n_out, pitch = 72, 43, 56
     x, kernel = normal((rows, n_in), dtype, 1), normal((n_out, n_in) if across else (n_in, n_out), dtype, 2, 0.1)
     y = torch.full((rows + 3, pitch), -7.0, dtype=dtype, device="cuda")
     a = nat.DenseArgs(layers.DTYPE[dtype], 2, across, 0, rows, n_in, n_out, x.data_ptr(), n_in, kernel.data_ptr(), n_in if across else n_out, None, None, 0, 1.0,

@@ -49,6 +49,7 @@ def test_dense_refuses_a_short_workspace(nat):
     assert need > 0
     assert L.vmcpde_dense(a, HERE, need - 1, None) == -1 and b"workspace" in L.vmcpde_last_error()
     assert L.vmcpde_dense(a, None, need, None) == -1
+    assert L.vmcpde_dense(a, HERE + 8, need, None) == -1 and b"aligned" in L.vmcpde_last_error()
     assert L.vmcpde_dense_workspace_bytes(a, 1) == 0   # dz is dy itself, and four rows' column sums take no partials
     a = dense_args(nat, rows=4, n_in=100000, ldx=100000, slope=HERE)
     need = L.vmcpde_dense_workspace_bytes(a, 1)

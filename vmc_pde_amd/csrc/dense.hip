@@ -492,6 +492,170 @@ __global__ __launch_bounds__(256) void product_join_kernel(const typename Wide<T
   if (row < m) finish<T, 4>(e, row, col, z);
 }
 
+// ---- few rows ------------------------------------------------------------------------------------------------------------------------
+
+// Up to four rows of C (a token, a handful of samples): bound by reading Q once, each number of which is used m times, so the vector units do and the matrix
+// pipe's tiles would be mostly empty.  Q goes from memory to registers, 16 bytes a lane at any alignment and pitch; k is shared by the waves of a workgroup,
+// whose sums are joined in LDS (in their order).  One row, us against the tiles': bf16 4096 x 16384 stored transposed 23.8 / 27.4, 16384 x 4096 30 / 33, 768 x 2304
+// 7.9 / 10.9; fp32 16384 x 4096 47 / 59 (5.7 TB/s), transposed 51 / 69.
+constexpr int FEW_ALONG = 4, FEW_ACROSS = 2, FEW_COLS = 4;      // most rows by Q's layout (across k, four rows' registers leave too few waves: 32 against the tiles' 26 us for 4 x 4096 x 12288)
+template <typename T>
+struct __attribute__((packed, aligned(sizeof(T)))) Packed { T v[vec_of<T>()]; };
+template <typename T>
+struct __attribute__((packed, aligned(sizeof(T)))) Eight { T v[8]; };
+
+// Q across k: ALONG lanes along a line, 64 / ALONG of them along k, eight lines each at a time.  32 lanes (512 bytes of a line) reach 5.6 TB/s, eight (128
+// bytes) 4.6, but make four times the workgroups, and where those suffice no second launch is needed.
+template <typename T, int M, int ALONG>
+__global__ __launch_bounds__(512) void few_across_kernel(Product g, int k_slice, typename Wide<T>::type* __restrict__ part, Epilogue<T> e) {
+  typedef typename Wide<T>::type A;
+  constexpr int V = vec_of<T>(), WAVES = 8, COLS = ALONG * V, CHUNK = 64 / ALONG * 8;
+  constexpr bool X_AHEAD = M * (int)sizeof(T) <= 8;      // (registers)
+  __shared__ A sh[WAVES][M][COLS];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane % ALONG, s = lane / ALONG;
+  const int col = blockIdx.x * COLS + i * V, from = min(col, g.n - V);             // (a vector that passes the end is moved back: the same sums twice)
+  const int k_begin = blockIdx.y * k_slice, k_end = min(k_begin + k_slice, g.k);
+  const T* q = static_cast<const T*>(g.q) + from;
+  const T* p = static_cast<const T*>(g.p);
+  A acc[M][V];
+#pragma unroll
+  for (int m = 0; m < M; ++m)
+#pragma unroll
+    for (int c = 0; c < V; ++c) acc[m][c] = 0;
+  Packed<T> w[8], w_next[8];
+  Eight<T> x[M], x_next[M];
+  auto fetch = [&](int k0) {
+    const T* at = q + (int64_t)(k0 + s * 8) * g.ldq;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) w_next[u] = *reinterpret_cast<const Packed<T>*>(at + u * g.ldq);
+  };
+  auto fetch_x = [&](int k0) {
+#pragma unroll
+    for (int m = 0; m < M; ++m) x_next[m] = *reinterpret_cast<const Eight<T>*>(p + min(m, g.m - 1) * g.ldp + k0 + s * 8);
+  };
+  auto add = [&](int u, const Packed<T>& line, const A (&xk)[M]) {
+#pragma unroll
+    for (int c = 0; c < V; ++c) {
+      const A v = (A)line.v[c];
+#pragma unroll
+      for (int m = 0; m < M; ++m) acc[m][c] = fma(xk[m], v, acc[m][c]);
+    }
+  };
+  int k0 = k_begin + wave * CHUNK;
+  if (k0 + CHUNK <= k_end) {
+    if (X_AHEAD) fetch_x(k0);
+    fetch(k0);
+  }
+  for (; k0 + CHUNK <= k_end; k0 += WAVES * CHUNK) {
+#pragma unroll
+    for (int u = 0; u < 8; ++u) w[u] = w_next[u];
+    if (!X_AHEAD) fetch_x(k0);
+#pragma unroll
+    for (int m = 0; m < M; ++m) x[m] = x_next[m];
+    if (k0 + (WAVES + 1) * CHUNK <= k_end) {
+      if (X_AHEAD) fetch_x(k0 + WAVES * CHUNK);
+      fetch(k0 + WAVES * CHUNK);
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      A xk[M];
+#pragma unroll
+      for (int m = 0; m < M; ++m) xk[m] = (A)x[m].v[u];
+      add(u, w[u], xk);
+    }
+  }
+  if (k0 < k_end)                                                                // the last, partial chunk
+    for (int k = k0 + s * 8; k < min(k0 + s * 8 + 8, k_end); ++k) {
+      A xk[M];
+#pragma unroll
+      for (int m = 0; m < M; ++m) xk[m] = (A)p[min(m, g.m - 1) * g.ldp + k];
+      add(0, *reinterpret_cast<const Packed<T>*>(q + k * g.ldq), xk);
+    }
+#pragma unroll
+  for (int m = 0; m < M; ++m)
+#pragma unroll
+    for (int c = 0; c < V; ++c) {
+      A v = acc[m][c];
+#pragma unroll
+      for (int d = ALONG; d < 64; d *= 2) v += __shfl_xor(v, d);
+      if (s == 0) sh[wave][m][i * V + c] = v;
+    }
+  __syncthreads();
+  for (int u = threadIdx.x; u < M * ALONG; u += 64 * WAVES) {
+    const int m = u / ALONG, j = u % ALONG, nominal = blockIdx.x * COLS + j * V;
+    if (m >= g.m || nominal >= g.n) continue;
+    A z[V];
+#pragma unroll
+    for (int c = 0; c < V; ++c) z[c] = sh[0][m][j * V + c];
+    for (int w = 1; w < WAVES; ++w)
+#pragma unroll
+      for (int c = 0; c < V; ++c) z[c] += sh[w][m][j * V + c];
+    const int to = min(nominal, g.n - V);
+    if (part) store_vec<A, V>(part + ((int64_t)blockIdx.y * g.m + m) * g.n, to, g.n, z);
+    else finish<T, V>(e, m, to, z);
+  }
+}
+
+// Q along k, the lanes too: a wave takes four columns, and SPLIT of a workgroup's four waves share them.
+template <typename T, int M, int SPLIT>
+__global__ __launch_bounds__(256) void few_along_kernel(Product g, int k_slice, typename Wide<T>::type* __restrict__ part, Epilogue<T> e) {
+  typedef typename Wide<T>::type A;
+  constexpr int V = vec_of<T>(), COLS = FEW_COLS, CHUNK = 64 * SPLIT * V;
+  __shared__ A sh[4][M][COLS];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col0 = (blockIdx.x * (4 / SPLIT) + wave / SPLIT) * COLS;
+  const int k_begin = blockIdx.y * k_slice, k_end = min(k_begin + k_slice, g.k);
+  const T* p = static_cast<const T*>(g.p);
+  const T* q = static_cast<const T*>(g.q);
+  A acc[M][COLS];
+#pragma unroll
+  for (int m = 0; m < M; ++m)
+#pragma unroll
+    for (int c = 0; c < COLS; ++c) acc[m][c] = 0;
+  auto row = [&](int m) { return p + min(m, g.m - 1) * g.ldp; };                  // (rows and columns that are not there: the last one again)
+  auto line = [&](int c) { return q + min(col0 + c, g.n - 1) * g.ldq; };
+#pragma unroll 2
+  for (int k = k_begin + (threadIdx.x % (64 * SPLIT)) * V; k < k_end; k += CHUNK) {
+    if (k + V <= k_end) {
+      Packed<T> w[COLS], x[M];
+#pragma unroll
+      for (int c = 0; c < COLS; ++c) w[c] = *reinterpret_cast<const Packed<T>*>(line(c) + k);
+#pragma unroll
+      for (int m = 0; m < M; ++m) x[m] = *reinterpret_cast<const Packed<T>*>(row(m) + k);
+#pragma unroll
+      for (int u = 0; u < V; ++u)
+#pragma unroll
+        for (int m = 0; m < M; ++m)
+#pragma unroll
+          for (int c = 0; c < COLS; ++c) acc[m][c] = fma((A)x[m].v[u], (A)w[c].v[u], acc[m][c]);
+    } else {
+      for (int j = k; j < k_end; ++j)
+#pragma unroll
+        for (int m = 0; m < M; ++m)
+#pragma unroll
+          for (int c = 0; c < COLS; ++c) acc[m][c] = fma((A)row(m)[j], (A)line(c)[j], acc[m][c]);
+    }
+  }
+#pragma unroll
+  for (int m = 0; m < M; ++m)
+#pragma unroll
+    for (int c = 0; c < COLS; ++c) {
+      const A v = group_sum<64>(acc[m][c]);
+      if (lane == 0) sh[wave][m][c] = v;
+    }
+  __syncthreads();
+  const int m = threadIdx.x % (64 * SPLIT);                                        // the first wave of those that share the columns
+  if (m >= g.m || col0 >= g.n) return;
+  A z[COLS];
+#pragma unroll
+  for (int c = 0; c < COLS; ++c) z[c] = sh[wave][m][c];
+#pragma unroll
+  for (int w = 1; w < SPLIT; ++w)
+#pragma unroll
+    for (int c = 0; c < COLS; ++c) z[c] += sh[wave + w][m][c];
+  if (part) store_vec<A, COLS>(part + ((int64_t)blockIdx.y * g.m + m) * g.n, col0, g.n, z);
+  else finish<T, COLS>(e, m, col0, z);
+}
+
 // ---- what is made ready before the products --------------------------------------------------------------------------------------------
 
 // Up to three copies in one launch: lines of n elements to lines of ld_to (zeros behind n), scaled by scale * slope: an operand into lines that the
@@ -841,9 +1005,53 @@ Tiles tiles_of(int64_t m, int64_t n, int64_t steps) {
   return best;
 }
 
+// Whether, for at most 32 rows of 16-bit numbers and a kernel across k, tiles 64 wide in one launch beat slices and a second launch: with a workgroup a CU a step
+// takes 0.32 us (8 x 4096 x 16384: 26 us against 30), slices reach 5.4 TB/s.  (fp32's and fp64's steps hold half the k and more.)
 template <typename T>
-int64_t product_bytes(int64_t m, int64_t n, int64_t k) {
-  const Tiles t = tiles_of<T>(m, n, ceil_div(k, step_of<T>()));
+bool one_launch(int64_t n, int64_t k) {
+  return sizeof(T) == 2 && n > 32 && n <= 64 * 256 && 0.32 * ceil_div(k, step_of<T>()) < (double)n * k * sizeof(T) / 5.4e6 + 4.5;
+}
+
+// Products that the kernels for few rows take, in any layout of their operands.  `fetchable`: the tiles could take q as it lies.
+template <typename T>
+bool few(int64_t m, int64_t n, int64_t k, bool q_across, bool fetchable) {
+  return m >= 1 && m <= (q_across ? FEW_ACROSS : FEW_ALONG) && n >= vec_of<T>() && !(q_across && fetchable && one_launch<T>(n, k));
+}
+
+// Their plan: bm = 0, bn = the lanes along a line (Q across k), slice_steps = a slice's k.  A CU gets 34 GB/s at most, all of them together 5.6 TB/s (28, 4.6 with eight lanes); slices of k
+// spread a product of few columns over the CUs, evenly, and cost a second launch (4.5 us) and their bytes.
+template <typename T>
+Tiles few_plan(int64_t m, int64_t n, int64_t k, bool across) {
+  const double bytes = (double)n * k * sizeof(T);
+  int64_t slices = 1;
+  Tiles best = {0, 32, 1, 0};
+  double shortest = INFINITY;
+  for (const int lanes : {32, 8}) {
+    if (!across && lanes != 32) break;
+    const int64_t groups = ceil_div(n, across ? lanes * vec_of<T>() : FEW_COLS), least = across ? 256 : 2048;
+    const double rate = across && lanes == 8 ? 4.6e6 : 5.6e6;
+    for (int64_t s = 1; s <= std::max<int64_t>(1, std::min<int64_t>(k / least, 64)); ++s) {
+      const double all = (double)groups * s, on_one = std::ceil(all / 256);
+      const double time = bytes / all * on_one / std::min(lanes == 8 ? 28e3 : 34e3, rate / std::min(all, 256.0)) +
+                          (s > 1 ? 4.5 + (double)s * m * n * 2 * sizeof(typename Wide<T>::type) / 4e6 : 0);
+      if (time < shortest) shortest = time, slices = s, best.bn = lanes;
+    }
+  }
+  best.slice_steps = (int)round_up(ceil_div(k, slices), 64);
+  best.slices = (int)ceil_div(k, best.slice_steps);
+  return best;
+}
+
+template <typename T>
+Tiles plan_of(int64_t m, int64_t n, int64_t k, bool p_across, bool q_across, bool few_rows) {
+  if (few_rows) return few_plan<T>(m, n, k, q_across);
+  const int64_t steps = ceil_div(k, step_of<T>());
+  if (m <= 32 && !p_across && q_across && one_launch<T>(n, k)) return {32, 64, 1, (int)std::max<int64_t>(1, steps)};
+  return tiles_of<T>(m, n, steps);
+}
+
+template <typename T>
+int64_t product_bytes(const Tiles& t, int64_t m, int64_t n) {
   return t.slices > 1 ? round_up((int64_t)t.slices * m * n * (int64_t)sizeof(typename Wide<T>::type), 256) : 0;
 }
 
@@ -856,19 +1064,39 @@ void product_as(const Product& g, bool p_across, bool q_across, const Tiles& t, 
   else product_kernel<T, BM, BN, WM, WN, false, false><<<grid, 64 * WM * WN, 0, s>>>(g, tiles_m, tiles_n, t.slice_steps * step_of<T>(), part, e);
 }
 
+template <typename T, int M>
+void product_few(const Product& g, bool q_across, const Tiles& t, typename Wide<T>::type* part, const Epilogue<T>& e, hipStream_t s) {
+  const unsigned slices = (unsigned)t.slices;
+  if (q_across) {
+    if constexpr (M <= FEW_ACROSS) {
+      if (t.bn == 32) few_across_kernel<T, M, 32><<<dim3((unsigned)ceil_div(g.n, 32 * vec_of<T>()), slices), 512, 0, s>>>(g, t.slice_steps, part, e);
+      else few_across_kernel<T, M, 8><<<dim3((unsigned)ceil_div(g.n, 8 * vec_of<T>()), slices), 512, 0, s>>>(g, t.slice_steps, part, e);
+    }
+  } else if (g.k < 256 * vec_of<T>()) few_along_kernel<T, M, 1><<<dim3((unsigned)ceil_div(g.n, 4 * FEW_COLS), slices), 256, 0, s>>>(g, t.slice_steps, part, e);   // (four waves do not fill one turn)
+  else few_along_kernel<T, M, 4><<<dim3((unsigned)ceil_div(g.n, FEW_COLS), slices), 256, 0, s>>>(g, t.slice_steps, part, e);
+}
+
 template <typename T>
-void product(const Product& g, bool p_across, bool q_across, const Epilogue<T>& e, void* workspace, hipStream_t s) {
+void product(const Product& g, bool p_across, bool q_across, const Tiles& t, const Epilogue<T>& e, void* workspace, hipStream_t s) {
   typedef typename Wide<T>::type A;
-  const Tiles t = tiles_of<T>(g.m, g.n, ceil_div(g.k, step_of<T>()));
   A* part = t.slices > 1 ? static_cast<A*>(workspace) : nullptr;
+  if (t.bm == 0) {
+    if (g.m == 1) product_few<T, 1>(g, q_across, t, part, e, s);
+    else if (g.m == 2) product_few<T, 2>(g, q_across, t, part, e, s);
+    else product_few<T, 4>(g, q_across, t, part, e, s);
+  }
   if constexpr (sizeof(T) == 2) {
     if (t.bm == 256) product_as<T, 256, 256, 2, 4>(g, p_across, q_across, t, part, e, s);
     if (t.bm == 128 && t.bn == 128) product_as<T, 128, 128, 2, 2>(g, p_across, q_across, t, part, e, s);
+    if (t.bm == 32 && t.bn == 64) {
+      const int tiles = (int)ceil_div(g.n, 64);
+      product_kernel<T, 32, 64, 1, 4, false, true><<<tiles, 256, 0, s>>>(g, 1, tiles, t.slice_steps * step_of<T>(), nullptr, e);
+    }
   }
   if (t.bm == 64) product_as<T, 64, 64, 2, 2>(g, p_across, q_across, t, part, e, s);
   else if (t.bm == 128 && t.bn == 32) product_as<T, 128, 32, 4, 1>(g, p_across, q_across, t, part, e, s);
   else if (t.bm == 32 && t.bn == 128) product_as<T, 32, 128, 1, 4>(g, p_across, q_across, t, part, e, s);
-  else if (t.bm == 32) product_as<T, 32, 32, 2, 2>(g, p_across, q_across, t, part, e, s);
+  else if (t.bm == 32 && t.bn == 32) product_as<T, 32, 32, 2, 2>(g, p_across, q_across, t, part, e, s);
   if (!part) return;
   const int64_t lanes = (int64_t)g.m * ((g.n + 3) / 4);
   if (t.slices > 16) product_join_kernel<T, 32><<<(unsigned)ceil_div(lanes, 8), 256, 0, s>>>(part, t.slices, g.m, g.n, e);
@@ -944,9 +1172,10 @@ struct Dense {
   }
 
   void multiply(const Lines& p, bool p_across, const Lines& q, bool q_across, int64_t m, int64_t n, int64_t k, const Epilogue<T>& e) {
-    const int64_t bytes = product_bytes<T>(m, n, k);
+    const Tiles t = plan_of<T>(m, n, k, p_across, q_across, !p_across && few<T>(m, n, k, q_across, fetchable<T>(q)));
+    const int64_t bytes = product_bytes<T>(t, m, n);
     void* rest = bytes ? take(bytes) : nullptr;
-    if (launch) product<T>({p.p, q.p, p.ld, q.ld, (int32_t)m, (int32_t)n, (int32_t)k}, p_across, q_across, e, rest, stream);
+    if (launch) product<T>({p.p, q.p, p.ld, q.ld, (int32_t)m, (int32_t)n, (int32_t)k}, p_across, q_across, t, e, rest, stream);
     used -= round_up(bytes, 256);
   }
 
@@ -1002,7 +1231,8 @@ struct Dense {
         return;
       }
     }
-    const Lines x = ready({a.x, a.rows, a.n_in, a.ldx}), kernel = ready(kernel_lines(a));
+    Lines x = {a.x, a.rows, a.n_in, a.ldx}, kernel = kernel_lines(a);
+    if (!few<T>(a.rows, a.n_out, a.n_in, !a.kernel_t, fetchable<T>(kernel))) x = ready(x), kernel = ready(kernel);
     launch_jobs();
     multiply(x, false, kernel, !a.kernel_t, a.rows, a.n_out, a.n_in, e);
   }
@@ -1033,7 +1263,9 @@ struct Dense {
       add(b);
     }
     const bool want_x = a.dx && a.rows;
-    const Lines kernel = want_x ? ready(kernel_lines(a)) : Lines(), x = a.dkernel ? ready({a.x, a.rows, a.n_in, a.ldx}) : Lines();
+    Lines kernel = want_x ? kernel_lines(a) : Lines();
+    if (want_x && !few<T>(a.rows, a.n_in, a.n_out, a.kernel_t, fetchable<T>(kernel))) kernel = ready(kernel);
+    const Lines x = a.dkernel ? ready({a.x, a.rows, a.n_in, a.ldx}) : Lines();
     launch_jobs();
     if (launch && b.partial) add_columns<A, T>(b.partial, b.groups, a.n_out, a.n_out, 0, static_cast<T*>(a.dbias), nullptr, stream);
     if (want_x) {
@@ -1104,6 +1336,7 @@ static int run(const vmcpde_dense_args* a, bool backward, void* workspace, int64
   if (!backward && a->rows == 0) return 0;
   const int64_t need = vmcpde_dense_workspace_bytes(a, backward);
   VMC_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), "dense: workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)need);
+  VMC_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "dense: the workspace is not aligned to 16 bytes");
   walk_type(*a, backward, workspace, static_cast<hipStream_t>(stream), true);
   VMC_CHECK_HIP(hipGetLastError());
   return 0;

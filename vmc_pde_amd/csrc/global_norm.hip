@@ -336,6 +336,7 @@ int vmcpde_global_norm(const vmcpde_tensor* tensors, int32_t count, int32_t clip
   }
   const int64_t need = p.groups * (int64_t)sizeof(Bins) + 16;
   VMC_REQUIRE(workspace && workspace_bytes >= need, "vmcpde_global_norm: workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)need);
+  VMC_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "vmcpde_global_norm: the workspace is not aligned to 16 bytes");
   Bins* partial = static_cast<Bins*>(workspace);
   double* factor = reinterpret_cast<double*>(partial + p.groups);
   int rc = for_tables(tensors, count, p, [&](const Table& tab, int64_t before) { squares_kernel<<<tab.groups, THREADS, 0, s>>>(tab, partial + before); });

@@ -637,6 +637,7 @@ int vmcpde_layer_norm_backward(const vmcpde_norm_args* a, void* workspace, int64
   VMC_REQUIRE(a->rows == 0 || (a->dy && a->ldd >= a->cols && a->mean && a->rstd), "vmcpde_layer_norm_backward: null dy, mean or rstd, or a row pitch below the columns");
   if (a->dweight || a->dbias) {
     const int64_t need = vmcpde_layer_norm_backward_workspace_bytes(a);
+    VMC_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "vmcpde_layer_norm_backward: the workspace is not aligned to 16 bytes");
     VMC_REQUIRE(workspace && workspace_bytes >= need, "vmcpde_layer_norm_backward: workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)need);
   } else if (a->rows == 0 || !a->dx) {
     return 0;
