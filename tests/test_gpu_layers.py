@@ -239,6 +239,38 @@ def test_dense_refuses_shapes(layers):
         layers.dense(x, k, scale=float("nan"))
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_native_calls_and_python_agree(layers, dtype, monkeypatch):
+    """Both forms of every operator on plain tensors, views, parameters, no rows, one axis, negated views and whole numbers for floats: the same bits."""
+    from vmc_pde_amd import _native as nat
+    wide, flat = normal((3, 9, 40), dtype, 1), normal((900,), dtype, 2)
+    kernel, bias = normal((24, 17), dtype, 3, 0.2), flat[1:18]
+    views = [wide[..., 3:27], wide[1, :, :24], wide[:, ::2, 16:40], wide[0, 0, :24], wide.transpose(0, 1)[..., :24], wide[..., ::2][..., :20].repeat(1, 1, 2)[..., :24],
+             wide[:0, :, :24], torch.nn.Parameter(wide[0, :, :24].contiguous()), torch._neg_view(wide[0, :, :24].contiguous()), wide[2, :1, 2:26]]
+    kernels = [kernel, kernel.t().contiguous().t(), torch._neg_view(kernel), torch.nn.Parameter(kernel), normal((48, 34), dtype, 4)[::2, ::2]]
+
+    def everything():
+        for x in views:
+            for k in kernels:
+                residual = wide.new_ones((*x.shape[:-1], 17))
+                y, slope = layers.dense(x, k, bias, activation="gelu", scale=2, residual=residual, want_slope=True)
+                yield from (y, slope, layers.dense(x, k), *layers.dense_backward(y, x, k, slope, scale=2), *layers.dense_backward(y, x, k, want_x=False))
+            w, b = flat[5:29], torch._neg_view(flat[100:124])
+            y, mean, rstd = layers.layer_norm(x, w, b, eps=1, want_stats=True)
+            yield from (y, mean, rstd, layers.layer_norm(x, bias=w), *layers.layer_norm_backward(y, x, mean, rstd, w), *layers.layer_norm_backward(y, x, mean, rstd, want_bias=False))
+            copies = [x.detach().clone(), kernel.clone()]
+            yield from (layers.clip_by_global_norm(copies, 1), *copies, layers.global_norm([x, kernel.contiguous()]) if x.is_contiguous() else None)
+
+    with torch.no_grad():
+        native = list(everything())
+        monkeypatch.setattr(nat, "_calls", (None,))
+        for a, b in zip(native, everything()):
+            assert (a is None) == (b is None)
+            assert a is None or a.shape == b.shape and a.dtype == b.dtype and a.stride() == b.stride() and torch.equal(a, b)
+    positive, negative = layers.dense(wide[0, :, :24], kernel), layers.dense(views[8], kernel)
+    assert torch.equal(positive, -negative)
+
+
 # ---- layer norm --------------------------------------------------------------------------------------------------------------------------
 
 NORM_SIZES = [(0, 5), (1, 1), (3, 1), (5, 2), (65, 21), (33, 64), (7, 100), (300, 129), (17, 512), (40, 777), (9, 1025), (66, 2048), (3, 4096), (600, 4099), (5, 8192),
@@ -431,9 +463,9 @@ def test_clipping_nothing(layers):
 
 
 def test_both_readers_of_a_list_of_tensors(layers, monkeypatch):
-    """The native reader and the Python code that it spares the host from: the same table, the same results, the same refusals."""
+    """The native form and the Python code that it spares the host from: the same results, the same refusals."""
     from vmc_pde_amd import _native as nat
-    assert nat.tensor_reader() is not None
+    assert nat.layer_calls() is not None
     tensors = parts([7, 0, 300, 41, 1], DTYPES, 3)
     out = [torch.empty_like(t) for t in tensors]
     nested = [tensors[0], [tensors[1], (tensors[2],)], {"a": tensors[3], "b": tensors[4]}]
@@ -444,7 +476,7 @@ def test_both_readers_of_a_list_of_tensors(layers, monkeypatch):
     parameter = torch.nn.Parameter(tensors[2].clone())
     for native in (True, False):
         if not native:
-            monkeypatch.setattr(nat, "_tensors", (None,))
+            monkeypatch.setattr(nat, "_calls", (None,))
         again = layers.clip_by_global_norm(tensors, 0.1, out=out)
         assert torch.equal(again, first) and all(torch.equal(a, b) for a, b in zip(out, kept))
         for t, o in bad:

@@ -7,6 +7,7 @@ raises ``VmcpdeError`` on a non-zero return code.
 from __future__ import annotations
 
 import ctypes as C
+import importlib.util
 import re
 from pathlib import Path
 
@@ -176,20 +177,23 @@ def lib():
     return _lib
 
 
-_tensors = None
+_calls = None
 
 
-def tensor_reader():
-    """`vmcpde_read_tensors` of csrc/tensor_list.cpp, or None where that library is not built: it only saves the host's time."""
-    global _tensors
-    if _tensors is None:
-        path = LIB_PATH.parent / "libvmcpde_tensors.so"
-        _tensors = (None,)
-        if path.exists():
-            f = C.PyDLL(str(path)).vmcpde_read_tensors
-            f.restype, f.argtypes = _int, [C.py_object, C.py_object, _int, _vp, _i64, _vp]
-            _tensors = (f,)
-    return _tensors[0]
+def layer_calls():
+    """The Python module of csrc/layer_calls.cpp, or None where it is not built or no GPU is there: it only saves the host's time."""
+    global _calls
+    if _calls is None:
+        path, module = _HERE / "_lib" / "vmcpde_layer_calls.so", None
+        if path.exists() and torch.cuda.device_count():
+            spec = importlib.util.spec_from_file_location("vmcpde_layer_calls", path)
+            module = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(module)
+            names = ("vmcpde_dense_workspace_bytes", "vmcpde_dense", "vmcpde_dense_backward", "vmcpde_layer_norm", "vmcpde_layer_norm_backward_workspace_bytes",
+                     "vmcpde_layer_norm_backward", "vmcpde_global_norm_workspace_bytes", "vmcpde_global_norm")
+            module.bind(*(C.cast(getattr(lib(), name), C.c_void_p).value for name in names))
+        _calls = (module,)
+    return _calls[0]
 
 
 def check(rc: int, what: str = ""):

@@ -18,8 +18,8 @@ LIB = LIBDIR / "libvmcpde.so"
 SOURCES = ["model.hip", "flow.hip", "sampler.hip", "gram.hip", "gram_i8.hip", "moments.hip", "solve.hip", "eig.hip", "jacobi.hip", "tridiag.hip", "comm.hip",
            "dense.hip", "layer_norm.hip", "global_norm.hip"]
 HEADERS = [CSRC / "common.hpp", CSRC / "mfma_tile.hpp", CSRC / "gram_order.hpp", CSRC / "wave_ops.hpp", CSRC / "layers.hpp", CSRC / "flow_kernels.inc", PKG.parent / "include" / "vmcpde.h"]
-# host code only, a library of its own: the one that knows torch's tensors (csrc/tensor_list.cpp says why)
-TENSORS_SOURCE, TENSORS_LIB = CSRC / "tensor_list.cpp", LIBDIR / "libvmcpde_tensors.so"
+# host code only, a Python module of its own: what knows torch's tensors (csrc/layer_calls.cpp says why)
+CALLS_SOURCE, CALLS_LIB = CSRC / "layer_calls.cpp", LIBDIR / "vmcpde_layer_calls.so"
 ARCH = "gfx950"
 # per-file flags.  solve.hip: keep MFMA accumulators in VGPRs -- the diagonal-block sweep edits them with VALU instructions between
 # MFMAs, and with the default AGPR form every step pays 40 v_accvgpr moves (measured: the whole factorisation 0.1 ms slower)
@@ -40,20 +40,20 @@ def _stale(target: Path, deps) -> bool:
     return any(Path(d).stat().st_mtime > t for d in deps)
 
 
-def build_tensors(force: bool = False, verbose: bool = False) -> Path:
+def build_calls(force: bool = False, verbose: bool = False) -> Path:
     import sysconfig
 
     import torch
     from torch.utils.cpp_extension import include_paths, library_paths
     LIBDIR.mkdir(exist_ok=True)
-    if force or _stale(TENSORS_LIB, [TENSORS_SOURCE]):
+    if force or _stale(CALLS_LIB, [CALLS_SOURCE, PKG.parent / "include" / "vmcpde.h"]):
         cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-w", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-               *[f"-I{p}" for p in [*include_paths(), sysconfig.get_paths()["include"]]], str(TENSORS_SOURCE), "-o", str(TENSORS_LIB),
+               *[f"-I{p}" for p in [*include_paths(), sysconfig.get_paths()["include"]]], str(CALLS_SOURCE), "-o", str(CALLS_LIB),
                *[f"-L{p}" for p in library_paths()], "-ltorch_python", "-ltorch_cpu", "-lc10"]
         if verbose:
             print(" ".join(cmd), flush=True)
         subprocess.run(cmd, check=True)
-    return TENSORS_LIB
+    return CALLS_LIB
 
 
 def build(force: bool = False, verbose: bool = False, variant: str = "", extra_flags=()) -> Path:
@@ -83,7 +83,7 @@ def build(force: bool = False, verbose: bool = False, variant: str = "", extra_f
             print(" ".join(cmd), flush=True)
         subprocess.run(cmd, check=True)
     if not variant:
-        build_tensors(force, verbose)
+        build_calls(force, verbose)
     return lib
 
 

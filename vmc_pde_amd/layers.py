@@ -8,8 +8,8 @@ a function of its own, and takes no part in torch's automatic differentiation (t
 All run on the current HIP stream, allocate through torch, never synchronise with the host, and can be captured into a graph.  Sums, statistics
 and epilogues are held in fp32 for fp32 and 16-bit elements, in fp64 for fp64.  None uses atomics: the same call gives the same bits.
 
-Small calls are bound by the host: arguments travel as one packed record per call (`vmcpde_dense_args`, `vmcpde_norm_args` of include/vmcpde.h)
-every tensor attribute is read once, and lists of tensors are read by csrc/tensor_list.cpp.
+Small calls are bound by the host, so each function first hands its arguments to its native form (csrc/layer_calls.cpp), which does the call if
+nothing has to be copied or refused.  What follows it here is the whole operator: every layout, and every refusal.
 """
 from __future__ import annotations
 
@@ -32,7 +32,7 @@ _HOST = "the layer operators run on device (HBM) tensors only"
 _pack_dense = struct.Struct("@4i3qPqPqPPqdPqPPqPPP").pack       # vmcpde_dense_args
 _pack_norm = struct.Struct("@2i2qPqPPdPqPPPqPPP").pack          # vmcpde_norm_args
 
-_empty, _device, _stream, _recording = torch.empty, torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream, torch.is_grad_enabled
+_calls, _empty, _device, _stream, _recording = nat.layer_calls, torch.empty, torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream, torch.is_grad_enabled
 _entry = {}
 
 
@@ -89,6 +89,7 @@ def _rows(t, cols, name):
     """(tensor, row pitch) of t as a matrix of `cols` columns whose rows' elements lie behind each other; copied only where no such view exists."""
     if t.dim() == 0 or t.shape[-1] != cols:
         raise ValueError(f"{name} has shape {tuple(t.shape)}: its last axis should have {cols}")
+    t = t.resolve_neg()
     if t.is_contiguous():
         return t, cols
     m = t.reshape(-1, cols)
@@ -109,6 +110,7 @@ def _kernel_layout(kernel):
     n_in, n_out = kernel.shape
     if n_in == 0 or n_out == 0:
         raise ValueError(f"kernel has shape {(n_in, n_out)}: no axis may be empty")
+    kernel = kernel.resolve_neg()
     s0, s1 = kernel.stride()
     if (s1 == 1 or n_out == 1) and (s0 >= n_out or n_in == 1):
         return kernel, n_in, n_out, max(s0, n_out), 0
@@ -124,6 +126,12 @@ def dense(x, kernel, bias=None, *, activation="none", scale=1.0, residual=None, 
     (n_out,); residual of y's shape.  activation: "none", "tanh", "gelu" (z Phi(z)), "silu".  `scale` is the output factor of the reference's
     conditioners (net.py:50, 61: 10 * tanh).  Widths and row pitches are below 2^22 (2^21 in fp64).  With `want_slope` returns (y, slope): act'(z),
     which `dense_backward` takes (None for "none"), of the type SLOPE[x.dtype] (fp16 for bf16, fp32 for fp16, else the element type)."""
+    calls = _calls()
+    if calls is not None:
+        device = _device()
+        done = calls.dense(x, kernel, bias, ACTIVATION.get(activation, -1), scale, residual, want_slope, device, _stream(device))
+        if done is not None:
+            return done
     dtype, index = _first(x)
     _agrees(kernel, "kernel", dtype, index)
     if bias is not None:
@@ -143,7 +151,7 @@ def dense(x, kernel, bias=None, *, activation="none", scale=1.0, residual=None, 
     x, ldx = _rows(x, n_in, "x")
     if bias is not None:
         _same_shape(bias, (n_out,), "bias")
-        bias = bias.contiguous()
+        bias = bias.resolve_neg().contiguous()
     ldr = 0
     if residual is not None:
         _same_shape(residual, shape, "residual")
@@ -162,6 +170,12 @@ def dense_backward(dy, x, kernel, slope=None, *, scale=1.0, want_x=True, want_ke
     """(dx, dkernel, dbias) of `dense` for the gradient dy of y, None where not wanted: with dz = scale * slope * dy, dx = dz @ kernel^T,
     dkernel = x^T @ dz (n_in, n_out), dbias = the sum of dz over the rows.  `slope` and `scale` as the forward call had them; the residual's
     gradient is dy itself.  dz is rounded to the element type, in which the matrix pipe takes it."""
+    calls = _calls()
+    if calls is not None:
+        device = _device()
+        done = calls.dense_backward(dy, x, kernel, slope, scale, want_x, want_kernel, want_bias, device, _stream(device))
+        if done is not None:
+            return done
     dtype, index = _first(dy)
     _agrees(x, "x", dtype, index)
     _agrees(kernel, "kernel", dtype, index)
@@ -179,7 +193,7 @@ def dense_backward(dy, x, kernel, slope=None, *, scale=1.0, want_x=True, want_ke
     if slope is not None:
         _agrees(slope, "slope", SLOPE[dtype], index)
         _same_shape(slope, shape, "slope")
-        slope = slope.contiguous()
+        slope = slope.resolve_neg().contiguous()
     dx = x.new_empty(x_shape) if want_x else None
     dkernel = x.new_empty((n_in, n_out)) if want_kernel else None
     dbias = x.new_empty(n_out) if want_bias else None
@@ -199,7 +213,7 @@ def _weights(t, name, dtype, index, cols):
         raise TypeError(f"{name} has type {t.dtype} beside {dtype}: the same, or fp32 beside 16-bit elements")
     _agrees(t, name, t.dtype, index)
     _same_shape(t, (cols,), name)
-    return t.contiguous()
+    return t.resolve_neg().contiguous()
 
 
 def _columns(x):
@@ -213,6 +227,12 @@ def layer_norm(x, weight=None, bias=None, *, eps=1e-6, want_stats=False):
 
     weight, bias (cols,): x's element type, or fp32 beside 16-bit elements.  With `want_stats` returns (y, mean, rstd), which
     `layer_norm_backward` takes: of the leading shape, fp32 (fp64 for fp64)."""
+    calls = _calls()
+    if calls is not None:
+        device = _device()
+        done = calls.layer_norm(x, weight, bias, eps, want_stats, device, _stream(device))
+        if done is not None:
+            return done
     dtype, index = _first(x)
     cols = _columns(x)
     weights = None
@@ -246,6 +266,12 @@ def layer_norm(x, weight=None, bias=None, *, eps=1e-6, want_stats=False):
 def layer_norm_backward(dy, x, mean, rstd, weight=None, *, want_x=True, want_weight=True, want_bias=True, weight_dtype=None):
     """(dx, dweight, dbias) of `layer_norm` for the gradient dy of y, None where not wanted; mean, rstd from `layer_norm(..., want_stats=True)`.
     dweight and dbias have the weight's type (without a weight `weight_dtype`, else x's)."""
+    calls = _calls()
+    if calls is not None and (weight is not None or weight_dtype is None):
+        device = _device()
+        done = calls.layer_norm_backward(dy, x, mean, rstd, weight, want_x, want_weight, want_bias, device, _stream(device))
+        if done is not None:
+            return done
     dtype, index = _first(dy)
     _agrees(x, "x", dtype, index)
     cols = _columns(x)
@@ -269,7 +295,7 @@ def layer_norm_backward(dy, x, mean, rstd, weight=None, *, want_x=True, want_wei
             return layer_norm_backward(dy, x, mean, rstd, weight, want_x=want_x, want_weight=want_weight, want_bias=want_bias, weight_dtype=weight_dtype)
     x, ldx = _rows(x, cols, "x")
     dy, ldd = _rows(dy, cols, "dy")
-    mean, rstd = mean.contiguous(), rstd.contiguous()
+    mean, rstd = mean.resolve_neg().contiguous(), rstd.resolve_neg().contiguous()
     dx = x.new_empty(shape) if want_x else None
     if want_weight and want_bias:
         dweight, dbias = _empty((2, cols), dtype=weights, device=index).unbind(0)
@@ -331,7 +357,7 @@ def _table(leaves, targets, clip):
     if targets is not None:
         if len(targets) != len(leaves):
             raise ValueError(f"{len(leaves)} tensors and {len(targets)} to write them to")
-        if [t.shape for t in targets] != [t.shape for t in leaves] or _codes(targets) != codes or any([t.get_device() != index for t in targets]) \
+        if [(t.shape, t.is_neg()) for t in targets] != [(t.shape, t.is_neg()) for t in leaves] or _codes(targets) != codes or any([t.get_device() != index for t in targets]) \
                 or not (plain and all([t.is_contiguous() for t in targets])) and [t.stride() for t in targets] != [t.stride() for t in leaves]:
             raise ValueError("out: shapes, strides, element types and devices have to be those of the tensors")
         to = [t.data_ptr() for t in targets]
@@ -342,24 +368,21 @@ def _table(leaves, targets, clip):
 
 def _global_norm(tensors, max_norm, out):
     clip = max_norm is not None
-    leaves = tensors if type(tensors) is list else _leaves(tensors, [])
+    calls = _calls()
+    if calls is not None:
+        device = _device()
+        done = calls.global_norm(tensors if type(tensors) is list else _leaves(tensors, []), out if out is None or type(out) is list else _leaves(out, []), max_norm,
+                                 device, _stream(device))
+        if done is not None:
+            return done
+    leaves = _leaves(tensors, [])
     if not leaves:
         raise ValueError("no tensors")
-    targets = out if out is None or type(out) is list else _leaves(out, [])
-    count = len(leaves)
-    read, table, place = nat.tensor_reader(), array("q", bytes(32 * count)), array("q", (0,))
-    if read is not None and read(leaves, targets, clip and _recording(), table.buffer_info()[0], count, place.buffer_info()[0]):
-        index = place[0]
-    else:
-        leaves = _leaves(leaves, [])
-        if not leaves:
-            raise ValueError("no tensors")
-        table, index = _table(leaves, None if targets is None else _leaves(targets, []), clip)
-        count = len(leaves)
+    table, index = _table(leaves, None if out is None else _leaves(out, []), clip)
     if _device() != index:
         with torch.cuda.device(index):
             return _global_norm(tensors, max_norm, out)
-    address = table.buffer_info()[0]
+    address, count = table.buffer_info()[0], len(leaves)
     norm = _empty((), dtype=torch.float64, device=index)
     ws, nbytes = _workspace("vmcpde_global_norm_workspace_bytes", index, address, count)
     _call("vmcpde_global_norm", address, count, clip, max_norm if clip else 0.0, norm.data_ptr(), None if ws is None else ws.data_ptr(), nbytes, _stream(index))
