@@ -196,9 +196,20 @@ __global__ __launch_bounds__(THREADS) void scale_kernel(Table tab, const double*
   scale_any(e, at, left < tab.chunk ? left : tab.chunk, threadIdx.x, THREADS, f);
 }
 
+// The kernel's first argument, brought into LDS at once: the arguments lie in the host's memory, and entry after entry each is a trip of its own (2 us).
+template <typename S>
+__device__ __forceinline__ void stage_arguments(S& to) {
+  static_assert(sizeof(S) % 4 == 0, "whole words");
+  const auto* from = (const __attribute__((address_space(4))) uint32_t*)__builtin_amdgcn_kernarg_segment_ptr();
+  for (int u = threadIdx.x; u < (int)(sizeof(S) / 4); u += blockDim.x) reinterpret_cast<uint32_t*>(&to)[u] = from[u];
+  __syncthreads();
+}
+
 // everything in one workgroup: a few thousand numbers cost three launches more than their arithmetic
-__global__ __launch_bounds__(SMALL_THREADS) void small_kernel(Table tab, int clip, double max_norm, double* __restrict__ norm) {
+__global__ __launch_bounds__(SMALL_THREADS) void small_kernel(Table, int clip, double max_norm, double* __restrict__ norm) {
   __shared__ double shared_factor;
+  __shared__ Table tab;
+  stage_arguments(tab);
   Bins b = {0, 0, 0};
   // leaves are mostly shorter than a wave: a wave takes every sixteenth tensor, and all of them share one that is long
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
@@ -215,6 +226,79 @@ __global__ __launch_bounds__(SMALL_THREADS) void small_kernel(Table tab, int cli
   const double f = shared_factor;
   for (int k = 0; k < tab.shared; ++k) scale_any(tab.e[k], 0, tab.e[k].n, threadIdx.x, SMALL_THREADS, f);
   for (int k = tab.shared + wave; k < tab.count; k += SMALL_THREADS / 64) scale_any(tab.e[k], 0, tab.e[k].n, lane, 64, f);
+}
+
+// The same for tensors of one type that fit the workgroup's registers, in pieces of 64 elements: every element is read once and all loads fly together.
+// 4213 fp64 numbers in 51 tensors (the leaves of a flow): 5.2 us against 10.
+template <int PIECES>      // of a wave: eight where they do, in fp64 (its three bins) the adding of absent ones takes 3 us
+struct Flat {
+  static constexpr int ALL = PIECES * SMALL_THREADS / 64;
+  static_assert(TABLE <= 256, "a byte numbers the tensors");
+  Entry e[TABLE];          // `first`: the tensor's first piece
+  int32_t pieces;
+  uint8_t tensor[ALL];
+};
+
+template <typename T, int PIECES>
+__global__ __launch_bounds__(SMALL_THREADS) void flat_kernel(Flat<PIECES>, int clip, double max_norm, double* __restrict__ norm) {
+  typedef typename Wide<T>::type A;
+  __shared__ double shared_factor;
+  __shared__ Flat<PIECES> tab;
+  stage_arguments(tab);
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, pieces = tab.pieces;
+  T v[PIECES];
+#pragma unroll
+  for (int j = 0; j < PIECES; ++j) {                   // (no branches: a lane without an element reads the tensor's first, so that all loads fly at once)
+    const int c = wave + j * (SMALL_THREADS / 64);
+    const Entry& e = tab.e[tab.tensor[min(c, pieces - 1)]];
+    const int at = (c - e.first) * 64 + lane;
+    const bool mine = c < pieces && at < e.n;
+    const T x = static_cast<const T*>(e.in)[mine ? at : 0];
+    v[j] = mine ? x : (T)0;
+  }
+  Bins b = {0, 0, 0};
+#pragma unroll
+  for (int j = 0; j < PIECES; ++j) add_square(b, v[j]);
+  b = group_bins<SMALL_THREADS / 64>(b);
+  if (threadIdx.x == 0) {
+    const double n = join(b);
+    *norm = n;
+    shared_factor = clip_factor(n, max_norm);
+  }
+  __syncthreads();
+  if (!clip) return;
+  const A f = (A)shared_factor;
+#pragma unroll
+  for (int j = 0; j < PIECES; ++j) {
+    const int c = wave + j * (SMALL_THREADS / 64);
+    if (c >= pieces) break;
+    const Entry& e = tab.e[tab.tensor[c]];
+    const int at = (c - e.first) * 64 + lane;
+    if (at < e.n) static_cast<T*>(e.out)[at] = (T)((A)v[j] * f);
+  }
+}
+
+// Launches flat_kernel; false: it does not take these tensors (several types, or too many pieces).
+template <int PIECES>
+bool flat(const vmcpde_tensor* t, int32_t count, int clip, double max_norm, double* norm, hipStream_t s) {
+  Flat<PIECES> tab;
+  int32_t filled = 0, dtype = 0;
+  tab.pieces = 0;
+  for (int32_t k = 0; k < count; ++k) {
+    if (t[k].n == 0) continue;
+    const int64_t pieces = ceil_div(t[k].n, 64);
+    if (filled == TABLE || (filled && t[k].dtype != dtype) || tab.pieces + pieces > tab.ALL) return false;
+    dtype = t[k].dtype;
+    tab.e[filled] = {t[k].in, t[k].out, t[k].n, t[k].dtype, tab.pieces};
+    for (int64_t c = 0; c < pieces; ++c) tab.tensor[tab.pieces++] = (uint8_t)filled;
+    ++filled;
+  }
+  if (!filled) return false;
+  if (dtype == VMCPDE_F64) flat_kernel<double><<<1, SMALL_THREADS, 0, s>>>(tab, clip, max_norm, norm);
+  else if (dtype == VMCPDE_F32) flat_kernel<float><<<1, SMALL_THREADS, 0, s>>>(tab, clip, max_norm, norm);
+  else if (dtype == VMCPDE_F16) flat_kernel<f16_t><<<1, SMALL_THREADS, 0, s>>>(tab, clip, max_norm, norm);
+  else flat_kernel<bf16_t><<<1, SMALL_THREADS, 0, s>>>(tab, clip, max_norm, norm);
+  return true;
 }
 
 struct Plan {
@@ -305,7 +389,8 @@ extern "C" {
 
 int64_t vmcpde_global_norm_workspace_bytes(const vmcpde_tensor* tensors, int32_t count) {
   if (check_tensors(tensors, count, false)) return -1;
-  return (plan_of(tensors, count).groups * (int64_t)sizeof(Bins) + 16 + 255) / 256 * 256;
+  const Plan p = plan_of(tensors, count);
+  return p.small ? 0 : round_up(p.groups * (int64_t)sizeof(Bins) + 16, 256);
 }
 
 int vmcpde_global_norm(const vmcpde_tensor* tensors, int32_t count, int32_t clip, double max_norm, double* norm, void* workspace,
@@ -322,6 +407,10 @@ int vmcpde_global_norm(const vmcpde_tensor* tensors, int32_t count, int32_t clip
   }
   const Plan p = plan_of(tensors, count);
   hipStream_t s = static_cast<hipStream_t>(stream);
+  if (p.small && (flat<8>(tensors, count, clip, max_norm, norm, s) || flat<16>(tensors, count, clip, max_norm, norm, s))) {
+    VMC_CHECK_HIP(hipGetLastError());
+    return 0;
+  }
   if (p.small) {
     Table tab;
     tab.count = 0;
