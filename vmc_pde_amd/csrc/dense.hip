@@ -90,7 +90,7 @@ __device__ __forceinline__ void activate_exact(int act, A z, A& a, A& slope) {
 
 // The same beside 16-bit elements, some 1e-7 absolute (2e-7 relative for small tanh), a tenth of the instructions: with the library's functions the
 // epilogue of a large product took as long as a quarter of its multiplications.  erf: the rational approximation 7.1.26 of Abramowitz and Stegun.
-__device__ __forceinline__ void activate_short(int act, float z, float& a, float& slope) {
+__device__ __forceinline__ void activate_short(int act, const float z, float& a, float& slope) {
   const float x = fabsf(z);
   if (act == VMCPDE_ACT_TANH) {
     const float e = __expf(-2 * x), y = z * z;
@@ -116,11 +116,32 @@ __device__ __forceinline__ void activate(int act, A z, A& a, A& slope) {
   if (act == VMCPDE_ACT_NONE) {
     a = z;
     slope = 1;
-  } else if constexpr (sizeof(T) == 2) {
-    activate_short(act, z, a, slope);
   } else {
     activate_exact<A>(act, z, a, slope);
   }
+}
+
+// The choice is made once for all N (so that they overlap) and slopes are computed where they are wanted (one by one: 4096 x 4096 x 16384 with tanh 500 us, so 460;
+// without activation 434).
+template <int ACT, int N>
+__device__ __forceinline__ void activate_shorts(bool want_slope, float (&z)[N], float (&slope)[N]) {
+  if (want_slope) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) activate_short(ACT, z[k], z[k], slope[k]);
+  } else {
+    float unused;
+#pragma unroll
+    for (int k = 0; k < N; ++k) activate_short(ACT, z[k], z[k], unused);
+  }
+}
+template <int N>
+__device__ __forceinline__ void activate_shorts(int act, bool want_slope, float (&z)[N], float (&slope)[N]) {
+  if (act == VMCPDE_ACT_TANH) activate_shorts<VMCPDE_ACT_TANH, N>(want_slope, z, slope);
+  else if (act == VMCPDE_ACT_GELU) activate_shorts<VMCPDE_ACT_GELU, N>(want_slope, z, slope);
+  else if (act == VMCPDE_ACT_SILU) activate_shorts<VMCPDE_ACT_SILU, N>(want_slope, z, slope);
+  else
+#pragma unroll
+    for (int k = 0; k < N; ++k) slope[k] = 1;
 }
 
 template <typename T>
@@ -136,24 +157,64 @@ struct Epilogue {
   int32_t act;
 };
 
-// columns col .. col + N of a row (those inside it), from their sums
+// N numbers as they lie in memory
+template <typename T, int N>
+struct __attribute__((packed, aligned(sizeof(T)))) Held { T v[N]; };
+// columns col .. col + N of a row, zero behind its end or without a row
+template <typename T, int N>
+__device__ __forceinline__ Held<T, N> held_at(const T* __restrict__ row, int64_t col, int64_t cols) {
+  Held<T, N> h = {};
+  if (!row) return h;
+  if (col + N <= cols) return *reinterpret_cast<const Held<T, N>*>(row + col);
+#pragma unroll
+  for (int k = 0; k < N; ++k)
+    if (col + k < cols) h.v[k] = row[col + k];
+  return h;
+}
+
+// columns col .. col + N of a row (those inside it), from their sums, the bias and the residual there
 template <typename T, int N, typename A>
-__device__ __forceinline__ void finish(const Epilogue<T>& e, int64_t row, int64_t col, A (&z)[N]) {
-  A slope[N], more[N];
+__device__ __forceinline__ void finish(const Epilogue<T>& e, int64_t row, int64_t col, A (&z)[N], const Held<T, N>& bias, const Held<T, N>& residual) {
+  A slope[N];
   if (e.bias) {
-    load_vec<T, N>(e.bias, col, e.n, more);
 #pragma unroll
-    for (int k = 0; k < N; ++k) z[k] += more[k];
+    for (int k = 0; k < N; ++k) z[k] += (A)bias.v[k];
   }
-  if (e.residual) load_vec<T, N>(e.residual + row * e.ldr, col, e.n, more);
+  activate_shorts<N>(e.act, e.slope != nullptr, z, slope);
 #pragma unroll
-  for (int k = 0; k < N; ++k) {
-    activate<T, A>(e.act, z[k], z[k], slope[k]);
-    z[k] *= e.scale;
-    if (e.residual) z[k] += more[k];
+  for (int k = 0; k < N; ++k) z[k] *= e.scale;
+  if (e.residual) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) z[k] += (A)residual.v[k];
   }
   store_vec<T, N>(e.y + row * e.ldy, col, e.n, z);
   if (e.slope) store_vec<typename Slope<T>::type, N>(e.slope + row * e.n, col, e.n, slope);
+}
+template <typename T, int N>
+__device__ __forceinline__ Held<T, N> residual_at(const Epilogue<T>& e, int64_t row, int64_t col) {
+  return held_at<T, N>(e.residual ? e.residual + row * e.ldr : nullptr, col, e.n);
+}
+template <typename T, int N, typename A>
+__device__ __forceinline__ void finish(const Epilogue<T>& e, int64_t row, int64_t col, A (&z)[N]) {
+  if constexpr (sizeof(T) == 2) {
+    finish<T, N, A>(e, row, col, z, held_at<T, N>(e.bias, col, e.n), residual_at<T, N>(e, row, col));
+  } else {                                 // (one number after the other: fewer registers, of which the occupancy of fp64's products depends)
+    A slope[N], more[N];
+    if (e.bias) {
+      load_vec<T, N>(e.bias, col, e.n, more);
+#pragma unroll
+      for (int k = 0; k < N; ++k) z[k] += more[k];
+    }
+    if (e.residual) load_vec<T, N>(e.residual + row * e.ldr, col, e.n, more);
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      activate<T, A>(e.act, z[k], z[k], slope[k]);
+      z[k] *= e.scale;
+      if (e.residual) z[k] += more[k];
+    }
+    store_vec<T, N>(e.y + row * e.ldy, col, e.n, z);
+    if (e.slope) store_vec<typename Slope<T>::type, N>(e.slope + row * e.n, col, e.n, slope);
+  }
 }
 
 // ---- products ----------------------------------------------------------------------------------------------------------------------
@@ -315,9 +376,9 @@ struct Tile {
 };
 
 // BM x BN of C by WM x WN waves; k in [k_begin, k_end) (k_begin a multiple of the step).  The column operand goes in as the matrix instruction's first, so a lane's results lie along a row of C.
-// out(row, col, v): the sums of C[row][col .. col + N].
+// out.put(row, col, v, ...): the sums of C[row][col .. col + N].
 template <typename T, int BM, int BN, int WM, int WN, bool PX, bool QX, typename F>
-__device__ __forceinline__ void tile_product(const Product& g, int row0, int col0, int k_begin, int k_end, F out) {
+__device__ __forceinline__ void tile_product(const Product& g, int row0, int col0, int k_begin, int k_end, const F& out) {
   typedef typename Wide<T>::type A;
   typedef typename Matrix<T>::Acc Acc;
   typedef typename Matrix<T>::Frag Frag;
@@ -409,9 +470,22 @@ __device__ __forceinline__ void tile_product(const Product& g, int row0, int col
     multiply(p1, q1);
   }
   // Sixteen rows at a time through a piece of LDS of the wave's own, so that a lane ends with N columns of a row and a row's lanes write whole lines.
-  // The loop stays rolled (the epilogue is long); the registers are picked by number inside it.
-  constexpr int N = TN == 1 ? 4 : 8, COLS = TN * 16, PITCH = COLS + 4;
+  // The loop stays rolled (the epilogue is long); the registers are picked by number inside it.  A lane's columns are the same every time; what it needs of
+  // the residual is asked for a turn ahead (4096 x 4096 x 16384 bf16 with a residual: 505 -> 482 us; fp32 and fp64, whose registers it would take from the
+  // product's occupancy, lost 2 and 6 %).
+  constexpr int N = TN == 1 ? 4 : 8, COLS = TN * 16, PITCH = COLS + 4, PARTS = 16 * COLS / N / 64;
+  constexpr bool AHEAD = sizeof(T) == 2;
   static_assert(WM * WN * 16 * PITCH * (int)sizeof(A) <= STAGES * (P::BYTES + Q::BYTES), "the rows fit the tiles' LDS");
+  static_assert(64 % (COLS / N) == 0, "a lane's columns are the same in every part");
+  auto row_of = [&](int turn, int j) { return row0 + wr + turn * 16 + (j * 64 + lane) / (COLS / N); };
+  Held<T, N> bias, residual[PARTS];
+  int col;
+  if constexpr (AHEAD) {
+    col = col0 + wc + lane % (COLS / N) * N;
+    bias = out.template bias<N>(col);
+#pragma unroll
+    for (int j = 0; j < PARTS; ++j) residual[j] = out.template residual<N>(row_of(0, j), col);
+  }
   __syncthreads();
   A* rows = reinterpret_cast<A*>(tiles) + wave * 16 * PITCH;
   const int i = lane & 15, group = lane >> 4;
@@ -430,16 +504,50 @@ __device__ __forceinline__ void tile_product(const Product& g, int row0, int col
           }
         }
       }
+    Held<T, N> now[PARTS];
 #pragma unroll
-    for (int j = 0; j < 16 * COLS / N / 64; ++j) {
-      const int u = j * 64 + lane, r = u / (COLS / N), c = u % (COLS / N) * N;
+    for (int j = 0; j < PARTS; ++j) {
+      if (AHEAD) now[j] = residual[j];
+      if (AHEAD && turn + 1 < TM) residual[j] = out.template residual<N>(row_of(turn + 1, j), col);
+    }
+#pragma unroll
+    for (int j = 0; j < PARTS; ++j) {
       A v[N];
 #pragma unroll
-      for (int k = 0; k < N; ++k) v[k] = rows[r * PITCH + c + k];
-      out(row0 + wr + turn * 16 + r, col0 + wc + c, v);
+      for (int k = 0; k < N; ++k) v[k] = rows[(j * 64 + lane) / (COLS / N) * PITCH + lane % (COLS / N) * N + k];
+      if constexpr (AHEAD) out.put(row_of(turn, j), col, v, bias, now[j]);
+      else out.put(row_of(turn, j), col0 + wc + (j * 64 + lane) % (COLS / N) * N, v);
     }
   }
 }
+
+// Where a tile's sums go: through the epilogue, or as a k slice's to `part`.
+template <typename T>
+struct Target {
+  typedef typename Wide<T>::type A;
+  const Epilogue<T>& e;
+  A* part;
+  const Product& g;
+  template <int N>
+  __device__ __forceinline__ Held<T, N> bias(int col) const { return held_at<T, N>(part ? nullptr : e.bias, col, e.n); }
+  template <int N>
+  __device__ __forceinline__ Held<T, N> residual(int row, int col) const {
+    if (part || !e.residual || row >= g.m) return {};
+    return residual_at<T, N>(e, row, col);
+  }
+  template <int N>
+  __device__ __forceinline__ void put(int row, int col, A (&v)[N], const Held<T, N>& bias, const Held<T, N>& residual) const {
+    if (row >= g.m || col >= g.n) return;
+    if (part) store_vec<A, N>(part + ((int64_t)blockIdx.y * g.m + row) * g.n, col, g.n, v);
+    else finish<T, N, A>(e, row, col, v, bias, residual);
+  }
+  template <int N>
+  __device__ __forceinline__ void put(int row, int col, A (&v)[N]) const {
+    if (row >= g.m || col >= g.n) return;
+    if (part) store_vec<A, N>(part + ((int64_t)blockIdx.y * g.m + row) * g.n, col, g.n, v);
+    else finish<T, N, A>(e, row, col, v);
+  }
+};
 
 // C in BM x BN tiles, slice blockIdx.y of the k range (`part` != null: its sums).  Workgroups go round the eight XCDs by their number: each
 // XCD takes one contiguous eighth of the tiles, in bands of eight tile rows, so that the operands a band shares stay in its L2.
@@ -453,12 +561,8 @@ __global__ __launch_bounds__(64 * WM * WN, BM * BN >= 256 * 256 ? 1 : 2) void pr
   const int band = (int)(tile / per_band), in_band = (int)(tile - band * per_band), height = min(8, tiles_m - band * 8);
   const int row0 = (band * 8 + in_band % height) * BM, col0 = (in_band / height) * BN;
   const int k_begin = blockIdx.y * k_slice, k_end = min(k_begin + k_slice, g.k);
-  tile_product<T, BM, BN, WM, WN, PX, QX>(g, row0, col0, k_begin, k_end, [&](int row, int col, auto& v) {
-    constexpr int N = sizeof(v) / sizeof(A);
-    if (row >= g.m || col >= g.n) return;
-    if (part) store_vec<A, N>(part + ((int64_t)blockIdx.y * g.m + row) * g.n, col, g.n, v);
-    else finish<T, N>(e, row, col, v);
-  });
+  const Target<T> to = {e, part, g};
+  tile_product<T, BM, BN, WM, WN, PX, QX>(g, row0, col0, k_begin, k_end, to);
 }
 
 // the slices' sums and the epilogue: four columns a lane.  PARTS lanes share them where there are many slices of a small product; a part's slices, then
