@@ -221,6 +221,23 @@ def test_dense_beyond_32_bits(layers):
     assert not bool(dkernel[:-40].any())
 
 
+def test_dense_of_a_token_beyond_32_bits(layers):
+    """One row, whose kernel's last lines lie more than 2^32 bytes behind its first ones: across k (the product) and along it (dx)."""
+    n_in, n_out = 8400, 262144
+    x = torch.zeros((1, n_in), dtype=torch.bfloat16, device="cuda")
+    x[:, -40:] = normal((1, 40), torch.bfloat16, 1)
+    dy = torch.zeros((1, n_out), dtype=torch.bfloat16, device="cuda")
+    dy[:, -40:] = normal((1, 40), torch.bfloat16, 2)
+    kernel = torch.zeros((n_in, n_out), dtype=torch.bfloat16, device="cuda")
+    kernel[-40:, -40:] = normal((40, 40), torch.bfloat16, 3)
+    want = plain.dense(x[:, -40:], kernel[-40:, -40:], None, None, "none", 1.0, dy[:, -40:], torch.bfloat16)
+    y = layers.dense(x, kernel)
+    dx, _, _ = layers.dense_backward(dy, x, kernel, want_kernel=False, want_bias=False)
+    for name, got in (("y", y), ("dx", dx)):
+        plain.agrees(got[:, -40:], want[name], name)
+        assert not bool(got[:, :-40].any())
+
+
 def test_dense_refuses_shapes(layers):
     x, k = torch.zeros(3, 4, device="cuda"), torch.zeros(4, 5, device="cuda")
     for call in (lambda: layers.dense(x, torch.zeros(5, 4, device="cuda")), lambda: layers.dense(x, k, torch.zeros(4, device="cuda")),
@@ -610,6 +627,60 @@ def test_a_training_step_in_a_graph(layers, dtype):
         torch.cuda.synchronize()
         assert torch.equal(norm, want[0]) and torch.equal(dx, want[1]) and torch.equal(captured.flat, eager.flat)
         x.copy_(normal(x.shape, dtype, 60))
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("rows", [1, 3, 20])
+def test_a_token_in_a_graph(layers, dtype, rows):
+    """A block's forward pass for single tokens and a small set clipped, captured and replayed with eager work between: the eager results bit for bit."""
+    x = normal((rows, 512), dtype, 1)
+    up, down = normal((512, 700), dtype, 2, 0.05), normal((512, 700), dtype, 3, 0.05).t()
+    weight, small = normal((512,), dtype, 4), [normal((n,), dtype, 5 + n) for n in (1, 70, 513)]
+
+    def token():
+        h = layers.dense(layers.layer_norm(x, weight), up, activation="silu")
+        y = layers.dense(h, down, residual=x)
+        out = [torch.empty_like(v) for v in small]
+        return (y, layers.clip_by_global_norm(small, 0.5, out=out), *out)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        token()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = token()
+    for k in range(4):
+        graph.replay()
+        want = token()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        x.copy_(normal(x.shape, dtype, 60 + k))
+
+
+def test_two_threads_at_once(layers):
+    """Python threads on streams of their own (a call releases the interpreter while it launches)."""
+    import threading
+    x = [normal((1 + k, 600), torch.bfloat16, k) for k in range(4)]
+    kernel = normal((600, 900), torch.bfloat16, 9, 0.05)
+    want = [layers.dense(v, kernel, activation="gelu") for v in x]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(k):
+        with torch.no_grad(), torch.cuda.stream(torch.cuda.Stream()):
+            results = [layers.dense(x[k], kernel, activation="gelu") for _ in range(50)]
+            torch.cuda.current_stream().synchronize()
+            if not all(torch.equal(r, want[k]) for r in results):
+                wrong.append(k)
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
 
 
 def test_two_streams_at_once(layers):
