@@ -9,6 +9,7 @@ from __future__ import annotations
 import os
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -68,15 +69,17 @@ def build(force: bool = False, verbose: bool = False, variant: str = "", extra_f
              "-Wall", "-Wno-unused-function", "-ffp-contract=on",
              "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",       # some packed fp32 forms have given wrong results on this chip
              *extra_flags]
+    commands = []
     for src in SOURCES:
         s = CSRC / src
         o = objdir / (src.replace(".hip", ".o"))
         if force or _stale(o, [s] + HEADERS):
-            cmd = [_hipcc(), *flags, *FILE_FLAGS.get(src, []), "-c", str(s), "-o", str(o)]
+            commands.append([_hipcc(), *flags, *FILE_FLAGS.get(src, []), "-c", str(s), "-o", str(o)])
             if verbose:
-                print(" ".join(cmd), flush=True)
-            subprocess.run(cmd, check=True)
+                print(" ".join(commands[-1]), flush=True)
         objs.append(o)
+    with ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as pool:
+        list(pool.map(lambda cmd: subprocess.run(cmd, check=True), commands))
     if force or _stale(lib, objs):
         cmd = [_hipcc(), "-shared", "-fPIC", f"--offload-arch={ARCH}", "-o", str(lib), *map(str, objs), "-ldl"]
         if verbose:
