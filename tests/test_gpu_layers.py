@@ -291,7 +291,7 @@ def test_native_calls_and_python_agree(layers, dtype, monkeypatch):
 # ---- layer norm --------------------------------------------------------------------------------------------------------------------------
 
 NORM_SIZES = [(0, 5), (1, 1), (3, 1), (5, 2), (65, 21), (33, 64), (7, 100), (300, 129), (17, 512), (40, 777), (9, 1025), (66, 2048), (3, 4096), (600, 4099), (5, 8192),
-              (2, 10001), (3, 16384), (2, 33000), (700, 70), (2050, 8)]
+              (2, 10001), (3, 16384), (2, 33000), (700, 70), (2050, 8), (3, 20001), (3, 32768), (5, 40003)]
 
 
 @pytest.mark.parametrize("dtype, weights", [(d, d) for d in DTYPES] + [(torch.float16, torch.float32), (torch.bfloat16, torch.float32)],
