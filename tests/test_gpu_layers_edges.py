@@ -1,0 +1,36 @@
+"""The layer operators at the edges of their types' ranges, of torch's bookkeeping and of what their layouts allow."""
+import math
+
+import pytest
+import torch
+
+import helpers_layers as plain
+from test_gpu_layers import layers, normal  # noqa: F401  (layers: the fixture)
+
+pytestmark = pytest.mark.gpu
+HALF = [torch.float16, torch.bfloat16]
+HALF_IDS = ["f16", "bf16"]
+
+
+# ---- dense -------------------------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("with_slope", [True, False], ids=["slope", "no-slope"])
+@pytest.mark.parametrize("dtype", HALF, ids=HALF_IDS)
+@pytest.mark.parametrize("size", [(2, 24, 40), (70, 24, 40), (3000, 33, 51), (5, 2000, 300), (600, 300, 520)], ids=lambda s: "x".join(map(str, s)))
+@pytest.mark.parametrize("scale, dy_size, operand_size", [(10.0, 7000.0, 1e-3), (1e-4, 1e-3, 30.0)], ids=["large", "small"])
+def test_dense_backward_keeps_the_range_of_dy(layers, scale, dy_size, operand_size, size, dtype, with_slope):  # noqa: F811
+    """Gradients that fit their type where scale * dy itself does not: beyond fp16's largest number, or among its subnormal ones.  In the 2-norm: one rounding of
+    slope * dy and one of the output, at most a half step each, and fp32 sums that cost less than a third one."""
+    rows, n_in, n_out = size
+    x, kernel = normal((rows, n_in), dtype, 1, operand_size), normal((n_in, n_out), dtype, 2, operand_size)
+    dy = normal((rows, n_out), dtype, 3).clamp(-1.5, 1.5) * dy_size
+    kept = layers.SLOPE[dtype]
+    slope = (0.5 + 0.5 * torch.rand((rows, n_out), generator=torch.Generator().manual_seed(4))).to(kept).cuda() if with_slope else None
+    dx, dkernel, _ = layers.dense_backward(dy, x, kernel, slope, scale=scale, want_bias=False)
+    dz = scale * plain.f64(dy) * (plain.f64(slope) if with_slope else 1)
+    for name, got, want in (("dx", dx, dz @ plain.f64(kernel).t()), ("dkernel", dkernel, plain.f64(x).t() @ dz)):
+        assert bool(torch.isfinite(got).all()), f"{name}: not finite"
+        # the smallest gradients (2 rows, small: dkernel of some 4e-6) are among fp16's subnormal numbers: there the output's own rounding costs half of its fixed
+        # step, 2^-25 = 3e-8, an element, root (elements) times that in the 2-norm
+        off, size_ = float(torch.linalg.norm(plain.f64(got) - want)), float(torch.linalg.norm(want))
+        assert off <= 3 * plain.half_step(dtype) * size_ + math.sqrt(want.numel()) * plain.smallest(dtype), f"{name}: off by {off / size_:.3g}"

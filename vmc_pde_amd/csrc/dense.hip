@@ -764,16 +764,17 @@ __global__ __launch_bounds__(256) void few_along_kernel(Product g, int k_slice, 
 
 // ---- what is made ready before the products --------------------------------------------------------------------------------------------
 
-// Up to three copies in one launch: lines of n elements to lines of ld_to (zeros behind n), scaled by scale * slope: an operand into lines that the
-// products can fetch, or dz = scale * slope * dy; `to` may be null.  With `sums` also the sums of dz's columns, or where several groups of workgroups share
-// the lines each one's part of them: partial[group][n].  `lanes` (a power of two) lie along the columns, 256 / lanes lines are taken at a time.  Bound by memory:
+// Up to three copies in one launch: lines of n elements to lines of ld_to (zeros behind n), times the slope: an operand into lines that the
+// products can fetch, or dz / scale = slope * dy; `to` may be null.  With `sums` also the sums of dz's columns (unrounded numbers', scaled at the end), or where several
+// groups of workgroups share the lines each one's part of them: partial[group][n].  The scale stays out of what is rounded and goes into the products' epilogue: fp16 has no
+// room for it (10 * 7000 is beyond its largest number, 1e-4 * 1e-3 among its last subnormal ones, where the gradients themselves may well fit).  `lanes` (a power of two) lie along the columns, 256 / lanes lines are taken at a time.  Bound by memory:
 // dz of 8192 x 4096 bf16 and its columns' sums 32 us = 6.2 TB/s.
 template <typename T>
 struct Job {
   const T* from;
   int64_t ld, lines, n;
   const typename Slope<T>::type* slope;
-  typename Wide<T>::type scale;
+  typename Wide<T>::type scale;      // of the sums
   T* to;
   int64_t ld_to;
   typename Wide<T>::type* partial;
@@ -806,7 +807,6 @@ __global__ __launch_bounds__(256) void prepare_kernel(Jobs<T> jobs) {
     if (b.slope) load_vec<typename Slope<T>::type, V>(b.slope + r * b.n, col, b.n, s);
 #pragma unroll
     for (int k = 0; k < V; ++k) {
-      v[k] *= b.scale;
       if (b.slope) v[k] *= s[k];
       if (col + k >= b.n) v[k] = 0;
       sum[k] += v[k];
@@ -820,6 +820,7 @@ __global__ __launch_bounds__(256) void prepare_kernel(Jobs<T> jobs) {
   for (int c = threadIdx.x; c < lanes * V; c += 256) {
     A v = 0;
     for (int p = 0; p < at_once; ++p) v += sh[p * lanes * V + c];
+    v *= b.scale;
     if (col0 + c < b.n) {
       if (b.groups == 1) b.sums[col0 + c] = (T)v;
       else b.partial[(int64_t)group * b.n + col0 + c] = v;
@@ -1355,7 +1356,7 @@ struct Dense {
     }
     const Lines dy = {a.dy, a.rows, a.n_out, a.ldd};
     Lines dz = dy;
-    const bool own = (a.dx || a.dkernel) && (a.slope || a.scale != 1.0 || !fetchable<T>(dy));
+    const bool own = (a.dx || a.dkernel) && (a.slope || !fetchable<T>(dy));
     Job<T> b = job_of(dy);
     if (own) {
       b.ld_to = round_up(a.n_out, vec_of<T>());
@@ -1377,11 +1378,11 @@ struct Dense {
     launch_jobs();
     if (launch && b.partial) add_columns<A, T>(b.partial, b.groups, a.n_out, a.n_out, 0, static_cast<T*>(a.dbias), nullptr, stream);
     if (want_x) {
-      const Epilogue<T> e = {nullptr, nullptr, 0, static_cast<T*>(a.dx), a.n_in, nullptr, a.n_in, 1, VMCPDE_ACT_NONE};
+      const Epilogue<T> e = {nullptr, nullptr, 0, static_cast<T*>(a.dx), a.n_in, nullptr, a.n_in, (A)a.scale, VMCPDE_ACT_NONE};
       multiply(dz, false, kernel, a.kernel_t, a.rows, a.n_in, a.n_out, e);
     }
     if (a.dkernel) {
-      const Epilogue<T> e = {nullptr, nullptr, 0, static_cast<T*>(a.dkernel), a.n_out, nullptr, a.n_out, 1, VMCPDE_ACT_NONE};
+      const Epilogue<T> e = {nullptr, nullptr, 0, static_cast<T*>(a.dkernel), a.n_out, nullptr, a.n_out, (A)a.scale, VMCPDE_ACT_NONE};
       multiply(x, true, dz, true, a.n_in, a.n_out, a.rows, e);
     }
   }

@@ -169,7 +169,8 @@ def dense(x, kernel, bias=None, *, activation="none", scale=1.0, residual=None, 
 def dense_backward(dy, x, kernel, slope=None, *, scale=1.0, want_x=True, want_kernel=True, want_bias=True):
     """(dx, dkernel, dbias) of `dense` for the gradient dy of y, None where not wanted: with dz = scale * slope * dy, dx = dz @ kernel^T,
     dkernel = x^T @ dz (n_in, n_out), dbias = the sum of dz over the rows.  `slope` and `scale` as the forward call had them; the residual's
-    gradient is dy itself.  dz is rounded to the element type, in which the matrix pipe takes it."""
+    gradient is dy itself.  slope * dy is rounded to the element type, in which the matrix pipe takes it (fp16: it has to stay below 65504, and slopes
+    reach 1.13); the scale is applied to the fp32 sums, and dbias sums unrounded numbers.  Tensors cast to fp32 beforehand round nothing on the way."""
     calls = _calls()
     if calls is not None:
         device = _device()
