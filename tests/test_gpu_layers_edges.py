@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import helpers_layers as plain
-from test_gpu_layers import layers, normal  # noqa: F401  (layers: the fixture)
+from test_gpu_layers import DTYPES, IDS, layers, normal  # noqa: F401  (layers: the fixture)
 
 pytestmark = pytest.mark.gpu
 HALF = [torch.float16, torch.bfloat16]
@@ -34,3 +34,22 @@ def test_dense_backward_keeps_the_range_of_dy(layers, scale, dy_size, operand_si
         # step, 2^-25 = 3e-8, an element, root (elements) times that in the 2-norm
         off, size_ = float(torch.linalg.norm(plain.f64(got) - want)), float(torch.linalg.norm(want))
         assert off <= 3 * plain.half_step(dtype) * size_ + math.sqrt(want.numel()) * plain.smallest(dtype), f"{name}: off by {off / size_:.3g}"
+
+
+# ---- layer norm --------------------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("cols", [9, 21, 33, 129, 257, 500, 1025])
+def test_layer_norm_of_equal_elements_is_equal(layers, dtype, cols):  # noqa: F811
+    """Every lane of a row has the row's sums to the last bit: what is equal in x (and dy) is equal in y (and dx), wherever it stands in the row."""
+    rows, g = 600, torch.Generator().manual_seed(cols)
+    which = torch.randint(0, 4, (rows, cols), generator=g)
+    x, dy = (torch.randn((rows, 4), generator=g, dtype=torch.float64).to(dtype).gather(1, which).cuda() for _ in range(2))
+    y, mean, rstd = layers.layer_norm(x, want_stats=True)
+    dx, _, _ = layers.layer_norm_backward(dy, x, mean, rstd)
+    for name, t in (("y", y), ("dx", dx)):
+        for v in range(4):
+            mine = (which == v).cuda()
+            low, high = t.masked_fill(~mine, math.inf).amin(1), t.masked_fill(~mine, -math.inf).amax(1)
+            there = mine.any(1)
+            assert torch.equal(low[there], high[there]), name

@@ -23,7 +23,8 @@ inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 
 inline int64_t round_up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
 inline int64_t ceil_div(int64_t v, int64_t m) { return (v + m - 1) / m; }
 
-// Sum over groups of GROUP consecutive lanes (16 or 64), every lane of the group returns it.  DPP steps, no LDS.
+// Sum over groups of GROUP consecutive lanes (16 or 64), every lane of the group returns it, to the last bit: partners exchange in every step, so both add
+// the same two numbers (rotations by four and eight do not: neighbouring quads' lanes added theirs in different orders).  DPP steps, no LDS.
 template <int CTRL>
 __device__ __forceinline__ float dpp_move(float v) {
   return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, false));
@@ -33,8 +34,8 @@ __device__ __forceinline__ A group_sum(A v) {
   static_assert(GROUP == 16 || GROUP == 64, "a DPP row or a wave");
   v += dpp_move<0xb1>(v);    // quad_perm [1,0,3,2]
   v += dpp_move<0x4e>(v);    // quad_perm [2,3,0,1]
-  v += dpp_move<0x124>(v);   // row_ror:4
-  v += dpp_move<0x128>(v);   // row_ror:8
+  v += dpp_move<0x141>(v);   // row_half_mirror: the other quad of eight lanes, of which all lanes hold one sum
+  v += dpp_move<0x140>(v);   // row_mirror: the other eight
   if constexpr (GROUP == 64) {
     v += __shfl_xor(v, 16);
     v += __shfl_xor(v, 32);
