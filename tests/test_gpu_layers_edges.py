@@ -53,3 +53,21 @@ def test_layer_norm_of_equal_elements_is_equal(layers, dtype, cols):  # noqa: F8
             low, high = t.masked_fill(~mine, math.inf).amin(1), t.masked_fill(~mine, -math.inf).amax(1)
             there = mine.any(1)
             assert torch.equal(low[there], high[there]), name
+
+
+@pytest.mark.parametrize("offset", [1e3, 1e4, 1e5])
+@pytest.mark.parametrize("cols", [3, 21, 100, 1000, 1024, 5000, 20001])
+def test_layer_norm_of_rows_far_from_zero(layers, cols, offset):  # noqa: F811
+    """fp32 rows of unit spread.  With u = 2^-24 and sums of depth D: the deviations from a first mean are rounded once (u) whatever that mean's own error; what it is
+    off by, the deviations' mean, is found to D u of their size and taken off (u); the variance is off by twice that and (D + 4) u, 1 / sqrt by half of it
+    and 6 u; two more roundings to y.  In all (|y| + 1) (3 D + 16) u, whatever the offset."""
+    x = (normal((40, cols), torch.float64, cols) + offset * (1 + 0.1 * normal((40, 1), torch.float64, cols + 1))).float()
+    y, mean, rstd = layers.layer_norm(x, eps=1e-6, want_stats=True)
+    exact = plain.f64(x)
+    centre = exact.mean(1, keepdim=True)
+    want_rstd = 1 / torch.sqrt(((exact - centre) ** 2).mean(1, keepdim=True) + 1e-6)
+    want, u, depth = (exact - centre) * want_rstd, 2.0 ** -24, 80 + cols / 512
+    plain.agrees(y, (want, (want.abs() + 1) * (3 * depth + 16) * u), "y")
+    plain.agrees(rstd, (want_rstd[:, 0], want_rstd[:, 0] * (2 * depth + 12) * u), "rstd")
+    # the mean: the nearest fp32 number, but for the correction's own error
+    plain.agrees(mean, (centre[:, 0], 1.01 * u * centre[:, 0].abs() + (depth + 4) * u * (exact - centre).abs().mean(1)), "mean")

@@ -265,7 +265,8 @@ def layer_norm(x, weight=None, bias=None, *, eps=1e-6, want_stats=False):
 
 
 def layer_norm_backward(dy, x, mean, rstd, weight=None, *, want_x=True, want_weight=True, want_bias=True, weight_dtype=None):
-    """(dx, dweight, dbias) of `layer_norm` for the gradient dy of y, None where not wanted; mean, rstd from `layer_norm(..., want_stats=True)`.
+    """(dx, dweight, dbias) of `layer_norm` for the gradient dy of y, None where not wanted; mean, rstd from `layer_norm(..., want_stats=True)`,
+    where the mean is rounded to fp32 (fp64 for fp64): normalised elements are off by up to 2^-24 |mean| rstd here, though y is not.
     dweight and dbias have the weight's type (without a weight `weight_dtype`, else x's)."""
     calls = _calls()
     if calls is not None and (weight is not None or weight_dtype is None):
