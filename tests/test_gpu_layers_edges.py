@@ -71,3 +71,18 @@ def test_layer_norm_of_rows_far_from_zero(layers, cols, offset):  # noqa: F811
     plain.agrees(rstd, (want_rstd[:, 0], want_rstd[:, 0] * (2 * depth + 12) * u), "rstd")
     # the mean: the nearest fp32 number, but for the correction's own error
     plain.agrees(mean, (centre[:, 0], 1.01 * u * centre[:, 0].abs() + (depth + 4) * u * (exact - centre).abs().mean(1)), "mean")
+
+
+# ---- global norm -------------------------------------------------------------------------------------------------------------------------
+
+def test_global_norm_of_many_large_numbers(layers):  # noqa: F811
+    """More than 2^24 numbers just below 2^500, whose squares add up to more than the largest fp64 number while their norm is some 2^512; and as many tiny ones."""
+    n = 18500000
+    for value in (0.99 * 2.0 ** 500, 0.99 * 2.0 ** 470, 1.01 * 2.0 ** -500):
+        t = torch.full((n,), value, dtype=torch.float64, device="cuda")
+        want = math.sqrt(n) * value
+        assert abs(float(layers.global_norm(t)) / want - 1) < 1e-12      # (some thousand additions of positive numbers in a row, 2^-53 each)
+        norm = layers.clip_by_global_norm(t, 1.0)
+        assert abs(float(norm) / want - 1) < 1e-12
+        if want > 1:
+            assert abs(float(t[0]) * math.sqrt(n) - 1) < 1e-12 and bool((t == t[0]).all())

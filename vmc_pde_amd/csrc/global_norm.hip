@@ -24,7 +24,8 @@ constexpr int64_t SMALL_SHARED = 512;  // a tensor of that launch that all its w
 constexpr int64_t MIN_CHUNK = 8192;
 constexpr int64_t GROUPS = 16384;      // workgroups a launch aims at: short ones balance better than eight a CU (1 GB clipped: 2048 651, 8192 584, 16384 573 us)
 
-constexpr double BIG = 0x1p500, TINY = 0x1p-500, DOWN = 0x1p-600, UP = 0x1p600;
+// Borders of the bins: the middle one's squares, from 2^-1000 to 2^960, leave room for 2^64 of them; so do the huge ones', from 2^-240 to 2^848, and the tiny ones', up to 2^200.
+constexpr double BIG = 0x1p480, TINY = 0x1p-500, DOWN = 0x1p-600, UP = 0x1p600;
 
 struct Entry {
   const void* in;
