@@ -86,3 +86,22 @@ def test_global_norm_of_many_large_numbers(layers):  # noqa: F811
         assert abs(float(norm) / want - 1) < 1e-12
         if want > 1:
             assert abs(float(t[0]) * math.sqrt(n) - 1) < 1e-12 and bool((t == t[0]).all())
+
+
+@pytest.mark.parametrize("dtype, size, max_norm", [(torch.float32, 1e37, 1e-3), (torch.float32, 1e37, 1e-28), (torch.bfloat16, 1e37, 1e-3), (torch.bfloat16, 1e37, 1e-28),
+                                                   (torch.float64, 1e300, 1e-15), (torch.float64, 1e300, 1e-280), (torch.float64, 1e-150, 1e-290)],
+                         ids=lambda v: str(v).replace("torch.", ""))
+@pytest.mark.parametrize("sizes", [[40], [300, 7, 21], [9000, 2000], [50000, 300], [300] * 130], ids=["40", "leaves", "9000", "50000", "130"])
+@pytest.mark.parametrize("mixed", [False, True], ids=["one-type", "mixed"])
+def test_clipping_far(layers, dtype, size, max_norm, sizes, mixed):  # noqa: F811
+    """max_norm / norm below the smallest normal number of the arithmetic: the clipped elements, which are ordinary numbers, keep their digits."""
+    tensors = [normal((n,), dtype, k, size) for k, n in enumerate(sizes)] + ([torch.ones(5, device="cuda", dtype=torch.float32)] if mixed else [])
+    exact = [plain.f64(t) for t in tensors]
+    largest = max(float(t.abs().max()) for t in exact)
+    norm = largest * math.sqrt(math.fsum(float(((t / largest) ** 2).sum()) for t in exact))
+    got = layers.clip_by_global_norm(tensors, max_norm)
+    assert abs(float(got) / norm - 1) < 1e-12
+    for t, e in zip(tensors, exact):
+        want = e / norm * max_norm if max_norm > 1e-200 else (e / norm) * max_norm
+        u, uw = plain.half_step(t.dtype), plain.half_step(plain.wide_of(t.dtype))
+        plain.agrees(t, (want, (u + 3 * uw + 2e-12) * want.abs() + 1.01 * plain.smallest(t.dtype)), "clipped")

@@ -92,11 +92,33 @@ __device__ void square_span(const T* __restrict__ p, int64_t n, int t, int threa
   if (tail + t < n) add_square(b, p[tail + t]);
 }
 
+// What clipping multiplies by: f 2^e.  Far below 1 (2^-100) f is kept in [1/4, 1), so that neither max / norm in fp64 nor f in fp32 is a subnormal number, which has lost
+// digits that the clipped elements, ordinary numbers at most max_norm, still have.
+struct Factor {
+  double f;
+  int32_t e;
+};
+__device__ __forceinline__ Factor clip_factor(double norm, double max_norm) {
+  if (!(norm > max_norm)) return {1.0, 0};                   // (NaN comes here)
+  const double q = max_norm / norm;
+  if (q >= 0x1p-100 || max_norm == 0 || norm == INFINITY) return {q, 0};
+  int en, em;
+  const double mn = frexp(norm, &en), mm = frexp(max_norm, &em);
+  return {0.5 * mm / mn, em - en + 1};
+}
+template <typename T, typename A>
+__device__ __forceinline__ T scaled(T v, A f, int e) {
+  const A r = (A)v * f;
+  if constexpr (sizeof(A) == 8) return (T)ldexp(r, e);
+  else return (T)ldexpf(r, e);
+}
+
 template <typename T>
-__device__ void scale_span(const T* p, T* o, int64_t n, int t, int threads, double factor) {
+__device__ void scale_span(const T* p, T* o, int64_t n, int t, int threads, Factor factor) {
   typedef typename Wide<T>::type A;
   constexpr int V = vec_of<T>();
-  const A f = (A)factor;
+  const A f = (A)factor.f;
+  const int e = factor.e;
   const int64_t vecs = n / V, tail = vecs * V;
   const Raw<T>* q = reinterpret_cast<const Raw<T>*>(p);
   Raw<T>* w = reinterpret_cast<Raw<T>*>(o);
@@ -108,17 +130,17 @@ __device__ void scale_span(const T* p, T* o, int64_t n, int t, int threads, doub
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
 #pragma unroll
-      for (int k = 0; k < V; ++k) r[u].v[k] = (T)((A)r[u].v[k] * f);
+      for (int k = 0; k < V; ++k) r[u].v[k] = scaled(r[u].v[k], f, e);
       __builtin_nontemporal_store(__builtin_bit_cast(uint4v, r[u]), reinterpret_cast<uint4v*>(w + j + u * threads));
     }
   }
   for (; j < vecs; j += threads) {
     Raw<T> r = q[j];
 #pragma unroll
-    for (int k = 0; k < V; ++k) r.v[k] = (T)((A)r.v[k] * f);
+    for (int k = 0; k < V; ++k) r.v[k] = scaled(r.v[k], f, e);
     w[j] = r;
   }
-  if (tail + t < n) o[tail + t] = (T)((A)p[tail + t] * f);
+  if (tail + t < n) o[tail + t] = scaled(p[tail + t], f, e);
 }
 
 __device__ void square_any(const Entry& e, int64_t at, int64_t n, int t, int threads, Bins& b) {
@@ -130,7 +152,7 @@ __device__ void square_any(const Entry& e, int64_t at, int64_t n, int t, int thr
   }
 }
 
-__device__ void scale_any(const Entry& e, int64_t at, int64_t n, int t, int threads, double factor) {
+__device__ void scale_any(const Entry& e, int64_t at, int64_t n, int t, int threads, Factor factor) {
   switch (e.dtype) {
     case VMCPDE_F64: scale_span(static_cast<const double*>(e.in) + at, static_cast<double*>(e.out) + at, n, t, threads, factor); break;
     case VMCPDE_F32: scale_span(static_cast<const float*>(e.in) + at, static_cast<float*>(e.out) + at, n, t, threads, factor); break;
@@ -153,8 +175,6 @@ __device__ Bins group_bins(Bins b) {
   return s;
 }
 
-__device__ __forceinline__ double clip_factor(double norm, double max_norm) { return norm > max_norm ? max_norm / norm : 1.0; }
-
 // the tensor that workgroup g of the launch works on: the last whose first workgroup is not behind g
 __device__ __forceinline__ int find(const Table& tab, int g) {
   int lo = 0, hi = tab.count - 1;
@@ -175,9 +195,8 @@ __global__ __launch_bounds__(THREADS) void squares_kernel(Table tab, Bins* __res
   if (threadIdx.x == 0) partial[g] = b;
 }
 
-// out2 = { norm, factor }
 __global__ __launch_bounds__(SMALL_THREADS) void join_kernel(const Bins* __restrict__ partial, int n, double max_norm, double* __restrict__ norm,
-                                                             double* __restrict__ factor) {
+                                                             Factor* __restrict__ factor) {
   Bins b = {0, 0, 0};
   for (int j = threadIdx.x; j < n; j += SMALL_THREADS) { b.big += partial[j].big; b.mid += partial[j].mid; b.tiny += partial[j].tiny; }
   b = group_bins<SMALL_THREADS / 64>(b);
@@ -188,11 +207,11 @@ __global__ __launch_bounds__(SMALL_THREADS) void join_kernel(const Bins* __restr
   }
 }
 
-__global__ __launch_bounds__(THREADS) void scale_kernel(Table tab, const double* __restrict__ factor) {
+__global__ __launch_bounds__(THREADS) void scale_kernel(Table tab, const Factor* __restrict__ factor) {
   const int g = blockIdx.x;
   const Entry& e = tab.e[find(tab, g)];
-  const double f = *factor;
-  if (f == 1.0 && e.in == e.out) return;
+  const Factor f = *factor;
+  if (f.f == 1.0 && e.in == e.out) return;       // (a far factor's f is below 1)
   const int64_t at = (int64_t)(g - e.first) * tab.chunk, left = e.n - at;
   scale_any(e, at, left < tab.chunk ? left : tab.chunk, threadIdx.x, THREADS, f);
 }
@@ -208,7 +227,7 @@ __device__ __forceinline__ void stage_arguments(S& to) {
 
 // everything in one workgroup: a few thousand numbers cost three launches more than their arithmetic
 __global__ __launch_bounds__(SMALL_THREADS) void small_kernel(Table, int clip, double max_norm, double* __restrict__ norm) {
-  __shared__ double shared_factor;
+  __shared__ Factor shared_factor;
   __shared__ Table tab;
   stage_arguments(tab);
   Bins b = {0, 0, 0};
@@ -224,7 +243,7 @@ __global__ __launch_bounds__(SMALL_THREADS) void small_kernel(Table, int clip, d
   }
   __syncthreads();
   if (!clip) return;
-  const double f = shared_factor;
+  const Factor f = shared_factor;
   for (int k = 0; k < tab.shared; ++k) scale_any(tab.e[k], 0, tab.e[k].n, threadIdx.x, SMALL_THREADS, f);
   for (int k = tab.shared + wave; k < tab.count; k += SMALL_THREADS / 64) scale_any(tab.e[k], 0, tab.e[k].n, lane, 64, f);
 }
@@ -243,7 +262,7 @@ struct Flat {
 template <typename T, int PIECES>
 __global__ __launch_bounds__(SMALL_THREADS) void flat_kernel(Flat<PIECES>, int clip, double max_norm, double* __restrict__ norm) {
   typedef typename Wide<T>::type A;
-  __shared__ double shared_factor;
+  __shared__ Factor shared_factor;
   __shared__ Flat<PIECES> tab;
   stage_arguments(tab);
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, pieces = tab.pieces;
@@ -268,14 +287,15 @@ __global__ __launch_bounds__(SMALL_THREADS) void flat_kernel(Flat<PIECES>, int c
   }
   __syncthreads();
   if (!clip) return;
-  const A f = (A)shared_factor;
+  const A f = (A)shared_factor.f;
+  const int f_e = shared_factor.e;
 #pragma unroll
   for (int j = 0; j < PIECES; ++j) {
     const int c = wave + j * (SMALL_THREADS / 64);
     if (c >= pieces) break;
     const Entry& e = tab.e[tab.tensor[c]];
     const int at = (c - e.first) * 64 + lane;
-    if (at < e.n) static_cast<T*>(e.out)[at] = (T)((A)v[j] * f);
+    if (at < e.n) static_cast<T*>(e.out)[at] = scaled(v[j], f, f_e);
   }
 }
 
@@ -391,7 +411,7 @@ extern "C" {
 int64_t vmcpde_global_norm_workspace_bytes(const vmcpde_tensor* tensors, int32_t count) {
   if (check_tensors(tensors, count, false)) return -1;
   const Plan p = plan_of(tensors, count);
-  return p.small ? 0 : round_up(p.groups * (int64_t)sizeof(Bins) + 16, 256);
+  return p.small ? 0 : round_up(p.groups * (int64_t)sizeof(Bins) + (int64_t)sizeof(Factor), 256);
 }
 
 int vmcpde_global_norm(const vmcpde_tensor* tensors, int32_t count, int32_t clip, double max_norm, double* norm, void* workspace,
@@ -424,11 +444,11 @@ int vmcpde_global_norm(const vmcpde_tensor* tensors, int32_t count, int32_t clip
     VMC_CHECK_HIP(hipGetLastError());
     return 0;
   }
-  const int64_t need = p.groups * (int64_t)sizeof(Bins) + 16;
+  const int64_t need = p.groups * (int64_t)sizeof(Bins) + (int64_t)sizeof(Factor);
   VMC_REQUIRE(workspace && workspace_bytes >= need, "vmcpde_global_norm: workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)need);
   VMC_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "vmcpde_global_norm: the workspace is not aligned to 16 bytes");
   Bins* partial = static_cast<Bins*>(workspace);
-  double* factor = reinterpret_cast<double*>(partial + p.groups);
+  Factor* factor = reinterpret_cast<Factor*>(partial + p.groups);
   int rc = for_tables(tensors, count, p, [&](const Table& tab, int64_t before) { squares_kernel<<<tab.groups, THREADS, 0, s>>>(tab, partial + before); });
   if (rc) return rc;
   join_kernel<<<1, SMALL_THREADS, 0, s>>>(partial, (int)p.groups, max_norm, norm, clip ? factor : nullptr);
