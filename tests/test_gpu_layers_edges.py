@@ -1,4 +1,5 @@
 """The layer operators at the edges of their types' ranges, of torch's bookkeeping and of what their layouts allow."""
+import ctypes as C
 import math
 
 import pytest
@@ -105,3 +106,46 @@ def test_clipping_far(layers, dtype, size, max_norm, sizes, mixed):  # noqa: F81
         want = e / norm * max_norm if max_norm > 1e-200 else (e / norm) * max_norm
         u, uw = plain.half_step(t.dtype), plain.half_step(plain.wide_of(t.dtype))
         plain.agrees(t, (want, (u + 3 * uw + 2e-12) * want.abs() + 1.01 * plain.smallest(t.dtype)), "clipped")
+
+
+# ---- errors, and what torch keeps account of -----------------------------------------------------------------------------------------------
+
+def test_a_call_that_failed_after_its_launch_is_not_made_again(layers):  # noqa: F811
+    """rc -1 is a refusal before any launch, which the Python code calls again and reports; any other error is raised as it is, with nothing run twice."""
+    from vmc_pde_amd import _native as nat
+    calls, library = nat.layer_calls(), nat.lib()
+    t, x, kernel = torch.full((10,), 2.0, device="cuda"), normal((3, 4), torch.float32, 1), normal((4, 5), torch.float32, 2)
+    y, mean, rstd = layers.layer_norm(x, want_stats=True)
+    names = ("vmcpde_dense_workspace_bytes", "vmcpde_dense", "vmcpde_dense_backward", "vmcpde_layer_norm", "vmcpde_layer_norm_backward_workspace_bytes",
+             "vmcpde_layer_norm_backward", "vmcpde_global_norm_workspace_bytes", "vmcpde_global_norm")      # (the order that bind takes them in)
+    seen = []
+
+    def entry(name, result):
+        """What stands for an entry point: needs no workspace, launches nothing, returns `result`."""
+        restype, argtypes = nat._PROTOS[name]
+
+        def stand_in(*arguments):
+            seen.append(name)
+            return 0 if name.endswith("_bytes") else result
+        return C.CFUNCTYPE(restype, *[a if a in (C.c_int32, C.c_int64, C.c_double) else C.c_void_p for a in argtypes])(stand_in)
+
+    every = {"vmcpde_dense": lambda: layers.dense(x, kernel), "vmcpde_dense_backward": lambda: layers.dense_backward(normal((3, 5), torch.float32, 3), x, kernel),
+             "vmcpde_layer_norm": lambda: layers.layer_norm(x), "vmcpde_layer_norm_backward": lambda: layers.layer_norm_backward(y, x, mean, rstd),
+             "vmcpde_global_norm": lambda: layers.clip_by_global_norm([t], 1.0)}
+    for result in (-2, -1):
+        stand_ins = [entry(name, result) for name in names]
+        calls.bind(*(C.cast(f, C.c_void_p).value for f in stand_ins))
+        try:
+            for name, call in every.items():
+                seen.clear()
+                if result == -2:
+                    with pytest.raises(nat.VmcpdeError, match=name):
+                        call()
+                else:
+                    call()                                   # (refused here, done by the Python code through the library's own entry)
+                assert seen.count(name) == 1
+            if result == -2:
+                assert bool((t == 2).all())
+        finally:
+            calls.bind(*(C.cast(getattr(library, name), C.c_void_p).value for name in names))
+    assert float(layers.global_norm([t])) == pytest.approx(1.0, rel=1e-6)

@@ -192,6 +192,7 @@ def layer_calls():
             names = ("vmcpde_dense_workspace_bytes", "vmcpde_dense", "vmcpde_dense_backward", "vmcpde_layer_norm", "vmcpde_layer_norm_backward_workspace_bytes",
                      "vmcpde_layer_norm_backward", "vmcpde_global_norm_workspace_bytes", "vmcpde_global_norm")
             module.bind(*(C.cast(getattr(lib(), name), C.c_void_p).value for name in names))
+            module.raising(VmcpdeError, C.cast(lib().vmcpde_last_error, C.c_void_p).value)
         _calls = (module,)
     return _calls[0]
 

@@ -2,8 +2,9 @@
 //
 // Host code only, a library of its own beside libvmcpde.so, whose boundary stays free of torch types.  A small call is bound by the host: Python's checks
 // and attribute reads and torch's allocations through Python took 5 of the 8.6 us of a token's norm and 28 us of a small training step's two.
-// Nothing is decided here: whatever is not plain (another device, layouts that need a copy, arguments that have to be refused, an error) returns
-// None, and vmc_pde_amd/layers.py, which can do all of it, handles or refuses the call.
+// Nothing is decided here: whatever is not plain (another device, layouts that need a copy, arguments that have to be refused) returns
+// None before anything is launched, and vmc_pde_amd/layers.py, which can do all of it, handles or refuses the call.  What fails behind that is raised: made a second time,
+// clipping in place would clip what is clipped already.
 #include <torch/csrc/autograd/python_variable.h>
 #include <ATen/ops/empty.h>
 #include <c10/core/GradMode.h>
@@ -27,7 +28,12 @@ struct {
   decltype(&vmcpde_global_norm) global_norm;
 } entry;
 
+// vmc_pde_amd._native's exception and the library's message
+PyObject* error_class = PyExc_RuntimeError;
+decltype(&vmcpde_last_error) last_error;
+
 struct NotPlain {};
+struct Raised {};      // a Python exception is set
 inline void need(bool plain) {
   if (!plain) throw NotPlain();
 }
@@ -110,19 +116,28 @@ struct Workspace {
   }
 };
 
-// one call into the library; what it refuses, the Python code calls again and reports
+// One call into the library.  What it refuses (-1, with nothing launched) the Python code calls again and reports; other errors may have come behind a launch.
 template <typename F>
-void call(F f) {
+void call(const char* name, F f) {
   int rc;
   Py_BEGIN_ALLOW_THREADS
   rc = f();
   Py_END_ALLOW_THREADS
-  need(rc == 0);
+  need(rc != -1);
+  if (rc == 0) return;
+  PyErr_Format(error_class, "%s failed (rc=%d): %s", name, rc, last_error ? last_error() : "");
+  throw Raised();
 }
 
+// (behind the call: nothing may send it back to the Python code)
 PyObject* wrap(const at::Tensor& t) {
-  if (t.defined()) return THPVariable_Wrap(t);
-  Py_RETURN_NONE;
+  if (!t.defined()) Py_RETURN_NONE;
+  try {
+    return THPVariable_Wrap(t);
+  } catch (...) {
+    if (!PyErr_Occurred()) PyErr_SetString(error_class, "a result could not be handed to Python");
+    return nullptr;
+  }
 }
 PyObject* wrap(const at::Tensor& a, const at::Tensor& b) { return Py_BuildValue("(NN)", wrap(a), wrap(b)); }
 PyObject* wrap(const at::Tensor& a, const at::Tensor& b, const at::Tensor& c) { return Py_BuildValue("(NNN)", wrap(a), wrap(b), wrap(c)); }
@@ -131,6 +146,8 @@ template <typename F>
 PyObject* plainly(F f) {
   try {
     return f();
+  } catch (const Raised&) {
+    return nullptr;
   } catch (...) {
     PyErr_Clear();
     Py_RETURN_NONE;
@@ -182,7 +199,7 @@ PyObject* dense(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const int64_t bytes = entry.dense_workspace(&a, 0);
     const Workspace space(bytes, x);
     void* stream = in.stream();
-    call([&] { return entry.dense(&a, space.p, bytes, stream); });
+    call("vmcpde_dense", [&] { return entry.dense(&a, space.p, bytes, stream); });
     return want_slope ? wrap(y, slope) : wrap(y);
   });
 }
@@ -224,7 +241,7 @@ PyObject* dense_backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const int64_t bytes = entry.dense_workspace(&a, 1);
     const Workspace space(bytes, x);
     void* stream = in.stream();
-    call([&] { return entry.dense_backward(&a, space.p, bytes, stream); });
+    call("vmcpde_dense_backward", [&] { return entry.dense_backward(&a, space.p, bytes, stream); });
     return wrap(dx, dkernel, dbias);
   });
 }
@@ -276,7 +293,7 @@ PyObject* layer_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
       need(a.rows > 0);                       // (no rows, no addresses: the Python code's)
     }
     void* stream = in.stream();
-    call([&] { return entry.layer_norm(&a, stream); });
+    call("vmcpde_layer_norm", [&] { return entry.layer_norm(&a, stream); });
     return want_stats ? wrap(y, mean, rstd) : wrap(y);
   });
 }
@@ -316,7 +333,7 @@ PyObject* layer_norm_backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const int64_t bytes = want_weight || want_bias ? entry.layer_norm_workspace(&a) : 0;
     const Workspace space(bytes, x);
     void* stream = in.stream();
-    call([&] { return entry.layer_norm_backward(&a, space.p, bytes, stream); });
+    call("vmcpde_layer_norm_backward", [&] { return entry.layer_norm_backward(&a, space.p, bytes, stream); });
     return wrap(dx, dweight, dbias);
   });
 }
@@ -345,7 +362,7 @@ PyObject* global_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const Workspace space(bytes, norm);
     void* stream = in.stream();
     double* to = static_cast<double*>(norm.data_ptr());
-    call([&] { return entry.global_norm(table.data(), (int32_t)count, clip, max_norm, to, space.p, bytes, stream); });
+    call("vmcpde_global_norm", [&] { return entry.global_norm(table.data(), (int32_t)count, clip, max_norm, to, space.p, bytes, stream); });
     return wrap(norm);
   });
 }
@@ -367,8 +384,22 @@ PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t n) {
   Py_RETURN_NONE;
 }
 
+// (the exception class to raise, the address of vmcpde_last_error)
+PyObject* raising(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  void* address = n == 2 && PyExceptionClass_Check(args[0]) ? PyLong_AsVoidPtr(args[1]) : nullptr;
+  if (!address) {
+    if (!PyErr_Occurred()) PyErr_SetString(PyExc_TypeError, "raising takes an exception class and the address of vmcpde_last_error");
+    return nullptr;
+  }
+  Py_INCREF(args[0]);      // (kept as long as the module, which is never unloaded)
+  error_class = args[0];
+  static_assert(sizeof(last_error) == sizeof(address), "a function's address");
+  std::memcpy(&last_error, &address, sizeof(address));
+  Py_RETURN_NONE;
+}
+
 #define METHOD(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
-PyMethodDef methods[] = {METHOD(bind),       METHOD(dense),       METHOD(dense_backward), METHOD(layer_norm), METHOD(layer_norm_backward),
+PyMethodDef methods[] = {METHOD(bind),       METHOD(raising),       METHOD(dense),       METHOD(dense_backward), METHOD(layer_norm), METHOD(layer_norm_backward),
                          METHOD(global_norm), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "vmcpde_layer_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
