@@ -13,6 +13,14 @@ HALF = [torch.float16, torch.bfloat16]
 HALF_IDS = ["f16", "bf16"]
 
 
+@pytest.fixture(params=[True, False], ids=["native", "python"])
+def either(request, monkeypatch):
+    """Both forms of a call: the native module, and the Python code that it spares the host from."""
+    from vmc_pde_amd import _native as nat
+    if not request.param:
+        monkeypatch.setattr(nat, "_calls", (None,))
+
+
 # ---- dense -------------------------------------------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("with_slope", [True, False], ids=["slope", "no-slope"])
@@ -149,3 +157,21 @@ def test_a_call_that_failed_after_its_launch_is_not_made_again(layers):  # noqa:
         finally:
             calls.bind(*(C.cast(getattr(library, name), C.c_void_p).value for name in names))
     assert float(layers.global_norm([t])) == pytest.approx(1.0, rel=1e-6)
+
+
+def test_clipping_in_place_is_seen_by_automatic_differentiation(layers, either):  # noqa: F811
+    for own in (True, False):
+        saved, given = torch.full((8,), 3.0, device="cuda"), torch.full((8,), 3.0, device="cuda")
+        x = torch.ones(8, device="cuda", requires_grad=True)
+        loss = (x * saved).sum()
+        before = saved._version
+        assert float(layers.global_norm([saved])) > 1 and saved._version == before
+        with torch.no_grad():
+            layers.clip_by_global_norm([saved] if own else [given], 1.0, out=None if own else [saved])
+        assert given._version == 0
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+    with torch.inference_mode():
+        free = torch.full((8,), 3.0, device="cuda")
+    layers.clip_by_global_norm([free], 1.0)                  # (such tensors have no account to keep)
+    assert float(layers.global_norm([free])) == pytest.approx(1.0, rel=1e-6)

@@ -349,12 +349,15 @@ PyObject* global_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
     need(count < (1 << 30));
     std::vector<vmcpde_tensor> table((size_t)count);
     at::TensorOptions options;
+    std::vector<at::Tensor> written;          // (held: other threads may change the lists while the interpreter is released)
+    if (clip) written.reserve((size_t)count);
     for (Py_ssize_t k = 0; k < count; ++k) {
       const at::Tensor& t = in.checked(PyList_GET_ITEM(tensors, k), clip && own);
       const at::Tensor& o = own ? t : in.checked(PyList_GET_ITEM(out, k), clip);
       need(t.is_contiguous() && (own || (o.is_contiguous() && o.sizes() == t.sizes() && o.scalar_type() == t.scalar_type())));
       table[(size_t)k] = {t.data_ptr(), o.data_ptr(), t.numel(), code_of(t.scalar_type()), 0};
       if (k == 0) options = t.options();
+      if (clip) written.push_back(o);
     }
     const double max_norm = clip ? in.number(2) : 0.0;
     const at::Tensor norm = at::empty({}, options.dtype(at::kDouble));
@@ -363,6 +366,9 @@ PyObject* global_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
     void* stream = in.stream();
     double* to = static_cast<double*>(norm.data_ptr());
     call("vmcpde_global_norm", [&] { return entry.global_norm(table.data(), (int32_t)count, clip, max_norm, to, space.p, bytes, stream); });
+    if (clip)                                 // written in place: a recorded graph that saved one of these has to see it
+      for (const at::Tensor& t : written)
+        if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
     return wrap(norm);
   });
 }

@@ -388,6 +388,10 @@ def _global_norm(tensors, max_norm, out):
     norm = _empty((), dtype=torch.float64, device=index)
     ws, nbytes = _workspace("vmcpde_global_norm_workspace_bytes", index, address, count)
     _call("vmcpde_global_norm", address, count, clip, max_norm if clip else 0.0, norm.data_ptr(), None if ws is None else ws.data_ptr(), nbytes, _stream(index))
+    if clip:                                   # written in place: a recorded graph that saved one of these has to see it
+        for t in leaves if out is None else _leaves(out, []):
+            if not t.is_inference():
+                torch.autograd.graph.increment_version(t)
     return norm
 
 
@@ -399,7 +403,7 @@ def global_norm(tensors):
 
 def clip_by_global_norm(tensors, max_norm, out=None):
     """Multiplies every tensor by max_norm / norm where their `global_norm` exceeds max_norm, in place or into `out` (tensors of the same shapes,
-    strides and types).  Returns the norm before clipping; nothing is read back to the host.  A NaN norm leaves the elements as they are, an
+    strides and types), which torch's version counters see.  Returns the norm before clipping; nothing is read back to the host.  A NaN norm leaves the elements as they are, an
     infinite one makes finite elements zero.  Tensors that overlap each other are refused: they would be scaled twice."""
     max_norm = float(max_norm)
     if not max_norm >= 0:
