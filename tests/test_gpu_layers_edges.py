@@ -4,6 +4,7 @@ import math
 
 import pytest
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 import helpers_layers as plain
 from test_gpu_layers import DTYPES, IDS, layers, normal  # noqa: F401  (layers: the fixture)
@@ -175,3 +176,23 @@ def test_clipping_in_place_is_seen_by_automatic_differentiation(layers, either):
         free = torch.full((8,), 3.0, device="cuda")
     layers.clip_by_global_norm([free], 1.0)                  # (such tensors have no account to keep)
     assert float(layers.global_norm([free])) == pytest.approx(1.0, rel=1e-6)
+
+
+def test_forward_mode_tangents_are_refused(layers, either):  # noqa: F811
+    x, kernel, bias, dy = normal((3, 4), torch.float32, 1), normal((4, 5), torch.float32, 2), normal((5,), torch.float32, 3), normal((3, 5), torch.float32, 4)
+    weight, slope = normal((4,), torch.float32, 5), torch.ones((3, 5), device="cuda")
+    y, mean, rstd = layers.layer_norm(x, want_stats=True)
+    with forward_ad.dual_level(), torch.no_grad():
+        def dual(t):
+            return forward_ad.make_dual(t, torch.ones_like(t))
+        for call in (lambda: layers.dense(dual(x), kernel), lambda: layers.dense(x, dual(kernel)), lambda: layers.dense(x, kernel, dual(bias)),
+                     lambda: layers.dense(x, kernel, residual=dual(dy)), lambda: layers.dense_backward(dual(dy), x, kernel), lambda: layers.dense_backward(dy, dual(x), kernel),
+                     lambda: layers.dense_backward(dy, x, dual(kernel)), lambda: layers.dense_backward(dy, x, kernel, dual(slope)), lambda: layers.layer_norm(dual(x)),
+                     lambda: layers.layer_norm(x, dual(weight)), lambda: layers.layer_norm(x, weight, dual(weight)), lambda: layers.layer_norm_backward(dual(x), x, mean, rstd),
+                     lambda: layers.layer_norm_backward(x, dual(x), mean, rstd), lambda: layers.layer_norm_backward(x, x, dual(mean), rstd),
+                     lambda: layers.layer_norm_backward(x, x, mean, dual(rstd)), lambda: layers.layer_norm_backward(x, x, mean, rstd, dual(weight)),
+                     lambda: layers.global_norm([x, dual(weight)]), lambda: layers.clip_by_global_norm([dual(weight)], 1.0),
+                     lambda: layers.clip_by_global_norm([weight], 1.0, out=[dual(torch.empty_like(weight))])):
+            with pytest.raises(ValueError, match="autograd"):
+                call()
+        assert torch.equal(layers.layer_norm(x), y)          # what has no tangent is taken there too

@@ -1,7 +1,24 @@
 """The host's part of the layer operators: loading, binding, and what is refused there (no GPU needed)."""
 from pathlib import Path
 
+import pytest
+import torch
+import torch.autograd.forward_ad as forward_ad
+
 ROOT = Path(__file__).resolve().parent.parent
+
+
+def test_forward_mode_tangents_are_refused_on_the_host():
+    from vmc_pde_amd import layers
+    x, kernel, stats = torch.zeros(3, 4), torch.zeros(4, 5), torch.zeros(3)
+    with forward_ad.dual_level(), torch.no_grad():
+        def dual(t):
+            return forward_ad.make_dual(t, torch.ones_like(t))
+        for call in (lambda: layers.dense(dual(x), kernel), lambda: layers.dense(x, dual(kernel)), lambda: layers.layer_norm(dual(x)), lambda: layers.layer_norm(x, dual(x[0])),
+                     lambda: layers.layer_norm_backward(x, x, dual(stats), stats), lambda: layers.global_norm([x, dual(x)]), lambda: layers.clip_by_global_norm(dual(x), 1.0),
+                     lambda: layers.clip_by_global_norm(x, 1.0, out=dual(x.clone()))):
+            with pytest.raises(ValueError, match="autograd"):
+                call()
 
 
 def test_every_lane_of_a_row_holds_the_same_sum():

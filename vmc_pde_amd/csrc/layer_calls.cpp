@@ -60,12 +60,13 @@ struct Arguments {
     need(n == wanted && device >= 0);
   }
   void* stream() const { return PyLong_AsVoidPtr(given[count - 1]); }
-  // a tensor on the device that automatic differentiation does not record
+  // a tensor on the device that automatic differentiation does not record, and without a forward-mode tangent
   const at::Tensor& tensor(int k) const { return checked(given[k], true); }
   const at::Tensor& checked(PyObject* p, bool written) const {
     need(THPVariable_Check(p));
     const at::Tensor& t = THPVariable_Unpack(p);
-    need(t.defined() && t.layout() == at::kStrided && t.is_cuda() && t.get_device() == device && !t.is_neg() && !(written && recording && t.requires_grad()));
+    need(t.defined() && t.layout() == at::kStrided && t.is_cuda() && t.get_device() == device && !t.is_neg() && !(written && recording && t.requires_grad()) &&
+         !t._fw_grad(/* level */ 0).defined());
     return t;
   }
   const at::Tensor* tensor_or_none(int k) const { return given[k] == Py_None ? nullptr : &tensor(k); }

@@ -3,7 +3,8 @@
 The conditioners of the coupling flow are chains of dense layers (reference: vmc_fluids/net.py:53-61) that `csrc/flow.hip` evaluates whole,
 per sample, with their weights in LDS.  These are the same layers as operators over a batch, of any width, in fp64, fp32, fp16 and bf16, with
 what a training step of a wide network needs around them.  Like the rest of this package they are explicit: every operator has its gradient as
-a function of its own, and takes no part in torch's automatic differentiation (tensors that require it are refused while it is recording).
+a function of its own, and takes no part in torch's automatic differentiation (tensors that require it are refused while it is recording, and so are
+those with a forward-mode tangent).
 
 All run on the current HIP stream, allocate through torch, never synchronise with the host, and can be captured into a graph.  Sums, statistics
 and epilogues are held in fp32 for fp32 and 16-bit elements, in fp64 for fp64.  None uses atomics: the same call gives the same bits.
@@ -18,6 +19,7 @@ import struct
 from array import array
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 
 from . import _native as nat
 
@@ -62,6 +64,12 @@ def _workspace(name, device, *arguments):
     return _empty(nbytes, dtype=torch.uint8, device=device), nbytes
 
 
+def _plain(t):
+    """Refuses what automatic differentiation, in either mode, would follow."""
+    if t.requires_grad and _recording() or unpack_dual(t).tangent is not None:
+        raise ValueError(_AUTOGRAD)
+
+
 def _first(t):
     """Element type and device index of the tensor that every other one has to agree with."""
     if not isinstance(t, torch.Tensor):
@@ -69,8 +77,7 @@ def _first(t):
     dtype = t.dtype
     if dtype not in DTYPE:
         raise TypeError(f"element type {dtype}: fp64, fp32, fp16 and bf16 are supported")
-    if t.requires_grad and _recording():
-        raise ValueError(_AUTOGRAD)
+    _plain(t)
     return dtype, t.get_device()
 
 
@@ -81,8 +88,7 @@ def _agrees(t, name, dtype, index):
         raise TypeError(f"{name} has type {t.dtype}: {dtype} is needed")
     if t.get_device() != index:
         raise ValueError(f"{name} is on {t.device}, not on " + (f"cuda:{index}" if index >= 0 else "cpu"))
-    if t.requires_grad and _recording():
-        raise ValueError(_AUTOGRAD)
+    _plain(t)
 
 
 def _rows(t, cols, name):
@@ -346,6 +352,8 @@ def _codes(leaves):
 def _table(leaves, targets, clip):
     """(rows of vmcpde_tensor, device index); refuses what cannot be reduced or written."""
     index, codes = leaves[0].get_device(), _codes(leaves)
+    if any([unpack_dual(t).tangent is not None for t in (leaves if targets is None else [*leaves, *targets])]):
+        raise ValueError(_AUTOGRAD)
     if index < 0:
         raise ValueError(_HOST)
     if any([t.get_device() != index for t in leaves]):
