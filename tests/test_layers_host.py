@@ -1,4 +1,6 @@
 """The host's part of the layer operators: loading, binding, and what is refused there (no GPU needed)."""
+import subprocess
+import sys
 from pathlib import Path
 
 import pytest
@@ -6,6 +8,22 @@ import torch
 import torch.autograd.forward_ad as forward_ad
 
 ROOT = Path(__file__).resolve().parent.parent
+
+
+def test_the_package_imports_where_torch_has_no_gpu_backend(lib_built):
+    """A torch build without one lacks the functions that ask for the current device and stream."""
+    code = ("import torch\n"
+            "for name in ('_cuda_getDevice', '_cuda_getCurrentRawStream'):\n"
+            "    if hasattr(torch._C, name): delattr(torch._C, name)\n"
+            "torch.cuda.device_count = lambda: 0\n"
+            "from vmc_pde_amd import layers\n"
+            "try:\n"
+            "    layers.dense(torch.zeros(3, 4), torch.zeros(4, 5))\n"
+            "except ValueError as refused:\n"
+            "    assert 'device' in str(refused)\n"
+            "else:\n"
+            "    raise SystemExit(1)\n")
+    subprocess.run([sys.executable, "-c", code], cwd=ROOT, check=True, timeout=300)
 
 
 def test_forward_mode_tangents_are_refused_on_the_host():

@@ -34,7 +34,9 @@ _HOST = "the layer operators run on device (HBM) tensors only"
 _pack_dense = struct.Struct("@4i3qPqPqPPqdPqPPqPPP").pack       # vmcpde_dense_args
 _pack_norm = struct.Struct("@2i2qPqPPdPqPPPqPPP").pack          # vmcpde_norm_args
 
-_calls, _empty, _device, _stream, _recording = nat.layer_calls, torch.empty, torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream, torch.is_grad_enabled
+_calls, _empty, _recording = nat.layer_calls, torch.empty, torch.is_grad_enabled
+# (torch built without a GPU backend lacks these; there every tensor is refused before they are needed)
+_device, _stream = getattr(torch._C, "_cuda_getDevice", None), getattr(torch._C, "_cuda_getCurrentRawStream", None)
 _entry = {}
 
 
