@@ -1,6 +1,7 @@
 """The host's part of the layer operators: loading, binding, and what is refused there (no GPU needed)."""
 import subprocess
 import sys
+import warnings
 from pathlib import Path
 
 import pytest
@@ -8,6 +9,13 @@ import torch
 import torch.autograd.forward_ad as forward_ad
 
 ROOT = Path(__file__).resolve().parent.parent
+
+
+@pytest.fixture()
+def nat(lib_built):
+    from vmc_pde_amd import _native
+    _native.lib()
+    return _native
 
 
 def test_the_package_imports_where_torch_has_no_gpu_backend(lib_built):
@@ -24,6 +32,42 @@ def test_the_package_imports_where_torch_has_no_gpu_backend(lib_built):
             "else:\n"
             "    raise SystemExit(1)\n")
     subprocess.run([sys.executable, "-c", code], cwd=ROOT, check=True, timeout=300)
+
+
+@pytest.mark.parametrize("case", ["another torch", "no library at all"])
+def test_a_stale_native_module_is_left_out(nat, monkeypatch, tmp_path, case):
+    """The Python code is the whole operator: a module that was built for another torch, or does not load, is left out with a warning."""
+    monkeypatch.setattr(torch.cuda, "device_count", lambda: 1)
+    monkeypatch.setattr(nat, "_calls", None)
+    if case == "another torch":
+        monkeypatch.setattr(torch, "__version__", "0.0.0")
+    else:
+        (tmp_path / "_lib").mkdir()
+        (tmp_path / "_lib" / "vmcpde_layer_calls.so").write_bytes(b"not a library")
+        monkeypatch.setattr(nat, "_HERE", tmp_path)
+    with pytest.warns(RuntimeWarning, match="vmcpde_layer_calls"):
+        assert nat.layer_calls() is None
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        assert nat.layer_calls() is None           # said once
+
+
+def test_the_native_module_loads(nat, monkeypatch):
+    monkeypatch.setattr(torch.cuda, "device_count", lambda: 1)
+    monkeypatch.setattr(nat, "_calls", None)
+    assert nat.layer_calls() is not None
+
+
+def test_the_native_module_is_built_again_for_another_torch(monkeypatch, tmp_path):
+    from vmc_pde_amd import build
+    commands = []
+    monkeypatch.setattr(build.subprocess, "run", lambda cmd, **_: commands.append(cmd))
+    monkeypatch.setattr(build, "_stale", lambda target, deps: False)
+    monkeypatch.setattr(build, "CALLS_LIB", tmp_path / "vmcpde_layer_calls.so")
+    for version, built in (("0.0.0", 1), ("0.0.0", 1), ("0.0.1", 2), ("0.0.1", 2)):
+        monkeypatch.setattr(torch, "__version__", version)
+        build.build_calls()
+        assert len(commands) == built
 
 
 def test_forward_mode_tangents_are_refused_on_the_host():

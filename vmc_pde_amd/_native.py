@@ -9,6 +9,8 @@ from __future__ import annotations
 import ctypes as C
 import importlib.util
 import re
+import sys
+import warnings
 from pathlib import Path
 
 import torch
@@ -180,15 +182,28 @@ def lib():
 _calls = None
 
 
+def torch_build() -> str:
+    """What csrc/layer_calls.cpp's module is tied to: this torch's C++ interface, and this Python's."""
+    return f"torch {torch.__version__}, python {sys.version_info[0]}.{sys.version_info[1]}"
+
+
 def layer_calls():
-    """The Python module of csrc/layer_calls.cpp, or None where it is not built or no GPU is there: it only saves the host's time."""
+    """The Python module of csrc/layer_calls.cpp, or None where no GPU is there, or where it is not built for this torch: it only saves the host's time."""
     global _calls
     if _calls is None:
         path, module = _HERE / "_lib" / "vmcpde_layer_calls.so", None
         if path.exists() and torch.cuda.device_count():
-            spec = importlib.util.spec_from_file_location("vmcpde_layer_calls", path)
-            module = importlib.util.module_from_spec(spec)
-            spec.loader.exec_module(module)
+            try:
+                spec = importlib.util.spec_from_file_location("vmcpde_layer_calls", path)
+                module = importlib.util.module_from_spec(spec)
+                spec.loader.exec_module(module)
+                if module.built_for != torch_build():
+                    raise ImportError(f"it was built for {module.built_for}, this is {torch_build()}")
+            except (ImportError, AttributeError) as stale:
+                module = None
+                warnings.warn(f"{path} is left out ({stale}): the layer operators' calls take longer on the host until it is built again "
+                              "(python -m vmc_pde_amd.build)", RuntimeWarning, stacklevel=2)
+        if module is not None:
             names = ("vmcpde_dense_workspace_bytes", "vmcpde_dense", "vmcpde_dense_backward", "vmcpde_layer_norm", "vmcpde_layer_norm_backward_workspace_bytes",
                      "vmcpde_layer_norm_backward", "vmcpde_global_norm_workspace_bytes", "vmcpde_global_norm")
             module.bind(*(C.cast(getattr(lib(), name), C.c_void_p).value for name in names))

@@ -46,14 +46,19 @@ def build_calls(force: bool = False, verbose: bool = False) -> Path:
 
     import torch
     from torch.utils.cpp_extension import include_paths, library_paths
+
+    from ._native import torch_build
     LIBDIR.mkdir(exist_ok=True)
-    if force or _stale(CALLS_LIB, [CALLS_SOURCE, PKG.parent / "include" / "vmcpde.h"]):
+    stamp, built_for = CALLS_LIB.with_suffix(".txt"), torch_build()      # (the module is tied to torch's C++ interface, which file times know nothing of)
+    if force or _stale(CALLS_LIB, [CALLS_SOURCE, PKG.parent / "include" / "vmcpde.h"]) or not stamp.exists() or stamp.read_text() != built_for:
         cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-w", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+               f'-DVMCPDE_BUILT_FOR="{built_for}"',
                *[f"-I{p}" for p in [*include_paths(), sysconfig.get_paths()["include"]]], str(CALLS_SOURCE), "-o", str(CALLS_LIB),
                *[f"-L{p}" for p in library_paths()], "-ltorch_python", "-ltorch_cpu", "-lc10"]
         if verbose:
             print(" ".join(cmd), flush=True)
         subprocess.run(cmd, check=True)
+        stamp.write_text(built_for)
     return CALLS_LIB
 
 

@@ -412,4 +412,9 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "vmcpde_layer_calls", nullptr, -1, 
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit_vmcpde_layer_calls() { return PyModule_Create(&module); }
+// built_for: the torch and Python that this was compiled against; of any other only this may be asked
+PyMODINIT_FUNC PyInit_vmcpde_layer_calls() {
+  PyObject* m = PyModule_Create(&module);
+  if (m && PyModule_AddStringConstant(m, "built_for", VMCPDE_BUILT_FOR)) Py_CLEAR(m);
+  return m;
+}
