@@ -1,6 +1,7 @@
 """The host's part of the layer operators: loading, binding, and what is refused there (no GPU needed)."""
 import subprocess
 import sys
+import threading
 import warnings
 from pathlib import Path
 
@@ -68,6 +69,31 @@ def test_the_native_module_is_built_again_for_another_torch(monkeypatch, tmp_pat
         monkeypatch.setattr(torch, "__version__", version)
         build.build_calls()
         assert len(commands) == built
+
+
+def test_entry_points_bound_by_two_threads(nat, monkeypatch):
+    """A thread that calls while another one binds the entry points finds all of them or binds them itself, never some."""
+    from vmc_pde_amd import layers
+    real, first, go_on = nat.lib(), threading.Event(), threading.Event()
+    binder = threading.Thread(target=lambda: layers._entries())
+
+    class Slow:
+        def __getitem__(self, name):
+            if threading.current_thread() is binder:
+                if first.is_set():
+                    go_on.wait(30)
+                first.set()
+            return real[name]
+    monkeypatch.setattr(layers, "_entry", {})
+    monkeypatch.setattr(nat, "lib", Slow)
+    binder.start()
+    assert first.wait(30)
+    try:
+        assert layers._workspace("vmcpde_global_norm_workspace_bytes", "cpu", None, 0) == (None, 0)       # (no tensors: nothing is read)
+    finally:
+        go_on.set()
+        binder.join()
+    assert len(layers._entry) == 8
 
 
 def test_forward_mode_tangents_are_refused_on_the_host():

@@ -42,12 +42,13 @@ _entry = {}
 
 def _entries():
     """The entry points with packed records as their first argument (bound on first use: the library may not be built yet)."""
-    library = nat.lib()
+    library, found = nat.lib(), {}
     for name, (result, arguments) in nat._PROTOS.items():
         if name.startswith(("vmcpde_dense", "vmcpde_layer_norm", "vmcpde_global_norm")):
             f = library[name]
             f.restype, f.argtypes = result, [C.c_void_p, *arguments[1:]]
-            _entry[name] = f
+            found[name] = f
+    _entry.update(found)                       # (at once: another thread finds none of them or all)
     return _entry
 
 
