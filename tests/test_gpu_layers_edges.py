@@ -46,6 +46,27 @@ def test_dense_backward_keeps_the_range_of_dy(layers, scale, dy_size, operand_si
         assert off <= 3 * plain.half_step(dtype) * size_ + math.sqrt(want.numel()) * plain.smallest(dtype), f"{name}: off by {off / size_:.3g}"
 
 
+@pytest.mark.parametrize("dtype", [torch.float64, torch.bfloat16], ids=["f64", "bf16"])
+def test_dense_copies_rows_that_lie_too_far_apart(layers, dtype):  # noqa: F811
+    """Row pitches beyond the kernels' 2^22 (2^21 in fp64) elements."""
+    pitch = (1 << 22) + 6
+    whole = torch.zeros((60, pitch), dtype=dtype, device="cuda")
+    for rows, n_in, n_out in ((3, 60, 50), (7, 50, 60)):
+        x, kernel, dy = whole[:rows, 10:10 + n_in], whole[:n_in, 200:200 + n_out], whole[:rows, 400:400 + n_out]
+        for k, t in enumerate((x, kernel, dy)):
+            t.copy_(normal(t.shape, dtype, k))
+        apart = whole[:n_out, 600:600 + n_in]
+        apart.copy_(kernel.t())
+        for far in (kernel, apart.t()):
+            y, slope = layers.dense(x, far, activation="tanh", want_slope=True)
+            clean = layers.dense(x.clone(), kernel.clone(), activation="tanh", want_slope=True)
+            want = plain.dense(x, kernel, None, None, "tanh", 1.0, dy, dtype)
+            plain.agrees(y, want["y"], "y")
+            assert torch.equal(slope, clean[1]) or far is not kernel
+            for name, got in zip(("dx", "dkernel", "dbias"), layers.dense_backward(dy, x, far, slope)):
+                plain.agrees(got, want[name], name)
+
+
 # ---- layer norm --------------------------------------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)

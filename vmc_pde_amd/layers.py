@@ -94,15 +94,21 @@ def _agrees(t, name, dtype, index):
     _plain(t)
 
 
-def _rows(t, cols, name):
-    """(tensor, row pitch) of t as a matrix of `cols` columns whose rows' elements lie behind each other; copied only where no such view exists."""
+def _far(dtype):
+    """Row pitch from which on the dense kernels, whose offsets within a tile have 31 bits, do not take a matrix."""
+    return 1 << (21 if dtype == torch.float64 else 22)
+
+
+def _rows(t, cols, name, far=None):
+    """(tensor, row pitch) of t as a matrix of `cols` columns whose rows' elements lie behind each other, less than `far` apart; copied only where no such
+    view exists."""
     if t.dim() == 0 or t.shape[-1] != cols:
         raise ValueError(f"{name} has shape {tuple(t.shape)}: its last axis should have {cols}")
     t = t.resolve_neg()
     if t.is_contiguous():
         return t, cols
     m = t.reshape(-1, cols)
-    if cols > 1 and m.stride(1) != 1 or m.shape[0] > 1 and m.stride(0) < cols:
+    if cols > 1 and m.stride(1) != 1 or m.shape[0] > 1 and (m.stride(0) < cols or far and m.stride(0) >= far > cols):
         return m.contiguous(), cols
     return m, m.stride(0) if m.shape[0] > 1 else cols
 
@@ -120,11 +126,11 @@ def _kernel_layout(kernel):
     if n_in == 0 or n_out == 0:
         raise ValueError(f"kernel has shape {(n_in, n_out)}: no axis may be empty")
     kernel = kernel.resolve_neg()
-    s0, s1 = kernel.stride()
-    if (s1 == 1 or n_out == 1) and (s0 >= n_out or n_in == 1):
-        return kernel, n_in, n_out, max(s0, n_out), 0
-    if (s0 == 1 or n_in == 1) and (s1 >= n_in or n_out == 1):
-        return kernel, n_in, n_out, max(s1, n_in), 1
+    (s0, s1), far = kernel.stride(), _far(kernel.dtype)
+    if (s1 == 1 or n_out == 1) and (n_out <= s0 < far or n_in == 1):
+        return kernel, n_in, n_out, s0 if n_in > 1 else n_out, 0
+    if (s0 == 1 or n_in == 1) and (n_in <= s1 < far or n_out == 1):
+        return kernel, n_in, n_out, s1 if n_out > 1 else n_in, 1
     return kernel.contiguous(), n_in, n_out, n_out, 0
 
 
@@ -133,7 +139,7 @@ def dense(x, kernel, bias=None, *, activation="none", scale=1.0, residual=None, 
 
     x (..., n_in); kernel (n_in, n_out), the layout of the flat parameter vector's leaves, or a transposed view of an (n_out, n_in) one; bias
     (n_out,); residual of y's shape.  activation: "none", "tanh", "gelu" (z Phi(z)), "silu".  `scale` is the output factor of the reference's
-    conditioners (net.py:50, 61: 10 * tanh).  Widths and row pitches are below 2^22 (2^21 in fp64).  With `want_slope` returns (y, slope): act'(z),
+    conditioners (net.py:50, 61: 10 * tanh).  Widths are below 2^22 (2^21 in fp64); rows that lie further apart are copied.  With `want_slope` returns (y, slope): act'(z),
     which `dense_backward` takes (None for "none"), of the type SLOPE[x.dtype] (fp16 for bf16, fp32 for fp16, else the element type)."""
     calls = _calls()
     if calls is not None:
@@ -157,7 +163,7 @@ def dense(x, kernel, bias=None, *, activation="none", scale=1.0, residual=None, 
         raise ValueError(f"activation {activation!r}: one of {sorted(ACTIVATION)} is needed")
     kernel, n_in, n_out, ldk, kernel_t = _kernel_layout(kernel)
     shape, device = (*x.shape[:-1], n_out), x.device
-    x, ldx = _rows(x, n_in, "x")
+    x, ldx = _rows(x, n_in, "x", _far(dtype))
     if bias is not None:
         _same_shape(bias, (n_out,), "bias")
         bias = bias.resolve_neg().contiguous()
@@ -198,8 +204,8 @@ def dense_backward(dy, x, kernel, slope=None, *, scale=1.0, want_x=True, want_ke
     x_shape, device = x.shape, x.device
     shape = (*x_shape[:-1], n_out)
     _same_shape(dy, shape, "dy")
-    x, ldx = _rows(x, n_in, "x")
-    dy, ldd = _rows(dy, n_out, "dy")
+    x, ldx = _rows(x, n_in, "x", _far(dtype))
+    dy, ldd = _rows(dy, n_out, "dy", _far(dtype))
     if slope is not None:
         _agrees(slope, "slope", SLOPE[dtype], index)
         _same_shape(slope, shape, "slope")
