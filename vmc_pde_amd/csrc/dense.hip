@@ -242,6 +242,9 @@ typedef __attribute__((address_space(3))) short4v lds_short4;
 constexpr int LINE = 128;                 // bytes of k a step: 64 16-bit numbers, 32 fp32, 16 fp64
 constexpr int OUTSIDE = 0x7ffffff0;       // byte offset behind every record: such a lane reads zeros
 template <typename T> constexpr int step_of() { return LINE / (int)sizeof(T); }
+// buffers of a BM x BN tile: two; four where a step is shorter than a fetch (16-bit small tiles: 10000 x 1024 x 1024 of fp32 lost a tenth to the CU's fewer workgroups)
+constexpr int stages_of(int size, int bm, int bn) { return bm * bn >= 128 * 128 || (size > 2 && bm * bn >= 64 * 64) ? 2 : 4; }
+constexpr int tile_lds(int size, int bm, int bn) { return stages_of(size, bm, bn) * (bm + bn) * LINE; }
 
 // What a lane holds of 16 rows: 16 bytes, E numbers behind each other in k; four groups of 16 lanes hold 4 E of them.  One instruction of 32 k for
 // the 16-bit types; fp32 and fp64 instructions take four k, one of each group, so E of them take the numbers one by one.
@@ -385,9 +388,9 @@ __device__ __forceinline__ void tile_product(const Product& g, int row0, int col
   constexpr int THREADS = 64 * WM * WN, TM = BM / WM / 16, TN = BN / WN / 16, STEP = step_of<T>();
   typedef Tile<T, BM, PX, THREADS> P;
   typedef Tile<T, BN, QX, THREADS> Q;
-  // buffers: two; four where a step is shorter than a fetch (16-bit small tiles: 10000 x 1024 x 1024 of fp32 lost a tenth to the CU's fewer workgroups)
-  constexpr int STAGES = BM * BN >= 128 * 128 || (sizeof(T) > 2 && BM * BN >= 64 * 64) ? 2 : 4;
+  constexpr int STAGES = stages_of(sizeof(T), BM, BN);
   __shared__ __attribute__((aligned(16))) char tiles[STAGES * (P::BYTES + Q::BYTES)];
+  static_assert(sizeof(tiles) == tile_lds(sizeof(T), BM, BN), "what the plans reckon with");
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const int wr = (wave / WN) * TM * 16, wc = (wave % WN) * TN * 16;
   P p;
@@ -1072,15 +1075,21 @@ __global__ __launch_bounds__(THIN_THREADS) void thin_backward_kernel(const T* __
 struct Tiles { int bm, bn, slices, slice_steps; };
 
 // What a step of k costs a CU in microseconds, by type and square tile: alone (its fetches and barrier), and each of several workgroups that share the CU
-// (the matrix pipe).  Measured on products of 512 to 10 000 rows; `held`: workgroups a CU holds.
+// (the matrix pipe).  `held`: workgroups a CU holds, by its LDS (64-wide 16-bit tiles: 64 KB each) or, for fp32 and fp64, its registers.  Measured as the difference of
+// products of 96 and 32 steps with one to eight tiles a CU: 64-wide bf16 tiles 0.34, 0.42, 0.70, 0.83 us for one to four, 128-wide 0.71, 0.85, 1.53, 1.74, 256-wide 1.46, 2.96,
+// fp32 0.68, 1.07, 1.53, 1.97, 3.00 for one to five, fp64 0.64, 1.08, 1.58, 2.15.
 struct Cost { int side, held; double alone, each; };
-constexpr Cost HALF_COSTS[] = {{64, 4, 0.5, 0.2}, {128, 2, 0.75, 0.48}, {256, 1, 1.6, 1.7}};
+constexpr Cost HALF_COSTS[] = {{64, 2, 0.34, 0.21}, {128, 2, 0.71, 0.43}, {256, 1, 1.46, 1.48}};
 constexpr Cost F32_COST = {64, 4, 0.65, 0.5}, F64_COST = {64, 4, 0.7, 0.55};
+constexpr int CU_LDS = 160 * 1024;
+constexpr bool fits(const Cost& c, int size) { return c.held * tile_lds(size, c.side, c.side) <= CU_LDS; }
+static_assert(fits(HALF_COSTS[0], 2) && fits(HALF_COSTS[1], 2) && fits(HALF_COSTS[2], 2) && fits(F32_COST, 4) && fits(F64_COST, 8), "a CU's LDS holds what the costs say");
 
 // Tile and k slices of a product of `steps` steps of k.  Sides of at most 32 rows or columns take 32, so that little is multiplied for nothing: those read
 // one long operand once, and the k range is cut until two workgroups a CU do.  Everything else takes the tile and the number of slices of the least
-// estimated time: the steps of the fullest CU, and with slices a second launch that reads and joins their sums (5 us, of which the host takes most, and their bytes at 4 TB/s).  The
-// estimate finds the best choice, or one within 15 % of it, for the 27 shapes that it was made from (three types, 0.1 to 140 GFLOP).
+// estimated time: the steps of the fullest CU, and with slices a second launch that reads and joins their sums (5 us, of which the host takes most, and their bytes at 4 TB/s).  Of 45
+// shapes (three types, 0.05 to 140 GFLOP) it finds the best choice, or one within 10 % of it, for 43; 1537 x 776 x 1000 of fp32 is off by 18 %, 256 x 256 x 65536 of bf16, which is
+// bound by reading, by 22 %.
 template <typename T>
 Tiles tiles_of(int64_t m, int64_t n, int64_t steps) {
   Tiles best = {m <= 32 ? 32 : 128, n <= 32 ? 32 : 128, 1, 0};
