@@ -431,7 +431,7 @@ enum { VMCPDE_ACT_NONE = 0, VMCPDE_ACT_TANH = 1, VMCPDE_ACT_GELU = 2 /* z Phi(z)
 
 /* y = scale * act(x W + b) + r for x [rows][n_in], W [n_in][n_out] (net.py:55-56: the kernel's layout in the flat parameter vector), or
  * stored [n_out][n_in] with kernel_t != 0.  b, r, slope may be NULL.  slope [rows][n_out] receives act'(x W + b) for the backward pass:
- * fp16 for bf16, fp32 for fp16, else the element type.
+ * fp16 for bf16 (slopes under 2^-25 become zero), fp32 for fp16, else the element type.
  * Backward, with dz = scale * slope * dy (slope NULL: 1):  dx = dz W^T [rows][n_in], dkernel = x^T dz [n_in][n_out] (this order whatever
  * kernel_t), dbias = sum of dz over the rows; each may be NULL = not wanted, x may be NULL without dkernel, kernel without dx.  The
  * residual's gradient is dy.  slope * dy is rounded to the element type, in which the matrix pipe takes it; the scale is applied to the sums,

@@ -11,8 +11,10 @@ typedef _Float16 f16_t;
 // Arithmetic type of an element type: sums, statistics and epilogues of 16-bit elements are held in fp32, of fp64 in fp64.
 template <typename T> struct Wide { typedef float type; };
 template <> struct Wide<double> { typedef double type; };
-// act'(z) kept between the passes, finer than the element type: fp16 for bf16, fp32 for fp16.  Every slope lies in [-0.13, 1.13]; rounded to the
-// element type itself it would add an error as large as the output's own rounding to every gradient.
+// act'(z) kept between the passes: fp16 for bf16, fp32 for fp16.  Every slope lies in [-0.13, 1.13]; rounded to the element type itself it would add an
+// error as large as the output's own rounding to every gradient.  fp16 is finer than bf16 for slopes above 2^-16; below, its steps are 2^-24, and a slope under 2^-25
+// is kept as zero: a bf16 tanh unit passes no gradient beyond |z| = 9.4 (where its output, rounded, has been +-1 since 3.5).  fp32 would keep those, for four bytes more
+// an element written and read (8192 x 8192 x 4096: some 26 us of 1360).
 template <typename T> struct Slope { typedef T type; };
 template <> struct Slope<bf16_t> { typedef f16_t type; };
 template <> struct Slope<f16_t> { typedef float type; };

@@ -140,7 +140,8 @@ def dense(x, kernel, bias=None, *, activation="none", scale=1.0, residual=None, 
     x (..., n_in); kernel (n_in, n_out), the layout of the flat parameter vector's leaves, or a transposed view of an (n_out, n_in) one; bias
     (n_out,); residual of y's shape.  activation: "none", "tanh", "gelu" (z Phi(z)), "silu".  `scale` is the output factor of the reference's
     conditioners (net.py:50, 61: 10 * tanh).  Widths are below 2^22 (2^21 in fp64); rows that lie further apart are copied.  With `want_slope` returns (y, slope): act'(z),
-    which `dense_backward` takes (None for "none"), of the type SLOPE[x.dtype] (fp16 for bf16, fp32 for fp16, else the element type)."""
+    which `dense_backward` takes (None for "none"), of the type SLOPE[x.dtype] (fp16 for bf16, where slopes under 2^-25 become zero; fp32 for fp16, else the element
+    type)."""
     calls = _calls()
     if calls is not None:
         device = _device()

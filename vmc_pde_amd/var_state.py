@@ -143,7 +143,10 @@ class VarState:
 
     # ---- var_state.py:36-64 -----------------------------------------------------------------------------------
     def __call__(self, coords, mode="eval", avg=False, max_norm=None):
-        """`max_norm` (with mode="costfun", avg=True): the averaged gradient clipped to that 2-norm (`layers.clip_by_global_norm`)."""
+        """`max_norm` (with mode="costfun", avg=True): the averaged gradient clipped to that 2-norm (`layers.clip_by_global_norm`).
+
+        The average, and with it the clipping, is over the samples given here.  Ranks that hold samples of their own and average their gradients want the
+        clipped mean, not the mean of clipped ones: leave `max_norm` out, average, and clip what comes of it with `layers.clip_by_global_norm`."""
         if max_norm is not None and not (mode == "costfun" and avg):
             raise ValueError('max_norm clips the averaged gradient: it needs mode="costfun" and avg=True')
         if mode == "eval":
