@@ -5,6 +5,7 @@
 // Nothing is decided here: whatever is not plain (another device, layouts that need a copy, arguments that have to be refused) returns
 // None before anything is launched, and vmc_pde_amd/layers.py, which can do all of it, handles or refuses the call.  What fails behind that is raised: made a second time,
 // clipping in place would clip what is clipped already.
+#include <torch/csrc/autograd/forward_grad.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <ATen/ops/empty.h>
 #include <c10/core/GradMode.h>
@@ -55,8 +56,9 @@ struct Arguments {
   PyObject* const* given;
   const Py_ssize_t count;
   const int64_t device;
-  const bool recording;
-  Arguments(PyObject* const* a, Py_ssize_t n, Py_ssize_t wanted) : given(a), count(n), device(n == wanted ? PyLong_AsLongLong(a[n - 2]) : -1), recording(c10::GradMode::is_enabled()) {
+  const bool recording, tangents;      // tangents: whether a forward-mode level (there is only the first) is entered, outside of which no tensor has one
+  Arguments(PyObject* const* a, Py_ssize_t n, Py_ssize_t wanted) : given(a), count(n), device(n == wanted ? PyLong_AsLongLong(a[n - 2]) : -1), recording(c10::GradMode::is_enabled()),
+                                                                      tangents(torch::autograd::ForwardADLevel::try_get_by_idx(0) != nullptr) {
     need(n == wanted && device >= 0);
   }
   void* stream() const { return PyLong_AsVoidPtr(given[count - 1]); }
@@ -66,7 +68,7 @@ struct Arguments {
     need(THPVariable_Check(p));
     const at::Tensor& t = THPVariable_Unpack(p);
     need(t.defined() && t.layout() == at::kStrided && t.is_cuda() && t.get_device() == device && !t.is_neg() && !(written && recording && t.requires_grad()) &&
-         !t._fw_grad(/* level */ 0).defined());
+         !(tangents && t._fw_grad(/* level */ 0).defined()));
     return t;
   }
   const at::Tensor* tensor_or_none(int k) const { return given[k] == Py_None ? nullptr : &tensor(k); }
@@ -350,15 +352,12 @@ PyObject* global_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
     need(count < (1 << 30));
     std::vector<vmcpde_tensor> table((size_t)count);
     at::TensorOptions options;
-    std::vector<at::Tensor> written;          // (held: other threads may change the lists while the interpreter is released)
-    if (clip) written.reserve((size_t)count);
     for (Py_ssize_t k = 0; k < count; ++k) {
       const at::Tensor& t = in.checked(PyList_GET_ITEM(tensors, k), clip && own);
       const at::Tensor& o = own ? t : in.checked(PyList_GET_ITEM(out, k), clip);
       need(t.is_contiguous() && (own || (o.is_contiguous() && o.sizes() == t.sizes() && o.scalar_type() == t.scalar_type())));
       table[(size_t)k] = {t.data_ptr(), o.data_ptr(), t.numel(), code_of(t.scalar_type()), 0};
       if (k == 0) options = t.options();
-      if (clip) written.push_back(o);
     }
     const double max_norm = clip ? in.number(2) : 0.0;
     const at::Tensor norm = at::empty({}, options.dtype(at::kDouble));
@@ -367,9 +366,14 @@ PyObject* global_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
     void* stream = in.stream();
     double* to = static_cast<double*>(norm.data_ptr());
     call("vmcpde_global_norm", [&] { return entry.global_norm(table.data(), (int32_t)count, clip, max_norm, to, space.p, bytes, stream); });
-    if (clip)                                 // written in place: a recorded graph that saved one of these has to see it
-      for (const at::Tensor& t : written)
-        if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+    if (clip) {                               // written in place: a recorded graph that saved one of these has to see it
+      PyObject* const written = own ? tensors : out;
+      for (Py_ssize_t k = 0; k < PyList_GET_SIZE(written); ++k)      // (looked at anew: another thread may have changed the list meanwhile)
+        if (THPVariable_Check(PyList_GET_ITEM(written, k))) {
+          const at::Tensor& t = THPVariable_Unpack(PyList_GET_ITEM(written, k));
+          if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+        }
+    }
     return wrap(norm);
   });
 }
