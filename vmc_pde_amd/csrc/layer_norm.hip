@@ -5,7 +5,7 @@
 // Bound by memory.  A row is read once and stays in registers (fp32, fp64 rows in fp64).  A first mean is taken, then the deviations from it: their own mean is what the
 // first one is off by, which for a row far from zero is many times the last place of its deviations, and is taken off again (fp32 columns of unit spread around
 // 1e5: y off by 4.5e-7, without it by 9e-3; the backward pass takes the mean as it is stored, rounded to its type).  That costs up to 4 % of a forward pass of 16-bit
-// elements and 0.9 of 7.1 us for 65 536 x 21 of fp64.  16, 64, 256 or 1024 lanes share a row, so that a lane holds at most four 16-byte
+// elements and 0.4 of 7.1 us for 65 536 x 21 of fp64.  16, 64, 256 or 1024 lanes share a row, so that a lane holds at most four 16-byte
 // vectors; longer rows go through the kernels that read them again.  Loads and stores are 16 bytes a lane at any
 // alignment (global memory takes them unaligned).  A row's last, partial vector is moved back to end with the row: it repeats columns of the lane before,
 // which it leaves out of the row's sums and otherwise computes and writes a second time, with the same result.  So a row is loaded without a branch, and
@@ -147,7 +147,7 @@ __global__ __launch_bounds__(THREADS) void norm_forward_kernel(const T* __restri
         q[1] += d;
       }
     row_sum<LANES>(q, sh[turn][1]);
-    const A off = q[1] * inv, rstd = reciprocal_root<A>(variance(q[0] / (A)cols, off) + eps), less = -off * rstd;
+    const A off = q[1] * inv, rstd = reciprocal_root<A>(variance(q[0] * inv, off) + eps), less = -off * rstd;
     if (GROUPS > 1 && row >= rows) continue;   // (a whole group of lanes; the sums above need every lane of a wave)
     if (lane == 0 && mean_out) {
       mean_out[row] = mean + off;
@@ -433,6 +433,7 @@ __global__ __launch_bounds__(256) void norm_forward_narrow_kernel(const T* __res
                                                                   typename Wide<T>::type* __restrict__ mean_out, typename Wide<T>::type* __restrict__ rstd_out) {
   typedef typename Wide<T>::type A;
   constexpr int MOST = vec_of<T>() - 1;
+  const A inv = (A)1 / (A)cols;
   A w[MOST], b[MOST];
 #pragma unroll
   for (int k = 0; k < MOST; ++k) {
@@ -453,8 +454,8 @@ __global__ __launch_bounds__(256) void norm_forward_narrow_kernel(const T* __res
       q += d * d;
       off += d;
     }
-    off /= (A)cols;
-    const A rstd = reciprocal_root<A>(variance(q / (A)cols, off) + eps);
+    off *= inv;
+    const A rstd = reciprocal_root<A>(variance(q * inv, off) + eps);
     if (mean_out) {
       mean_out[row] = mean + off;
       rstd_out[row] = rstd;
