@@ -106,14 +106,16 @@ __device__ __forceinline__ Factor clip_factor(double norm, double max_norm) {
   const double mn = frexp(norm, &en), mm = frexp(max_norm, &em);
   return {0.5 * mm / mn, em - en + 1};
 }
-template <typename T, typename A>
+template <bool FAR = true, typename T, typename A>
 __device__ __forceinline__ T scaled(T v, A f, int e) {
   const A r = (A)v * f;
-  if constexpr (sizeof(A) == 8) return (T)ldexp(r, e);
+  if constexpr (!FAR) return (T)r;
+  else if constexpr (sizeof(A) == 8) return (T)ldexp(r, e);
   else return (T)ldexpf(r, e);
 }
 
-template <typename T>
+// FAR: e is not 0 (asked once: with its power of two for every element 1 GB clipped took 558 us, not 550)
+template <bool FAR, typename T>
 __device__ void scale_span(const T* p, T* o, int64_t n, int t, int threads, Factor factor) {
   typedef typename Wide<T>::type A;
   constexpr int V = vec_of<T>();
@@ -130,17 +132,17 @@ __device__ void scale_span(const T* p, T* o, int64_t n, int t, int threads, Fact
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
 #pragma unroll
-      for (int k = 0; k < V; ++k) r[u].v[k] = scaled(r[u].v[k], f, e);
+      for (int k = 0; k < V; ++k) r[u].v[k] = scaled<FAR>(r[u].v[k], f, e);
       __builtin_nontemporal_store(__builtin_bit_cast(uint4v, r[u]), reinterpret_cast<uint4v*>(w + j + u * threads));
     }
   }
   for (; j < vecs; j += threads) {
     Raw<T> r = q[j];
 #pragma unroll
-    for (int k = 0; k < V; ++k) r.v[k] = scaled(r.v[k], f, e);
+    for (int k = 0; k < V; ++k) r.v[k] = scaled<FAR>(r.v[k], f, e);
     w[j] = r;
   }
-  if (tail + t < n) o[tail + t] = scaled(p[tail + t], f, e);
+  if (tail + t < n) o[tail + t] = scaled<FAR>(p[tail + t], f, e);
 }
 
 __device__ void square_any(const Entry& e, int64_t at, int64_t n, int t, int threads, Bins& b) {
@@ -152,12 +154,19 @@ __device__ void square_any(const Entry& e, int64_t at, int64_t n, int t, int thr
   }
 }
 
+template <typename T>
+__device__ __forceinline__ void scale_typed(const Entry& e, int64_t at, int64_t n, int t, int threads, Factor factor) {
+  const T* p = static_cast<const T*>(e.in) + at;
+  T* o = static_cast<T*>(e.out) + at;
+  if (factor.e) scale_span<true>(p, o, n, t, threads, factor);
+  else scale_span<false>(p, o, n, t, threads, factor);
+}
 __device__ void scale_any(const Entry& e, int64_t at, int64_t n, int t, int threads, Factor factor) {
   switch (e.dtype) {
-    case VMCPDE_F64: scale_span(static_cast<const double*>(e.in) + at, static_cast<double*>(e.out) + at, n, t, threads, factor); break;
-    case VMCPDE_F32: scale_span(static_cast<const float*>(e.in) + at, static_cast<float*>(e.out) + at, n, t, threads, factor); break;
-    case VMCPDE_F16: scale_span(static_cast<const f16_t*>(e.in) + at, static_cast<f16_t*>(e.out) + at, n, t, threads, factor); break;
-    default: scale_span(static_cast<const bf16_t*>(e.in) + at, static_cast<bf16_t*>(e.out) + at, n, t, threads, factor);
+    case VMCPDE_F64: scale_typed<double>(e, at, n, t, threads, factor); break;
+    case VMCPDE_F32: scale_typed<float>(e, at, n, t, threads, factor); break;
+    case VMCPDE_F16: scale_typed<f16_t>(e, at, n, t, threads, factor); break;
+    default: scale_typed<bf16_t>(e, at, n, t, threads, factor);
   }
 }
 

@@ -12,7 +12,7 @@
 // the next row's loads fly while one is reduced.
 // The weights' gradients: every workgroup takes every gridDim-th group of rows and adds its columns in registers; the workgroups' sums are
 // added in index order by a second launch -- no atomics, the same bits every time.
-// 16384 x 8192 of bf16: 94 us, 150 us backward (5.3 TB/s); 10 000 x 1001 of fp32 16 and 22 us; 65 536 x 21 of fp64 8.5 and 8.5 us.
+// 16384 x 8192 of bf16: 97 us, 150 us backward (5.3 TB/s); 10 000 x 1001 of fp32 16 and 22 us; 65 536 x 21 of fp64 9.0 and 8.5 us.
 #include <algorithm>
 
 #include "layers.hpp"
@@ -172,7 +172,7 @@ __global__ __launch_bounds__(THREADS) void norm_forward_kernel(const T* __restri
 }
 
 // Rows that no 1024 lanes hold: read three times, the second and third time from the caches.  A lane takes four vectors at a time, whose loads fly together
-// (the last one moved back, as above): 4096 x 8200 of fp64 138 us, one after the other 162; the backward pass of 4096 x 20000 of bf16 220, 372.
+// (the last one moved back, as above): 4096 x 8200 of fp64 143 us (one after the other it lost 24); the backward pass of 4096 x 20000 of bf16 220, 372.
 template <int V, typename F>
 __device__ __forceinline__ void wide_row(int64_t cols, F f) {
   for (int64_t first = (int64_t)threadIdx.x * V; first < cols; first += 4 * 1024 * V) {
