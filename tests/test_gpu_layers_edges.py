@@ -104,6 +104,21 @@ def test_layer_norm_of_rows_far_from_zero(layers, cols, offset):  # noqa: F811
     plain.agrees(mean, (centre[:, 0], 1.01 * u * centre[:, 0].abs() + (depth + 4) * u * (exact - centre).abs().mean(1)), "mean")
 
 
+@pytest.mark.parametrize("dtype", HALF, ids=HALF_IDS)
+@pytest.mark.parametrize("cols, spread", [(7, 1.0), (100, 1.0), (1000, 1.0), (8192, 1.0), (8192, 20.0), (40000, 1.0)])
+def test_layer_norm_of_16_bit_rows_far_from_zero(layers, dtype, cols, spread):  # noqa: F811
+    """Numbers around 300, in steps of 1/4 (fp16) and 2 (bf16).  As above, but with the first mean as it is, which is off by its own last place and one of a sum that is
+    exact up to 2^13 and 2^16 numbers (beyond, D / 80 more): 4 u |mean| / standard deviation on every y; and the output's rounding."""
+    x = (300 + spread * normal((40, cols), torch.float64, cols)).to(dtype)
+    y, mean, rstd = layers.layer_norm(x, eps=1e-6, want_stats=True)
+    exact = plain.f64(x)
+    centre = exact.mean(1, keepdim=True)
+    want_rstd = 1 / torch.sqrt(((exact - centre) ** 2).mean(1, keepdim=True) + 1e-6)
+    want, u, depth = (exact - centre) * want_rstd, 2.0 ** -24, 80 + cols / 512
+    bound = (want.abs() + 1) * ((3 * depth + 16) * u + 4 * depth / 80 * u * centre.abs() * want_rstd)
+    plain.agrees(y, (want, bound + plain.half_step(dtype) * (want.abs() + bound) + plain.smallest(dtype)), "y")
+
+
 # ---- global norm -------------------------------------------------------------------------------------------------------------------------
 
 def test_global_norm_of_many_large_numbers(layers):  # noqa: F811

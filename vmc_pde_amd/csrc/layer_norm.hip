@@ -4,15 +4,16 @@
 //
 // Bound by memory.  A row is read once and stays in registers (fp32, fp64 rows in fp64).  A first mean is taken, then the deviations from it: their own mean is what the
 // first one is off by, which for a row far from zero is many times the last place of its deviations, and is taken off again (fp32 columns of unit spread around
-// 1e5: y off by 4.5e-7, without it by 9e-3; the backward pass takes the mean as it is stored, rounded to its type).  That costs up to 4 % of a forward pass of 16-bit
-// elements and 0.4 of 7.1 us for 65 536 x 21 of fp64.  16, 64, 256 or 1024 lanes share a row, so that a lane holds at most four 16-byte
+// 1e5: y off by 4.5e-7, without it by 9e-3; the backward pass takes the mean as it is stored, rounded to its type).  That costs 0.4 of 7.1 us for 65 536 x 21 of fp64.
+// 16-bit elements go without: the fp32 sum of 2^13 fp16 or 2^16 bf16 numbers of one binade is exact, the mean off by 2^-24 of it, where the elements' own steps are
+// 2^-11 and 2^-8 of it (with it 16384 x 8192 of bf16, at the clocks of a long run, took 134 us instead of 118).  16, 64, 256 or 1024 lanes share a row, so that a lane holds at most four 16-byte
 // vectors; longer rows go through the kernels that read them again.  Loads and stores are 16 bytes a lane at any
 // alignment (global memory takes them unaligned).  A row's last, partial vector is moved back to end with the row: it repeats columns of the lane before,
 // which it leaves out of the row's sums and otherwise computes and writes a second time, with the same result.  So a row is loaded without a branch, and
 // the next row's loads fly while one is reduced.
 // The weights' gradients: every workgroup takes every gridDim-th group of rows and adds its columns in registers; the workgroups' sums are
 // added in index order by a second launch -- no atomics, the same bits every time.
-// 16384 x 8192 of bf16: 97 us, 150 us backward (5.3 TB/s); 10 000 x 1001 of fp32 16 and 22 us; 65 536 x 21 of fp64 9.0 and 8.5 us.
+// 16384 x 8192 of bf16: 94 us, 150 us backward (5.3 TB/s); 10 000 x 1001 of fp32 16 and 22 us; 65 536 x 21 of fp64 9.0 and 8.5 us.
 #include <algorithm>
 
 #include "layers.hpp"
@@ -24,6 +25,9 @@ namespace {
 template <typename A> __device__ __forceinline__ A reciprocal_root(A v);
 template <> __device__ __forceinline__ float reciprocal_root(float v) { return 1.0f / sqrtf(v); }
 template <> __device__ __forceinline__ double reciprocal_root(double v) { return 1.0 / sqrt(v); }
+
+// whether the deviations' mean is taken off (above)
+template <typename T> constexpr bool refined() { return sizeof(T) > 2; }
 
 // the variance from the mean of the squared deviations from a mean that is off by `off` (rounding may leave less than nothing of it; NaN stays)
 template <typename A>
@@ -102,7 +106,7 @@ __global__ __launch_bounds__(THREADS) void norm_forward_kernel(const T* __restri
                                                                typename Wide<T>::type* __restrict__ mean_out, typename Wide<T>::type* __restrict__ rstd_out) {
   typedef typename Wide<T>::type A;
   constexpr int V = vec_of<T>(), GROUPS = THREADS / LANES, WAVES = THREADS / 64;
-  constexpr bool KEEP = ITER * V <= 16;
+  constexpr bool KEEP = ITER * V <= 16, REFINED = refined<T>();
   __shared__ A sh[2][3][WAVES];                // (two sets of slots in turn: a wave may be a row ahead of the slowest)
   const int lane = threadIdx.x % LANES;
   const A inv = (A)1 / (A)cols;
@@ -126,7 +130,7 @@ __global__ __launch_bounds__(THREADS) void norm_forward_kernel(const T* __restri
   for (int turn = 0; first < rows; turn ^= 1) {
     const int64_t row = first + threadIdx.x / LANES;
     first += (int64_t)gridDim.x * GROUPS;
-    A v[ITER][V], s[1] = {0}, q[2] = {0, 0};
+    A v[ITER][V], s[1] = {0}, q[REFINED ? 2 : 1] = {};
 #pragma unroll
     for (int i = 0; i < ITER; ++i)
 #pragma unroll
@@ -144,10 +148,12 @@ __global__ __launch_bounds__(THREADS) void norm_forward_kernel(const T* __restri
         v[i][k] -= mean;
         const A d = EXACT || k >= at.skip[i] ? v[i][k] : (A)0;
         q[0] += d * d;
-        q[1] += d;
+        if constexpr (REFINED) q[1] += d;
       }
     row_sum<LANES>(q, sh[turn][1]);
-    const A off = q[1] * inv, rstd = reciprocal_root<A>(variance(q[0] * inv, off) + eps), less = -off * rstd;
+    A off = 0;
+    if constexpr (REFINED) off = q[1] * inv;
+    const A rstd = reciprocal_root<A>(variance(q[0] * inv, off) + eps), less = -off * rstd;
     if (GROUPS > 1 && row >= rows) continue;   // (a whole group of lanes; the sums above need every lane of a wave)
     if (lane == 0 && mean_out) {
       mean_out[row] = mean + off;
@@ -165,7 +171,7 @@ __global__ __launch_bounds__(THREADS) void norm_forward_kernel(const T* __restri
         weights_at<W, V>(bias, at.base[i], (A)0, bi);
       }
 #pragma unroll
-      for (int k = 0; k < V; ++k) v[i][k] = fma(v[i][k], rstd, less) * wi[k] + bi[k];
+      for (int k = 0; k < V; ++k) v[i][k] = (REFINED ? fma(v[i][k], rstd, less) : v[i][k] * rstd) * wi[k] + bi[k];
       if (EXACT || at.skip[i] < V) put<T, V>(yr + at.base[i], v[i]);
     }
   }
@@ -197,7 +203,8 @@ __global__ __launch_bounds__(1024) void norm_forward_wide_kernel(const T* __rest
   __shared__ A sh[3][16];
   const int64_t row = blockIdx.x;
   const T* xr = x + row * ldx;
-  A s[1] = {0}, q[2] = {0, 0};
+  constexpr bool REFINED = refined<T>();
+  A s[1] = {0}, q[REFINED ? 2 : 1] = {};
   auto load = [&](const int64_t (&base)[4], Raw<T, V> (&r)[4]) {
 #pragma unroll
     for (int u = 0; u < 4; ++u) r[u] = raw_at<T, V>(xr + base[u]);
@@ -221,11 +228,13 @@ __global__ __launch_bounds__(1024) void norm_forward_wide_kernel(const T* __rest
       for (int k = 0; k < V; ++k) {
         const A d = k >= skip[u] ? (A)r[u].v[k] - mean : (A)0;
         q[0] += d * d;
-        q[1] += d;
+        if constexpr (REFINED) q[1] += d;
       }
   });
   row_sum<1024>(q, sh[1]);
-  const A off = q[1] / (A)cols, rstd = reciprocal_root<A>(variance(q[0] / (A)cols, off) + eps), less = -off * rstd;
+  A off = 0;
+  if constexpr (REFINED) off = q[1] / (A)cols;
+  const A rstd = reciprocal_root<A>(variance(q[0] / (A)cols, off) + eps), less = -off * rstd;
   if (threadIdx.x == 0 && mean_out) {
     mean_out[row] = mean + off;
     rstd_out[row] = rstd;
@@ -239,7 +248,7 @@ __global__ __launch_bounds__(1024) void norm_forward_wide_kernel(const T* __rest
       weights_at<W, V>(weight, base[u], (A)1, w);
       weights_at<W, V>(bias, base[u], (A)0, b);
 #pragma unroll
-      for (int k = 0; k < V; ++k) v[k] = fma((A)r[u].v[k] - mean, rstd, less) * w[k] + b[k];
+      for (int k = 0; k < V; ++k) v[k] = (REFINED ? fma((A)r[u].v[k] - mean, rstd, less) : ((A)r[u].v[k] - mean) * rstd) * w[k] + b[k];
       if (skip[u] < V) put<T, V>(y + row * ldy + base[u], v);
     }
   });
@@ -452,7 +461,7 @@ __global__ __launch_bounds__(256) void norm_forward_narrow_kernel(const T* __res
       v[k] -= mean;
       const A d = k < cols ? v[k] : (A)0;
       q += d * d;
-      off += d;
+      if constexpr (refined<T>()) off += d;
     }
     off *= inv;
     const A rstd = reciprocal_root<A>(variance(q * inv, off) + eps);
