@@ -435,7 +435,8 @@ enum { VMCPDE_ACT_NONE = 0, VMCPDE_ACT_TANH = 1, VMCPDE_ACT_GELU = 2 /* z Phi(z)
  * Backward, with dz = scale * slope * dy (slope NULL: 1):  dx = dz W^T [rows][n_in], dkernel = x^T dz [n_in][n_out] (this order whatever
  * kernel_t), dbias = sum of dz over the rows; each may be NULL = not wanted, x may be NULL without dkernel, kernel without dx.  The
  * residual's gradient is dy.  slope * dy is rounded to the element type, in which the matrix pipe takes it; the scale is applied to the sums,
- * which are fp32 / fp64.  (fp16: slope * dy itself has to stay below 65504; slopes reach 1.13.)  No atomics: the same call gives the same bits.  Rows below 2^30, widths and pitches below 2^22 (2^21 in fp64). */
+ * which are fp32 / fp64.  (fp16: slope * dy itself has to stay below 65504; slopes reach 1.13.)  No atomics: the same call gives the same bits.  Rows below 2^30 (and fewer than 2^24 tiles of 64 x 64 to a
+ * product in fp32 and fp64: rows x n_out, or rows x n_in for dx, below 2^36), widths and pitches below 2^22 (2^21 in fp64). */
 typedef struct {
   int32_t dtype, activation, kernel_t, reserved;
   int64_t rows, n_in, n_out;

@@ -96,6 +96,21 @@ def test_entry_points_bound_by_two_threads(nat, monkeypatch):
     assert len(layers._entry) == 8
 
 
+@pytest.mark.parametrize("dtype, rows, n_in, n_out, backward, fits", [
+    (1, 1 << 29, 8, 128, 0, False), (1, (1 << 29) - 64, 8, 128, 0, True), (0, 1 << 29, 100, 8, 1, False), (0, 1 << 29, 8, 64, 0, True), (3, 1 << 29, 8, 128, 0, True),
+    (3, (1 << 30) - 1, 8, 64, 0, False), (2, (1 << 30) - 1, 8, 32, 0, True)])
+def test_dense_refuses_more_tiles_than_a_launch_takes(nat, dtype, rows, n_in, n_out, backward, fits):
+    """2^24 tiles of 256 lanes: on the host, before the first of the call's launches."""
+    here = 4096      # stands for an address
+    a = nat.DenseArgs(dtype=dtype, activation=0, kernel_t=0, rows=rows, n_in=n_in, n_out=n_out, x=here, ldx=n_in, kernel=here, ldk=n_out, scale=1.0, y=here, ldy=n_out,
+                      dy=here, ldd=n_out, dx=here, dkernel=None, dbias=None)
+    need = nat.lib().vmcpde_dense_workspace_bytes(a, backward)
+    assert (need >= 0) == fits
+    if not fits:
+        run = nat.lib().vmcpde_dense_backward if backward else nat.lib().vmcpde_dense
+        assert run(a, here, 1 << 60, None) == -1 and b"tiles" in nat.lib().vmcpde_last_error()
+
+
 def test_forward_mode_tangents_are_refused_on_the_host():
     from vmc_pde_amd import layers
     x, kernel, stats = torch.zeros(3, 4), torch.zeros(4, 5), torch.zeros(3)

@@ -1243,7 +1243,7 @@ struct Dense {
   char* workspace;
   hipStream_t stream;
   int64_t used = 0, most = 0;
-  bool launch;
+  bool launch, too_many = false;      // too_many: a product's tiles are more than one launch takes
   Jobs<T> jobs;
   Dense(void* w, hipStream_t s, bool l) : workspace(static_cast<char*>(w)), stream(s), launch(l) { jobs.count = jobs.blocks = 0; }
 
@@ -1291,6 +1291,7 @@ struct Dense {
 
   void multiply(const Lines& p, bool p_across, const Lines& q, bool q_across, int64_t m, int64_t n, int64_t k, const Epilogue<T>& e) {
     const Tiles t = plan_of<T>(m, n, k, p_across, q_across, !p_across && few<T>(m, n, k, q_across, fetchable<T>(q)));
+    if (t.bm && ceil_div(m, t.bm) * ceil_div(n, t.bn) * (t.bm == 256 ? 512 : 256) >= (int64_t)1 << 32) too_many = true;      // (a launch has 2^32 lanes along an axis)
     const int64_t bytes = product_bytes<T>(t, m, n);
     void* rest = bytes ? take(bytes) : nullptr;
     if (launch) product<T>({p.p, q.p, p.ld, q.ld, (int32_t)m, (int32_t)n, (int32_t)k}, p_across, q_across, t, e, rest, stream);
@@ -1397,13 +1398,13 @@ struct Dense {
   }
 };
 
-// the bytes of workspace that the call needs; `launch`: the call itself
+// the bytes of workspace that the call needs, -1: more tiles than a launch takes; `launch`: the call itself
 template <typename T>
 int64_t walk(const vmcpde_dense_args& a, bool backward, void* workspace, hipStream_t s, bool launch) {
   Dense<T> d(workspace, s, launch);
   if (backward) d.backward(a);
   else d.forward(a);
-  return d.most;
+  return d.too_many ? -1 : d.most;
 }
 
 int64_t walk_type(const vmcpde_dense_args& a, bool backward, void* workspace, hipStream_t s, bool launch) {
@@ -1446,13 +1447,17 @@ extern "C" {
 
 int64_t vmcpde_dense_workspace_bytes(const vmcpde_dense_args* a, int32_t backward) {
   if (check(a, backward != 0)) return -1;
-  return walk_type(*a, backward != 0, nullptr, nullptr, false);
+  const int64_t bytes = walk_type(*a, backward != 0, nullptr, nullptr, false);
+  VMC_REQUIRE(bytes >= 0, "dense: rows %lld, n_in %lld, n_out %lld: a product of 2^24 tiles and more (64 x 64 in fp32 and fp64)", (long long)a->rows, (long long)a->n_in,
+              (long long)a->n_out);
+  return bytes;
 }
 
 static int run(const vmcpde_dense_args* a, bool backward, void* workspace, int64_t workspace_bytes, void* stream) {
   if (const int rc = check(a, backward)) return rc;
   if (!backward && a->rows == 0) return 0;
   const int64_t need = vmcpde_dense_workspace_bytes(a, backward);
+  if (need < 0) return -1;
   VMC_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), "dense: workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)need);
   VMC_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "dense: the workspace is not aligned to 16 bytes");
   walk_type(*a, backward, workspace, static_cast<hipStream_t>(stream), true);
